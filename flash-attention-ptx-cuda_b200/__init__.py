@@ -33,6 +33,9 @@ FA_ERR_NOT_SM100 = -7
 FA_ERR_NCCL = -8
 FA_DTYPE_F16, FA_DTYPE_BF16, FA_DTYPE_E4M3 = 0, 1, 2
 DTYPES = {"f16": FA_DTYPE_F16, "bf16": FA_DTYPE_BF16, "e4m3": FA_DTYPE_E4M3}
+FA_CACHE_16BIT, FA_CACHE_E4M3, FA_CACHE_U4 = 0, 1, 2
+CACHES = {"f16": FA_CACHE_16BIT, "bf16": FA_CACHE_16BIT, "e4m3": FA_CACHE_E4M3, "u4": FA_CACHE_U4}
+ROPE_SCALINGS = {"plain": 0, "linear": 1, "base": 2, "parts": 3, "smooth": 4}
 
 # Every symbol include/fa_b200.h declares; the CPU-only tests check they all resolve.
 EXPORTED_SYMBOLS = (
@@ -43,6 +46,7 @@ EXPORTED_SYMBOLS = (
     "fa_clear_device_status", "fa_error_string", "fa_last_cuda_error", "fa_version",
     "fa_set_prefill_variant", "fa_combine_packed", "fa_decode_kv_sharded", "fa_decode_kv_sharded_gather_bytes",
     "fa_nccl_unique_id", "fa_nccl_comm_create", "fa_nccl_comm_destroy", "fa_status_word_to_error",
+    "fa_rope", "fa_rope_inv_freq", "fa_cache_append", "fa_cache_read_u4",
 )
 
 
@@ -100,6 +104,73 @@ class BackwardArgs(ctypes.Structure):
         ("batch_size", ctypes.c_int), ("num_heads", ctypes.c_int), ("seq_len", ctypes.c_int),
         ("d_head", ctypes.c_int), ("scale", ctypes.c_float), ("causal", ctypes.c_int), ("dtype", ctypes.c_int),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
+    ]
+
+
+class Rotary(ctypes.Structure):
+    """Mirror of ``fa_rotary`` (include/fa_b200.h)."""
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("rotary_dim", ctypes.c_int), ("interleaved", ctypes.c_int),
+                ("amplitude", ctypes.c_float)]
+
+
+class Strides(ctypes.Structure):
+    """Mirror of ``fa_strides`` (include/fa_b200.h)."""
+    _fields_ = [("batch", ctypes.c_longlong), ("head", ctypes.c_longlong), ("row", ctypes.c_longlong)]
+
+
+class RopeArgs(ctypes.Structure):
+    """Mirror of ``fa_rope_args`` (include/fa_b200.h)."""
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
+        ("q_strides", Strides), ("k_strides", Strides), ("q_out_strides", Strides), ("k_out_strides", Strides),
+        ("batch_size", ctypes.c_int), ("num_q_heads", ctypes.c_int), ("num_kv_heads", ctypes.c_int),
+        ("seq_len", ctypes.c_int), ("d_head", ctypes.c_int), ("dtype", ctypes.c_int),
+        ("positions", ctypes.c_void_p), ("positions_stride", ctypes.c_int), ("position_offset", ctypes.c_int),
+        ("inverse", ctypes.c_int), ("rotary", Rotary), ("stream", ctypes.c_void_p),
+    ]
+
+
+class RopeScaling(ctypes.Structure):
+    """Mirror of ``fa_rope_scaling`` (include/fa_b200.h)."""
+    _fields_ = [("kind", ctypes.c_int), ("base", ctypes.c_double), ("factor", ctypes.c_double),
+                ("original_length", ctypes.c_double), ("slow", ctypes.c_double), ("fast", ctypes.c_double)]
+
+
+class CacheLayout(ctypes.Structure):
+    """Mirror of ``fa_cache_layout`` (include/fa_b200.h)."""
+    _fields_ = [
+        ("block_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong), ("row_stride", ctypes.c_longlong),
+        ("param_block_stride", ctypes.c_longlong), ("param_head_stride", ctypes.c_longlong),
+        ("param_row_stride", ctypes.c_longlong),
+        ("block_table", ctypes.c_void_p), ("block_table_stride", ctypes.c_int), ("page_size", ctypes.c_int),
+        ("num_pages", ctypes.c_int), ("seq_lens", ctypes.c_void_p),
+    ]
+
+
+class CacheAppendArgs(ctypes.Structure):
+    """Mirror of ``fa_cache_append_args`` (include/fa_b200.h)."""
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
+        ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p), ("k_params", ctypes.c_void_p),
+        ("v_params", ctypes.c_void_p),
+        ("q_token_stride", ctypes.c_longlong), ("k_token_stride", ctypes.c_longlong), ("v_token_stride", ctypes.c_longlong),
+        ("batch_size", ctypes.c_int), ("num_tokens", ctypes.c_int), ("num_q_heads", ctypes.c_int),
+        ("num_kv_heads", ctypes.c_int), ("seq_len_kv", ctypes.c_int), ("d_head", ctypes.c_int),
+        ("dtype", ctypes.c_int), ("cache", ctypes.c_int), ("layout", CacheLayout),
+        ("num_new", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("rotary", Rotary),
+        ("q_scale", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class CacheReadArgs(ctypes.Structure):
+    """Mirror of ``fa_cache_read_args`` (include/fa_b200.h)."""
+    _fields_ = [
+        ("k_cache", ctypes.c_void_p), ("k_params", ctypes.c_void_p), ("v_cache", ctypes.c_void_p),
+        ("v_params", ctypes.c_void_p), ("k_out", ctypes.c_void_p), ("v_out", ctypes.c_void_p),
+        ("batch_size", ctypes.c_int), ("num_kv_heads", ctypes.c_int), ("seq_len_kv", ctypes.c_int),
+        ("d_head", ctypes.c_int), ("num_rows", ctypes.c_int), ("dtype", ctypes.c_int), ("layout", CacheLayout),
+        ("first_rows", ctypes.c_void_p), ("stream", ctypes.c_void_p),
     ]
 
 
@@ -173,6 +244,15 @@ def lib() -> ctypes.CDLL:
         l.fa_status_word_to_error.argtypes = [ctypes.c_int]
         l.fa_set_prefill_variant.restype = ctypes.c_int
         l.fa_set_prefill_variant.argtypes = [ctypes.c_int]
+        l.fa_rope.restype = ctypes.c_int
+        l.fa_rope.argtypes = [ctypes.POINTER(RopeArgs)]
+        l.fa_rope_inv_freq.restype = ctypes.c_int
+        l.fa_rope_inv_freq.argtypes = [ctypes.POINTER(RopeScaling), ctypes.c_int, ctypes.POINTER(ctypes.c_double),
+                                       ctypes.POINTER(ctypes.c_float)]
+        l.fa_cache_append.restype = ctypes.c_int
+        l.fa_cache_append.argtypes = [ctypes.POINTER(CacheAppendArgs)]
+        l.fa_cache_read_u4.restype = ctypes.c_int
+        l.fa_cache_read_u4.argtypes = [ctypes.POINTER(CacheReadArgs)]
         _lib = l
     return _lib
 
@@ -309,6 +389,92 @@ def backward(*args, **kw) -> None:
     rc = backward_raw(*args, **kw)
     if rc != FA_OK:
         raise FaError(rc, "fa_backward")
+
+
+def _rotary(inv_freq, rotary_dim, interleaved, amplitude) -> Rotary:
+    """``inv_freq``: doubles in host memory - a CPU tensor, a ctypes array or an address."""
+    if isinstance(inv_freq, ctypes.Array):
+        inv_freq = ctypes.addressof(inv_freq)
+    return Rotary(_ptr(inv_freq), rotary_dim, int(interleaved), amplitude)
+
+
+def rope_inv_freq(rotary_dim, base=10000.0, scaling="plain", factor=1.0, original_length=0.0, slow=0.0, fast=0.0):
+    """fa_rope_inv_freq: (ctypes array of rotary_dim / 2 doubles, amplitude).  ``scaling``: "plain", "linear", "base",
+    "parts" or "smooth"."""
+    sc = RopeScaling(ROPE_SCALINGS[scaling], base, factor, original_length, slow, fast)
+    out = (ctypes.c_double * max(1, rotary_dim // 2))()
+    amp = ctypes.c_float(1.0)
+    rc = lib().fa_rope_inv_freq(ctypes.byref(sc), rotary_dim, out, ctypes.byref(amp))
+    if rc != FA_OK:
+        raise FaError(rc, "fa_rope_inv_freq")
+    return out, amp.value
+
+
+def rope_raw(q, k, q_out, k_out, batch_size, num_q_heads, num_kv_heads, seq_len, d_head, inv_freq, rotary_dim,
+             interleaved=False, amplitude=1.0, dtype="f16", positions=None, positions_stride=0, position_offset=0,
+             inverse=False, q_strides=(0, 0, 0), k_strides=(0, 0, 0), q_out_strides=(0, 0, 0), k_out_strides=(0, 0, 0),
+             stream=None) -> int:
+    """fa_rope; strides are (batch, head, row) in elements ((0, 0, 0) = dense [B, H, S, D]).  Returns the status code."""
+    a = RopeArgs(_ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), Strides(*q_strides), Strides(*k_strides),
+                 Strides(*q_out_strides), Strides(*k_out_strides), batch_size, num_q_heads, num_kv_heads, seq_len, d_head,
+                 DTYPES[dtype] if isinstance(dtype, str) else dtype, _ptr(positions), positions_stride, position_offset,
+                 int(inverse), _rotary(inv_freq, rotary_dim, interleaved, amplitude), _stream_handle(stream))
+    return lib().fa_rope(ctypes.byref(a))
+
+
+def rope(*args, **kw) -> None:
+    rc = rope_raw(*args, **kw)
+    if rc != FA_OK:
+        raise FaError(rc, "fa_rope")
+
+
+def _layout(kv_strides, param_strides, block_table, block_table_stride, page_size, num_pages, seq_lens) -> CacheLayout:
+    return CacheLayout(*kv_strides, *param_strides, _ptr(block_table), block_table_stride, page_size, num_pages,
+                       _ptr(seq_lens))
+
+
+def cache_append_raw(k, v, k_cache, v_cache, batch_size, num_tokens, num_kv_heads, seq_len_kv, d_head, dtype="f16",
+                     cache_dtype="f16", kv_strides=(0, 0, 0), q=None, q_out=None, num_q_heads=0,
+                     token_strides=(0, 0, 0), k_params=None, v_params=None, param_strides=(0, 0, 0), block_table=None,
+                     block_table_stride=0, page_size=0, num_pages=0, seq_lens=None, num_new=None, positions=None,
+                     inv_freq=None, rotary_dim=0, interleaved=False, amplitude=1.0, q_scale=None, k_scale=None,
+                     v_scale=None, stream=None) -> int:
+    """fa_cache_append; ``cache_dtype`` is that of q, k and v, "e4m3" or "u4"; ``kv_strides`` and ``param_strides`` are
+    (block, head, row) strides of the cache, a block being a page or a whole sequence; ``token_strides`` those between
+    the tokens of q, k, v.  Returns the status code."""
+    if cache_dtype in ("f16", "bf16") and cache_dtype != dtype:
+        return FA_ERR_UNSUPPORTED
+    a = CacheAppendArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), _ptr(k_params),
+                        _ptr(v_params), *token_strides, batch_size, num_tokens, num_q_heads, num_kv_heads, seq_len_kv,
+                        d_head, DTYPES[dtype] if isinstance(dtype, str) else dtype,
+                        CACHES[cache_dtype] if isinstance(cache_dtype, str) else cache_dtype,
+                        _layout(kv_strides, param_strides, block_table, block_table_stride, page_size, num_pages, seq_lens),
+                        _ptr(num_new), _ptr(positions), _rotary(inv_freq, rotary_dim, interleaved, amplitude),
+                        _ptr(q_scale), _ptr(k_scale), _ptr(v_scale), _stream_handle(stream))
+    return lib().fa_cache_append(ctypes.byref(a))
+
+
+def cache_append(*args, **kw) -> None:
+    rc = cache_append_raw(*args, **kw)
+    if rc != FA_OK:
+        raise FaError(rc, "fa_cache_append")
+
+
+def cache_read_u4_raw(k_cache, k_params, v_cache, v_params, k_out, v_out, batch_size, num_kv_heads, seq_len_kv, d_head,
+                      num_rows, dtype="f16", first_rows=None, kv_strides=(0, 0, 0), param_strides=(0, 0, 0),
+                      block_table=None, block_table_stride=0, page_size=0, num_pages=0, seq_lens=None, stream=None) -> int:
+    """fa_cache_read_u4; the cache is described as for cache_append.  Returns the status code."""
+    a = CacheReadArgs(_ptr(k_cache), _ptr(k_params), _ptr(v_cache), _ptr(v_params), _ptr(k_out), _ptr(v_out), batch_size,
+                      num_kv_heads, seq_len_kv, d_head, num_rows, DTYPES[dtype] if isinstance(dtype, str) else dtype,
+                      _layout(kv_strides, param_strides, block_table, block_table_stride, page_size, num_pages, seq_lens),
+                      _ptr(first_rows), _stream_handle(stream))
+    return lib().fa_cache_read_u4(ctypes.byref(a))
+
+
+def cache_read_u4(*args, **kw) -> None:
+    rc = cache_read_u4_raw(*args, **kw)
+    if rc != FA_OK:
+        raise FaError(rc, "fa_cache_read_u4")
 
 
 def combine(o_parts, lse_parts, n_parts, rows, d_head, o, lse, dtype="f16", stream=None) -> None:

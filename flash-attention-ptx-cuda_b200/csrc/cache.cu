@@ -1,0 +1,660 @@
+// The steps around attention that move q, k and v rows: rotary positions (fa_rope), filling a KV cache
+// with the rotation on the way (fa_cache_append) and reading a 4-bit cache back (fa_cache_read_u4).
+//
+// The reference has none of them: its programs start from Q, K and V (src/demo.cu:28-70).
+//
+// All three read every element once and write it once, so HBM bounds them.  A row of D elements is covered by D / 8
+// lanes with one 16-byte access each; a block of 256 threads has 16 (D = 128) or 32 (D = 64) rows in flight at a time,
+// kUnroll such groups before it uses the first.  A thread keeps to one token and walks heads, so cos and sin of its 8
+// elements are read once, from a table in shared memory that the block computes for its tokens.
+#include <cmath>
+#include <cuda_fp8.h>
+
+#include "host_common.h"
+#include "ptx.cuh"
+#include "u4.cuh"
+
+namespace fa {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;
+constexpr int kMaxPairs = 64;
+
+// What a kernel gets of fa_rotary: each pair's turns per position as a 64-bit fraction of a turn.  position * turns modulo
+// 2^64 is the exact fraction of a turn that the position has come to, for any 32-bit position: nothing is lost to
+// the whole turns, which in 32-bit floating point cost far positions their angle (position 10^6: 0.06 rad).
+struct Rotary {
+    unsigned long long turns[kMaxPairs];
+    double amplitude;
+    int dim;                             // elements that turn; 0: none
+};
+
+__device__ __forceinline__ void cos_sin(const Rotary& r, int position, int pair, bool inverse, float* c, float* s) {
+    const long long frac = (long long)((unsigned long long)(long long)position * r.turns[pair]);   // of a turn, times 2^64
+    double sd, cd;
+    sincospi((double)frac * 0x1p-63, &sd, &cd);
+    *c = (float)(cd * r.amplitude);
+    *s = (float)((inverse ? -sd : sd) * r.amplitude);
+}
+
+// A thread's part of a row: 8 elements from `lane * 8` on, turned.  With the half layout its partners lie in the lane
+// `partner`; `sin` comes with the sign of its half.
+template <bool BF16, bool INTER>
+struct Turn {
+    float c[INTER ? 4 : 8], s[INTER ? 4 : 8];
+    int partner;
+    bool on;
+    // `table`: cos and sin of the thread's token, pair by pair
+    template <int LPR>
+    __device__ __forceinline__ void load(const float2* table, int lane, int dim) {
+        on = lane * 8 < dim;
+        partner = lane;
+        if (!on) return;
+        if constexpr (INTER) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) { c[e] = table[lane * 4 + e].x; s[e] = table[lane * 4 + e].y; }
+        } else {
+            const int half = dim / 16;                     // lanes of the first halves
+            const bool second = lane >= half;
+            partner = second ? lane - half : lane + half;
+            const int p = (second ? lane - half : lane) * 8;
+#pragma unroll
+            for (int e = 0; e < 8; e++) { c[e] = table[p + e].x; s[e] = second ? table[p + e].y : -table[p + e].y; }
+        }
+    }
+    // All lanes of the warp call this.  Products and sums are rounded one by one, so that a value is the same
+    // wherever it is computed: a cache in 4 bits takes its levels from it.
+    template <int LPR>
+    __device__ __forceinline__ uint4 apply(const uint4& x) const {
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        uint32_t y[4];
+        if constexpr (INTER) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 a = unpack16<BF16>(w[i]);
+                y[i] = pack16<BF16>(__fsub_rn(__fmul_rn(a.x, c[i]), __fmul_rn(a.y, s[i])),
+                                    __fadd_rn(__fmul_rn(a.y, c[i]), __fmul_rn(a.x, s[i])));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t pw = __shfl_sync(0xffffffffu, w[i], partner, LPR);
+                const float2 a = unpack16<BF16>(w[i]), p = unpack16<BF16>(pw);
+                y[i] = pack16<BF16>(__fadd_rn(__fmul_rn(a.x, c[2 * i]), __fmul_rn(p.x, s[2 * i])),
+                                    __fadd_rn(__fmul_rn(a.y, c[2 * i + 1]), __fmul_rn(p.y, s[2 * i + 1])));
+            }
+        }
+        return on ? make_uint4(y[0], y[1], y[2], y[3]) : x;
+    }
+};
+
+__device__ __forceinline__ uint4 ld_row_16(const uint16_t* p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+
+// ------------------------------------------------------------------------------------------ fa_rope
+struct RopeTensor {
+    const uint16_t* in;
+    uint16_t* out;
+    fa_strides is, os;
+};
+struct RopeArgs {
+    RopeTensor q, k;
+    Rotary rot;
+    int hq, heads, seq_len, tiles;       // heads of q and k together, token tiles of a sequence
+    int tokens;                          // of a block: a power of two
+    int splits;                          // blocks that share a tile's heads
+    const int* positions;
+    int positions_stride, position_offset;
+    bool inverse;
+};
+
+template <int D, bool BF16, bool INTER>
+__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
+    constexpr int LPR = D / 8, SLOTS = kThreads / LPR;
+    extern __shared__ float2 table[];                       // [tokens][dim / 2]
+    const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits;
+    const int b = tile / a.tiles, s0 = (tile - b * a.tiles) * a.tokens;
+    const int pairs = a.rot.dim / 2;
+    if (a.positions != nullptr) grid_dependency_wait();     // known positions: the table overlaps the kernel before
+    for (int i = threadIdx.x; i < a.tokens * pairs; i += kThreads) {
+        const int t = i / pairs, s = min(s0 + t, a.seq_len - 1);
+        const int pos = a.positions == nullptr ? s + a.position_offset : a.positions[(long long)b * a.positions_stride + s];
+        float2 cs;
+        cos_sin(a.rot, pos, i - t * pairs, a.inverse, &cs.x, &cs.y);
+        table[i] = cs;
+    }
+    grid_dependency_wait();
+    grid_launch_dependents();
+    __syncthreads();
+    const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR;
+    const int t = slot & (a.tokens - 1), step = SLOTS / a.tokens;
+    const int s = s0 + t;
+    Turn<BF16, INTER> turn;
+    turn.template load<LPR>(table + t * pairs, lane, a.rot.dim);
+    const int per = (a.heads + a.splits - 1) / a.splits, h_end = min(a.heads, (split + 1) * per);
+    for (int h0 = split * per; h0 < h_end; h0 += step * kUnroll) {
+        uint4 x[kUnroll];
+        bool live[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; u++) {
+            const int h = h0 + u * step + slot / a.tokens;
+            live[u] = h < h_end && s < a.seq_len;
+            x[u] = make_uint4(0, 0, 0, 0);
+            if (live[u]) {
+                const RopeTensor& r = h < a.hq ? a.q : a.k;
+                x[u] = ld_row_16(r.in + b * r.is.batch + (h < a.hq ? h : h - a.hq) * r.is.head + s * r.is.row + lane * 8);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; u++) {
+            const int h = h0 + u * step + slot / a.tokens;
+            const uint4 y = turn.template apply<LPR>(x[u]);
+            if (live[u]) {
+                const RopeTensor& r = h < a.hq ? a.q : a.k;
+                *reinterpret_cast<uint4*>(r.out + b * r.os.batch + (h < a.hq ? h : h - a.hq) * r.os.head + s * r.os.row + lane * 8) = y;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------ fa_cache_append
+struct AppendArgs {
+    const uint16_t *q, *k, *v;
+    void* q_out;
+    uint8_t *k_cache, *v_cache;
+    __half2 *k_params, *v_params;
+    long long q_stride, k_stride, v_stride;
+    Rotary rot;
+    int hq, hkv, n_tokens, n_all, seq_len_kv;    // tokens of a sequence, of all
+    int tokens, splits;                          // as in RopeArgs
+    CacheMap map;
+    long long block_stride, head_stride, row_stride;          // bytes
+    long long p_block_stride, p_head_stride, p_row_stride;    // pairs
+    const int *seq_lens, *num_new, *positions;
+    const float *q_scale, *k_scale, *v_scale;
+};
+
+struct Token {
+    int b, row, position;
+    bool live;                                   // is stored
+};
+__device__ __forceinline__ Token token(const AppendArgs& a, int n) {
+    Token r;
+    r.b = n / a.n_tokens;
+    const int t = n - r.b * a.n_tokens;
+    r.row = sequence_length(a.seq_lens, r.b, a.seq_len_kv) - a.n_tokens + t;
+    r.live = r.row >= 0 && (a.num_new == nullptr || t >= a.n_tokens - a.num_new[r.b]);
+    r.position = a.positions == nullptr ? r.row : a.positions[n];
+    return r;
+}
+
+__device__ __forceinline__ uint32_t e4m3x4(float2 a, float2 b) {
+    const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3);
+    const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3);
+    return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+// 8 elements as e4m3 codes of value * inv.
+template <bool BF16>
+__device__ __forceinline__ uint2 to_e4m3(const uint4& x, float inv) {
+    const float2 a = unpack16<BF16>(x.x), b = unpack16<BF16>(x.y), c = unpack16<BF16>(x.z), d = unpack16<BF16>(x.w);
+    return make_uint2(e4m3x4(make_float2(a.x * inv, a.y * inv), make_float2(b.x * inv, b.y * inv)),
+                      e4m3x4(make_float2(c.x * inv, c.y * inv), make_float2(d.x * inv, d.y * inv)));
+}
+// 8 elements as 4-bit codes; the 8 lanes of a group of 64 call this together.  Returns the codes, and scale and
+// offset in every lane.
+template <bool BF16>
+__device__ __forceinline__ uint32_t to_u4(const uint4& x, __half2* param) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 a = unpack16<BF16>(w[i]);
+        f[2 * i] = max_nan(min_nan(a.x, kU4Max), -kU4Max);
+        f[2 * i + 1] = max_nan(min_nan(a.y, kU4Max), -kU4Max);
+    }
+    float lo = f[0], hi = f[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) { lo = min_nan(lo, f[i]); hi = max_nan(hi, f[i]); }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    const __half z16 = __float2half_rn(lo);
+    const float z = __half2float(z16);
+    const __half s16 = __float2half_rn(__fmul_rn(__fsub_rn(hi, z), 1.0f / 15.0f));
+    const float s = __half2float(s16), inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
+    uint32_t codes = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(f[i], z), inv), 0.0f), 15.0f);
+        codes |= (uint32_t)__float2int_rn(c) << (4 * i);
+    }
+    *param = __halves2half2(s16, z16);
+    return codes;
+}
+
+template <int D, bool BF16, bool INTER, int CACHE>
+__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a) {
+    constexpr int LPR = D / 8, SLOTS = kThreads / LPR;
+    extern __shared__ float2 table[];                       // [tokens][dim / 2]
+    const int split = blockIdx.x % a.splits, n0 = blockIdx.x / a.splits * a.tokens;
+    const int pairs = a.rot.dim / 2;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int heads = a.hq + 2 * a.hkv, per = (heads + a.splits - 1) / a.splits;
+    const int h_begin = split * per, h_end = min(heads, h_begin + per);
+    if (h_begin < a.hq + a.hkv)                             // not v alone
+        for (int i = threadIdx.x; i < a.tokens * pairs; i += kThreads) {
+            const int t = i / pairs;
+            float2 cs;
+            cos_sin(a.rot, token(a, min(n0 + t, a.n_all - 1)).position, i - t * pairs, false, &cs.x, &cs.y);
+            table[i] = cs;
+        }
+    __syncthreads();
+    const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR;
+    const int t = slot & (a.tokens - 1), step = SLOTS / a.tokens;
+    const int n = n0 + t;
+    const bool in = n < a.n_all;
+    const Token tk = token(a, min(n, a.n_all - 1));
+    CacheRow at = {-1, 0};
+    if (in && tk.live) at = cache_row(a.map, tk.b, tk.row);
+    Turn<BF16, INTER> turn;
+    turn.template load<LPR>(table + t * pairs, lane, a.rot.dim);
+    const int group = a.hq / a.hkv;
+    for (int h0 = h_begin; h0 < h_end; h0 += step * kUnroll) {
+        uint4 x[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; u++) {
+            const int h = h0 + u * step + slot / a.tokens;
+            x[u] = make_uint4(0, 0, 0, 0);
+            if (h < h_end && in && tk.live) {
+                const uint16_t* p = h < a.hq ? a.q + n * a.q_stride + h * D
+                                  : h < a.hq + a.hkv ? a.k + n * a.k_stride + (h - a.hq) * D
+                                                     : a.v + n * a.v_stride + (h - a.hq - a.hkv) * D;
+                x[u] = ld_row_16(p + lane * 8);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; u++) {
+            const int h = h0 + u * step + slot / a.tokens;
+            const bool mine = h < h_end && in;
+            const uint4 turned = turn.template apply<LPR>(x[u]);
+            const uint4 y = h < a.hq + a.hkv ? turned : x[u];
+            const bool is_v = h >= a.hq + a.hkv;
+            const int kv_head = is_v ? h - a.hq - a.hkv : h - a.hq;
+            if (h < a.hq) {
+                if (mine) {
+                    const long long o = ((long long)n * a.hq + h) * D + lane * 8;
+                    if constexpr (CACHE == FA_CACHE_E4M3) {
+                        const float inv = tk.live ? __frcp_rn(a.q_scale[tk.b * a.hkv + h / group]) : 0.0f;
+                        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.q_out) + o) = tk.live ? to_e4m3<BF16>(y, inv) : make_uint2(0, 0);
+                    } else {
+                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.q_out) + o) = tk.live ? y : make_uint4(0, 0, 0, 0);
+                    }
+                }
+            }
+            const bool store = mine && h >= a.hq && at.block >= 0;
+            uint8_t* row = (is_v ? a.v_cache : a.k_cache) + at.block * a.block_stride + (long long)kv_head * a.head_stride + at.in_block * a.row_stride;
+            if constexpr (CACHE == FA_CACHE_U4) {
+                __half2 param;
+                const uint32_t codes = to_u4<BF16>(y, &param);       // lanes of a row agree on `store`; all take part
+                if (store) {
+                    *reinterpret_cast<uint32_t*>(row + lane * 4) = codes;
+                    if ((lane & 7) == 0)
+                        (is_v ? a.v_params : a.k_params)[at.block * a.p_block_stride + (long long)kv_head * a.p_head_stride + at.in_block * a.p_row_stride + lane / 8] = param;
+                }
+            } else if (store) {
+                if constexpr (CACHE == FA_CACHE_E4M3) {
+                    const float inv = __frcp_rn((is_v ? a.v_scale : a.k_scale)[tk.b * a.hkv + kv_head]);
+                    *reinterpret_cast<uint2*>(row + lane * 8) = to_e4m3<BF16>(y, inv);
+                } else {
+                    *reinterpret_cast<uint4*>(row + lane * 16) = y;
+                }
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------ fa_cache_read_u4
+struct ReadArgs {
+    const uint8_t *k, *v;
+    const __half2 *kp, *vp;
+    uint16_t *k_out, *v_out;
+    int hkv, seq_len_kv, n_rows, tiles;
+    CacheMap map;
+    long long block_stride, head_stride, row_stride;          // bytes
+    long long p_block_stride, p_head_stride, p_row_stride;    // pairs
+    const int *seq_lens, *first_rows;
+};
+
+template <bool BF16>
+__device__ __forceinline__ uint4 from_u4(uint32_t codes, __half2 param) {
+    const float s = __low2float(param), z = __high2float(param);
+    uint32_t y[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float a = fmaf(s, (float)((codes >> (8 * i)) & 15u), z), b = fmaf(s, (float)((codes >> (8 * i + 4)) & 15u), z);
+        if constexpr (!BF16) { a = min_nan(a, kU4Max); b = min_nan(b, kU4Max); }    // a scale rounded up: -65504 + 15 * 8736 = 65536
+        y[i] = pack16<BF16>(a, b);
+    }
+    return make_uint4(y[0], y[1], y[2], y[3]);
+}
+
+// A block takes kUnroll groups of consecutive rows of one head.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads) read_u4_kernel(const __grid_constant__ ReadArgs a) {
+    constexpr int LPR = D / 8, SLOTS = kThreads / LPR;
+    const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR;
+    const int bh = blockIdx.x / a.tiles, tile = blockIdx.x - bh * a.tiles;
+    const int b = bh / a.hkv, h = bh - b * a.hkv;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int len = sequence_length(a.seq_lens, b, a.seq_len_kv);
+    const int first = a.first_rows == nullptr ? 0 : a.first_rows[b];
+    uint32_t kc[kUnroll], vc[kUnroll];
+    __half2 kp[kUnroll], vp[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+        const int n = (tile * kUnroll + u) * SLOTS + slot;
+        const long long row = (long long)first + n;
+        kc[u] = vc[u] = 0;
+        kp[u] = vp[u] = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+        if (n < a.n_rows && row >= 0 && row < len) {
+            const CacheRow at = cache_row(a.map, b, (int)row);
+            if (at.block >= 0) {
+                const long long o = at.block * a.block_stride + h * a.head_stride + at.in_block * a.row_stride + lane * 4;
+                const long long p = at.block * a.p_block_stride + h * a.p_head_stride + at.in_block * a.p_row_stride + lane / 8;
+                kc[u] = *reinterpret_cast<const uint32_t*>(a.k + o);
+                vc[u] = *reinterpret_cast<const uint32_t*>(a.v + o);
+                kp[u] = a.kp[p];
+                vp[u] = a.vp[p];
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+        const int n = (tile * kUnroll + u) * SLOTS + slot;
+        if (n < a.n_rows) {
+            const long long o = (((long long)b * a.n_rows + n) * a.hkv + h) * D + lane * 8;
+            *reinterpret_cast<uint4*>(a.k_out + o) = from_u4<BF16>(kc[u], kp[u]);
+            *reinterpret_cast<uint4*>(a.v_out + o) = from_u4<BF16>(vc[u], vp[u]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------ host
+int make_rotary(const fa_rotary& r, int d_head, bool optional, Rotary* out) {
+    *out = Rotary{};
+    if (r.rotary_dim < 0) return FA_ERR_INVALID_ARGUMENT;
+    if (r.rotary_dim == 0) return optional ? FA_OK : FA_ERR_INVALID_ARGUMENT;
+    if (r.rotary_dim > d_head || r.rotary_dim % 16 != 0) return FA_ERR_UNSUPPORTED;
+    if (r.inv_freq == nullptr || !std::isfinite(r.amplitude) || (r.interleaved != 0 && r.interleaved != 1)) return FA_ERR_INVALID_ARGUMENT;
+    const long double two_pi = 6.283185307179586476925286766559L;
+    for (int i = 0; i < r.rotary_dim / 2; i++) {
+        if (!std::isfinite(r.inv_freq[i])) return FA_ERR_INVALID_ARGUMENT;
+        long double f = r.inv_freq[i] / two_pi;
+        f -= std::floor(f);                                  // whole turns are none
+        out->turns[i] = f >= 1.0L ? 0ull : (unsigned long long)(f * 18446744073709551616.0L);
+    }
+    out->amplitude = r.amplitude;
+    out->dim = r.rotary_dim;
+    return FA_OK;
+}
+
+// Blocks that share a tile's heads.  A block computes cos and sin for all of its tokens, so few blocks with many heads
+// are better until the GPU has idle SMs: two blocks an SM.
+int head_splits(long long tiles, int heads, int rows_at_once, int sm_count) {
+    const long long want = (2ll * sm_count + tiles - 1) / tiles;
+    const int most = (heads + rows_at_once - 1) / rows_at_once;
+    return want < 1 ? 1 : want > most ? most : (int)want;
+}
+int pow2_at_least(int n, int most) {
+    int p = 1;
+    while (p < n && p < most) p *= 2;
+    return p;
+}
+
+bool strides_ok(const fa_strides& s) { return s.batch >= 0 && s.head >= 0 && s.row >= 0; }
+bool strides_aligned(const fa_strides& s) { return s.batch % 8 == 0 && s.head % 8 == 0 && s.row % 8 == 0; }
+fa_strides or_dense(const fa_strides& s, int heads, int seq_len, int d_head) {
+    if (s.batch || s.head || s.row) return s;
+    return {(long long)heads * seq_len * d_head, (long long)seq_len * d_head, d_head};
+}
+
+template <int D, bool BF16, bool INTER>
+int run_rope(const RopeArgs& a, unsigned blocks, cudaStream_t stream) {
+    return launch_dependent(rope_kernel<D, BF16, INTER>, blocks, kThreads, (size_t)a.tokens * (a.rot.dim / 2) * sizeof(float2), stream, 1, a);
+}
+template <int D, bool BF16, bool INTER, int CACHE>
+int run_append(const AppendArgs& a, unsigned blocks, cudaStream_t stream) {
+    return launch_dependent(append_kernel<D, BF16, INTER, CACHE>, blocks, kThreads, (size_t)a.tokens * (a.rot.dim / 2) * sizeof(float2), stream, 1, a);
+}
+template <int D, bool BF16, bool INTER>
+int run_append_to(const AppendArgs& a, int cache, unsigned blocks, cudaStream_t stream) {
+    if (cache == FA_CACHE_U4) return run_append<D, BF16, INTER, FA_CACHE_U4>(a, blocks, stream);
+    if constexpr (D == 128)
+        if (cache == FA_CACHE_E4M3) return run_append<D, BF16, INTER, FA_CACHE_E4M3>(a, blocks, stream);
+    return run_append<D, BF16, INTER, FA_CACHE_16BIT>(a, blocks, stream);
+}
+
+}  // namespace
+
+// Checks a layout and gives where the rows lie; strides in bytes (`elem` bytes an element, half a byte: elem = 0).
+int check_layout(const fa_cache_layout& l, int cache, int d_head, int seq_len_kv, int elem, CacheMap* map) {
+    const long long unit = cache == FA_CACHE_U4 ? 1 : elem, row = cache == FA_CACHE_U4 ? d_head / 2 : (long long)d_head * elem;
+    if (l.block_stride <= 0 || l.head_stride <= 0 || l.row_stride * unit < row) return FA_ERR_INVALID_ARGUMENT;
+    if (l.block_stride * unit % 16 || l.head_stride * unit % 16 || l.row_stride * unit % 16) return FA_ERR_MISALIGNED;
+    if (cache == FA_CACHE_U4) {
+        const int pairs = d_head / kU4Group;
+        if (l.param_block_stride <= 0 || l.param_head_stride <= 0 || l.param_row_stride < pairs) return FA_ERR_INVALID_ARGUMENT;
+        if (l.param_block_stride % pairs || l.param_head_stride % pairs || l.param_row_stride % pairs) return FA_ERR_MISALIGNED;
+    }
+    *map = CacheMap{nullptr, 0, -1, 0};
+    if (l.block_table != nullptr) {
+        const int ps = l.page_size;
+        if (ps < 16 || (ps & (ps - 1)) != 0 || l.num_pages <= 0) return FA_ERR_INVALID_ARGUMENT;
+        if ((long long)l.block_table_stride * ps < seq_len_kv) return FA_ERR_INVALID_ARGUMENT;
+        int shift = 0;
+        while ((1 << shift) < ps) shift++;
+        *map = CacheMap{l.block_table, l.block_table_stride, shift, l.num_pages};
+    }
+    return FA_OK;
+}
+
+}  // namespace fa
+
+using namespace fa;
+
+FA_EXPORT int fa_rope(const fa_rope_args* p) {
+    if (!p || !p->q || !p->q_out) return FA_ERR_INVALID_ARGUMENT;
+    if (p->batch_size <= 0 || p->num_q_heads <= 0 || p->num_kv_heads < 0 || p->seq_len <= 0) return FA_ERR_INVALID_ARGUMENT;
+    if ((p->num_kv_heads > 0) != (p->k != nullptr) || (p->k != nullptr) != (p->k_out != nullptr)) return FA_ERR_INVALID_ARGUMENT;
+    if (p->inverse != 0 && p->inverse != 1) return FA_ERR_INVALID_ARGUMENT;
+    if (p->positions_stride < 0 || (long long)p->position_offset + p->seq_len - 1 > 0x7FFFFFFFll) return FA_ERR_INVALID_ARGUMENT;
+    if (!strides_ok(p->q_strides) || !strides_ok(p->k_strides) || !strides_ok(p->q_out_strides) || !strides_ok(p->k_out_strides))
+        return FA_ERR_INVALID_ARGUMENT;
+    if (p->d_head != 64 && p->d_head != 128) return FA_ERR_UNSUPPORTED;
+    if (p->dtype != FA_DTYPE_F16 && p->dtype != FA_DTYPE_BF16) return FA_ERR_UNSUPPORTED;
+    RopeArgs a;
+    int rc = make_rotary(p->rotary, p->d_head, false, &a.rot);
+    if (rc != FA_OK) return rc;
+    if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->q_out) || !aligned16(p->k_out)) return FA_ERR_MISALIGNED;
+    if (!strides_aligned(p->q_strides) || !strides_aligned(p->k_strides) || !strides_aligned(p->q_out_strides) || !strides_aligned(p->k_out_strides))
+        return FA_ERR_MISALIGNED;
+    DeviceState* st = device_state();
+    if (!st) return FA_ERR_CUDA;
+    if (st->cc_major != 10) return FA_ERR_NOT_SM100;
+    a.q = {static_cast<const uint16_t*>(p->q), static_cast<uint16_t*>(p->q_out), or_dense(p->q_strides, p->num_q_heads, p->seq_len, p->d_head),
+           or_dense(p->q_out_strides, p->num_q_heads, p->seq_len, p->d_head)};
+    a.k = {static_cast<const uint16_t*>(p->k), static_cast<uint16_t*>(p->k_out), or_dense(p->k_strides, p->num_kv_heads, p->seq_len, p->d_head),
+           or_dense(p->k_out_strides, p->num_kv_heads, p->seq_len, p->d_head)};
+    a.hq = p->num_q_heads;
+    a.heads = p->num_q_heads + p->num_kv_heads;
+    a.seq_len = p->seq_len;
+    a.tokens = pow2_at_least(p->seq_len, 8);
+    a.tiles = (p->seq_len + a.tokens - 1) / a.tokens;
+    const long long tiles = (long long)a.tiles * p->batch_size;
+    const int slots = kThreads / (p->d_head / 8);
+    a.splits = head_splits(tiles, a.heads, slots / a.tokens, st->sm_count);
+    a.positions = p->positions;
+    a.positions_stride = p->positions_stride;
+    a.position_offset = p->position_offset;
+    a.inverse = p->inverse != 0;
+    if (tiles * a.splits > 0x7FFFFFFFll) return FA_ERR_INVALID_ARGUMENT;
+    const unsigned blocks = (unsigned)(tiles * a.splits);
+    cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
+    const bool bf = p->dtype == FA_DTYPE_BF16, inter = p->rotary.interleaved != 0;
+    if (p->d_head == 64)
+        return bf ? (inter ? run_rope<64, true, true>(a, blocks, stream) : run_rope<64, true, false>(a, blocks, stream))
+                  : (inter ? run_rope<64, false, true>(a, blocks, stream) : run_rope<64, false, false>(a, blocks, stream));
+    return bf ? (inter ? run_rope<128, true, true>(a, blocks, stream) : run_rope<128, true, false>(a, blocks, stream))
+              : (inter ? run_rope<128, false, true>(a, blocks, stream) : run_rope<128, false, false>(a, blocks, stream));
+}
+
+FA_EXPORT int fa_rope_inv_freq(const fa_rope_scaling* s, int rotary_dim, double* inv_freq, float* amplitude) {
+    if (!s || !inv_freq) return FA_ERR_INVALID_ARGUMENT;
+    if (rotary_dim <= 0 || rotary_dim % 16 != 0 || rotary_dim > 2 * kMaxPairs) return FA_ERR_UNSUPPORTED;
+    if (s->kind < FA_ROPE_PLAIN || s->kind > FA_ROPE_SMOOTH) return FA_ERR_UNSUPPORTED;
+    if (!(s->base > 1.0) || !std::isfinite(s->base)) return FA_ERR_INVALID_ARGUMENT;
+    if (s->kind != FA_ROPE_PLAIN && (!(s->factor >= 1.0) || !std::isfinite(s->factor))) return FA_ERR_INVALID_ARGUMENT;
+    const bool mixed = s->kind == FA_ROPE_PARTS || s->kind == FA_ROPE_SMOOTH;
+    if (mixed && (!(s->original_length > 0.0) || !std::isfinite(s->original_length) || !(s->slow > 0.0) || !(s->fast > s->slow) || !std::isfinite(s->fast)))
+        return FA_ERR_INVALID_ARGUMENT;
+    const double two_pi = 6.283185307179586476925286766559, r = rotary_dim;
+    const double base = s->kind == FA_ROPE_BASE ? s->base * std::pow(s->factor, r / (r - 2.0)) : s->base;
+    // index at which a pair makes `turns` turns over the original length
+    auto index_of = [&](double turns) { return r * std::log(s->original_length / (turns * two_pi)) / (2.0 * std::log(base)); };
+    double lo = 0.0, hi = 0.0;
+    if (s->kind == FA_ROPE_PARTS) {
+        lo = std::fmax(std::floor(index_of(s->fast)), 0.0);
+        hi = std::fmin(std::ceil(index_of(s->slow)), r - 1.0);
+        if (hi - lo < 1e-3) hi = lo + 1e-3;                  // a step instead of a ramp
+    }
+    for (int i = 0; i < rotary_dim / 2; i++) {
+        const double f = std::pow(base, -2.0 * i / r);
+        double keep = s->kind == FA_ROPE_LINEAR ? 0.0 : 1.0;
+        if (s->kind == FA_ROPE_PARTS) keep = 1.0 - std::fmin(std::fmax((i - lo) / (hi - lo), 0.0), 1.0);
+        if (s->kind == FA_ROPE_SMOOTH) keep = std::fmin(std::fmax((s->original_length * f / two_pi - s->slow) / (s->fast - s->slow), 0.0), 1.0);
+        inv_freq[i] = keep == 1.0 ? f : keep * f + (1.0 - keep) * f / s->factor;
+    }
+    if (amplitude) *amplitude = s->kind == FA_ROPE_PARTS ? (float)(0.1 * std::log(s->factor) + 1.0) : 1.0f;
+    return FA_OK;
+}
+
+FA_EXPORT int fa_cache_append(const fa_cache_append_args* p) {
+    if (!p || !p->k || !p->v || !p->k_cache || !p->v_cache) return FA_ERR_INVALID_ARGUMENT;
+    if (p->batch_size <= 0 || p->num_tokens <= 0 || p->num_kv_heads <= 0 || p->num_q_heads < 0 || p->seq_len_kv <= 0) return FA_ERR_INVALID_ARGUMENT;
+    if ((p->q != nullptr) != (p->num_q_heads > 0) || (p->q != nullptr) != (p->q_out != nullptr)) return FA_ERR_INVALID_ARGUMENT;
+    if (p->num_q_heads % p->num_kv_heads != 0 || p->num_tokens > p->seq_len_kv) return FA_ERR_INVALID_ARGUMENT;
+    if (p->q_token_stride < 0 || p->k_token_stride < 0 || p->v_token_stride < 0) return FA_ERR_INVALID_ARGUMENT;
+    if (p->d_head != 64 && p->d_head != 128) return FA_ERR_UNSUPPORTED;
+    if (p->dtype != FA_DTYPE_F16 && p->dtype != FA_DTYPE_BF16) return FA_ERR_UNSUPPORTED;
+    if (p->cache != FA_CACHE_16BIT && p->cache != FA_CACHE_E4M3 && p->cache != FA_CACHE_U4) return FA_ERR_UNSUPPORTED;
+    if (p->cache == FA_CACHE_E4M3) {
+        if (p->d_head != 128) return FA_ERR_UNSUPPORTED;
+        if (!p->k_scale || !p->v_scale || (p->q && !p->q_scale)) return FA_ERR_INVALID_ARGUMENT;
+    }
+    if (p->cache == FA_CACHE_U4 && (!p->k_params || !p->v_params)) return FA_ERR_INVALID_ARGUMENT;
+    const long long n_all = (long long)p->batch_size * p->num_tokens;
+    const int heads = p->num_q_heads + 2 * p->num_kv_heads;
+    if (n_all * heads > 0x7FFFFFFFll) return FA_ERR_INVALID_ARGUMENT;
+    AppendArgs a;
+    int rc = make_rotary(p->rotary, p->d_head, true, &a.rot);
+    if (rc != FA_OK) return rc;
+    const int elem = p->cache == FA_CACHE_E4M3 ? 1 : 2;
+    const long long unit = p->cache == FA_CACHE_U4 ? 1 : elem;
+    if ((rc = check_layout(p->layout, p->cache, p->d_head, p->seq_len_kv, elem, &a.map)) != FA_OK) return rc;
+    if (p->q_token_stride % 8 || p->k_token_stride % 8 || p->v_token_stride % 8) return FA_ERR_MISALIGNED;
+    if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->q_out) || !aligned16(p->k_cache) || !aligned16(p->v_cache) ||
+        !aligned16(p->k_params) || !aligned16(p->v_params))
+        return FA_ERR_MISALIGNED;
+    const long long dense_kv = (long long)p->num_kv_heads * p->d_head, dense_q = (long long)p->num_q_heads * p->d_head;
+    a.q_stride = p->q_token_stride ? p->q_token_stride : dense_q;
+    a.k_stride = p->k_token_stride ? p->k_token_stride : dense_kv;
+    a.v_stride = p->v_token_stride ? p->v_token_stride : dense_kv;
+    if (a.q_stride < dense_q || a.k_stride < dense_kv || a.v_stride < dense_kv) return FA_ERR_INVALID_ARGUMENT;
+    DeviceState* st = device_state();
+    if (!st) return FA_ERR_CUDA;
+    if (st->cc_major != 10) return FA_ERR_NOT_SM100;
+    a.q = static_cast<const uint16_t*>(p->q);
+    a.k = static_cast<const uint16_t*>(p->k);
+    a.v = static_cast<const uint16_t*>(p->v);
+    a.q_out = p->q_out;
+    a.k_cache = static_cast<uint8_t*>(p->k_cache);
+    a.v_cache = static_cast<uint8_t*>(p->v_cache);
+    a.k_params = static_cast<__half2*>(p->k_params);
+    a.v_params = static_cast<__half2*>(p->v_params);
+    a.hq = p->num_q_heads;
+    a.hkv = p->num_kv_heads;
+    a.n_tokens = p->num_tokens;
+    a.n_all = (int)n_all;
+    a.seq_len_kv = p->seq_len_kv;
+    a.tokens = pow2_at_least((int)((n_all + 2 * st->sm_count - 1) / (2 * st->sm_count)), 8);
+    const long long tiles = (n_all + a.tokens - 1) / a.tokens;
+    a.splits = head_splits(tiles, heads, kThreads / (p->d_head / 8) / a.tokens, st->sm_count);
+    a.block_stride = p->layout.block_stride * unit;
+    a.head_stride = p->layout.head_stride * unit;
+    a.row_stride = p->layout.row_stride * unit;
+    a.p_block_stride = p->layout.param_block_stride;
+    a.p_head_stride = p->layout.param_head_stride;
+    a.p_row_stride = p->layout.param_row_stride;
+    a.seq_lens = p->layout.seq_lens;
+    a.num_new = p->num_new;
+    a.positions = p->positions;
+    a.q_scale = p->q_scale;
+    a.k_scale = p->k_scale;
+    a.v_scale = p->v_scale;
+    const unsigned blocks = (unsigned)(tiles * a.splits);
+    cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
+    const bool bf = p->dtype == FA_DTYPE_BF16, inter = p->rotary.interleaved != 0;
+    if (p->d_head == 64)
+        return bf ? (inter ? run_append_to<64, true, true>(a, p->cache, blocks, stream) : run_append_to<64, true, false>(a, p->cache, blocks, stream))
+                  : (inter ? run_append_to<64, false, true>(a, p->cache, blocks, stream) : run_append_to<64, false, false>(a, p->cache, blocks, stream));
+    return bf ? (inter ? run_append_to<128, true, true>(a, p->cache, blocks, stream) : run_append_to<128, true, false>(a, p->cache, blocks, stream))
+              : (inter ? run_append_to<128, false, true>(a, p->cache, blocks, stream) : run_append_to<128, false, false>(a, p->cache, blocks, stream));
+}
+
+FA_EXPORT int fa_cache_read_u4(const fa_cache_read_args* p) {
+    if (!p || !p->k_cache || !p->k_params || !p->v_cache || !p->v_params || !p->k_out || !p->v_out) return FA_ERR_INVALID_ARGUMENT;
+    if (p->batch_size <= 0 || p->num_kv_heads <= 0 || p->seq_len_kv <= 0 || p->num_rows <= 0) return FA_ERR_INVALID_ARGUMENT;
+    if (p->d_head != 64 && p->d_head != 128) return FA_ERR_UNSUPPORTED;
+    if (p->dtype != FA_DTYPE_F16 && p->dtype != FA_DTYPE_BF16) return FA_ERR_UNSUPPORTED;
+    ReadArgs a;
+    int rc = check_layout(p->layout, FA_CACHE_U4, p->d_head, p->seq_len_kv, 0, &a.map);
+    if (rc != FA_OK) return rc;
+    if (!aligned16(p->k_cache) || !aligned16(p->v_cache) || !aligned16(p->k_params) || !aligned16(p->v_params) || !aligned16(p->k_out) || !aligned16(p->v_out))
+        return FA_ERR_MISALIGNED;
+    const int slots = kThreads / (p->d_head / 8);
+    const long long tiles = ((long long)p->num_rows + slots * kUnroll - 1) / (slots * kUnroll);
+    const long long blocks = tiles * p->batch_size * p->num_kv_heads;
+    if (blocks > 0x7FFFFFFFll || (long long)p->num_rows + slots * kUnroll > 0x7FFFFFFFll) return FA_ERR_INVALID_ARGUMENT;
+    DeviceState* st = device_state();
+    if (!st) return FA_ERR_CUDA;
+    if (st->cc_major != 10) return FA_ERR_NOT_SM100;
+    a.k = static_cast<const uint8_t*>(p->k_cache);
+    a.v = static_cast<const uint8_t*>(p->v_cache);
+    a.kp = static_cast<const __half2*>(p->k_params);
+    a.vp = static_cast<const __half2*>(p->v_params);
+    a.k_out = static_cast<uint16_t*>(p->k_out);
+    a.v_out = static_cast<uint16_t*>(p->v_out);
+    a.hkv = p->num_kv_heads;
+    a.seq_len_kv = p->seq_len_kv;
+    a.n_rows = p->num_rows;
+    a.tiles = (int)tiles;
+    a.block_stride = p->layout.block_stride;
+    a.head_stride = p->layout.head_stride;
+    a.row_stride = p->layout.row_stride;
+    a.p_block_stride = p->layout.param_block_stride;
+    a.p_head_stride = p->layout.param_head_stride;
+    a.p_row_stride = p->layout.param_row_stride;
+    a.seq_lens = p->layout.seq_lens;
+    a.first_rows = p->first_rows;
+    const bool bf = p->dtype == FA_DTYPE_BF16;
+    auto kernel = p->d_head == 64 ? (bf ? read_u4_kernel<64, true> : read_u4_kernel<64, false>) : (bf ? read_u4_kernel<128, true> : read_u4_kernel<128, false>);
+    return launch_dependent(kernel, (unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(p->stream), 1, a);
+}

@@ -135,4 +135,9 @@ struct GqaLaunch {
 };
 int launch_decode_gqa(const GqaLaunch& g, DeviceState* st);
 
+// Caches of fa_cache_layout (u4.cuh): checks a layout and gives where its rows lie.  `elem`: bytes of an element of
+// a 16-bit or e4m3 cache.
+struct CacheMap;
+int check_layout(const fa_cache_layout& l, int cache, int d_head, int seq_len_kv, int elem, CacheMap* map);
+
 }  // namespace fa

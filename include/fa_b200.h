@@ -305,6 +305,187 @@ typedef struct fa_backward_args {
 size_t fa_backward_workspace_bytes(int batch_size, int num_heads, int seq_len);
 int fa_backward(const fa_backward_args* args);
 
+/* ---------------------------------------------------------------------------
+ * fa_rope: rotary positions of q and k, the step before fa_prefill; with `inverse` its
+ * gradient.  No reference counterpart (the reference's programs start from Q, K, V).
+ *
+ * Pair i (i < rotary_dim / 2) of a row at position p turns by p * inv_freq[i] radians:
+ *     (x1, x2) -> amplitude * (x1 cos - x2 sin, x2 cos + x1 sin)
+ * with x1, x2 the elements i and i + rotary_dim / 2 of the row (interleaved = 0) or 2i and
+ * 2i + 1 (interleaved = 1); elements from rotary_dim on are copied.  The angle is reduced in
+ * 64-bit fixed point, so positions may be any int32 and far ones lose nothing; cos and sin
+ * are computed in 64 bits and rounded to 32, each product and the sum of the two are
+ * rounded to 32 bits, the result to the tensor's type.
+ *
+ * fa_rotary::inv_freq is a HOST array of rotary_dim / 2 doubles, read during the call (a
+ * captured graph keeps the values).  rotary_dim: a multiple of 16, at most d_head.
+ * ------------------------------------------------------------------------- */
+typedef struct fa_rotary {
+    const double* inv_freq;       /* host */
+    int           rotary_dim;     /* fa_cache_append: 0 = no rotation */
+    int           interleaved;    /* 0 / 1 */
+    float         amplitude;      /* finite; 1 without attention scaling */
+} fa_rotary;
+
+/* Offsets in elements of entry (batch, head, row) of a tensor whose last dimension is
+ * contiguous; multiples of 8.  All zero = dense [B, H, S, D]. */
+typedef struct fa_strides {
+    long long batch;
+    long long head;
+    long long row;
+} fa_strides;
+
+typedef struct fa_rope_args {
+    const void* q;                /* [B, Hq, S, D] by q_strides */
+    const void* k;                /* [B, Hkv, S, D], or NULL (then num_kv_heads is 0) */
+    void*       q_out;            /* may be q itself, with the same strides */
+    void*       k_out;
+    fa_strides  q_strides, k_strides, q_out_strides, k_out_strides;
+    int         batch_size;
+    int         num_q_heads;
+    int         num_kv_heads;
+    int         seq_len;
+    int         d_head;           /* 64 or 128 */
+    int         dtype;            /* FA_DTYPE_F16 or FA_DTYPE_BF16 */
+    const int*  positions;        /* device; NULL = row s has position position_offset + s */
+    int         positions_stride; /* between sequences; 0 = all sequences share [S] positions */
+    int         position_offset;
+    int         inverse;          /* 1: turn by the negative angles (the transposed map) */
+    fa_rotary   rotary;
+    void*       stream;
+} fa_rope_args;
+
+int fa_rope(const fa_rope_args* args);
+
+/*
+ * Frequencies for fa_rotary on the host (no device is touched): writes rotary_dim / 2 doubles
+ * and, if amplitude is not NULL, the amplitude that goes with them.  f_i = base^(-2i/rotary_dim) and
+ *   FA_ROPE_PLAIN     f_i
+ *   FA_ROPE_LINEAR    f_i / factor  (positions interpolated)
+ *   FA_ROPE_BASE      f_i with base * factor^(rotary_dim / (rotary_dim - 2)): the slowest pair turns
+ *                     `factor` times slower, the fastest as before
+ *   FA_ROPE_PARTS     f_i / factor and f_i mixed by how often the pair turns over original_length
+ *                     positions: at least `fast` turns keep f_i, at most `slow` turns take
+ *                     f_i / factor, linear in the pair's index between (borders rounded outwards);
+ *                     amplitude 0.1 ln(factor) + 1
+ *   FA_ROPE_SMOOTH    the same mix, linear in the number of turns between `slow` and `fast`; amplitude 1
+ */
+enum { FA_ROPE_PLAIN = 0, FA_ROPE_LINEAR = 1, FA_ROPE_BASE = 2, FA_ROPE_PARTS = 3, FA_ROPE_SMOOTH = 4 };
+typedef struct fa_rope_scaling {
+    int    kind;
+    double base;                  /* > 1 */
+    double factor;                /* >= 1; not used by FA_ROPE_PLAIN */
+    double original_length;       /* FA_ROPE_PARTS, FA_ROPE_SMOOTH: positions of the unscaled range */
+    double slow, fast;            /* same: 0 < slow < fast */
+} fa_rope_scaling;
+int fa_rope_inv_freq(const fa_rope_scaling* scaling, int rotary_dim, double* inv_freq, float* amplitude);
+
+/* ---------------------------------------------------------------------------
+ * Caches of fa_cache_append, fa_cache_read_u4 and fa_decode_gqa_u4.  A block is a whole
+ * sequence, or a page if block_table is given; row r of KV head h lies in block c at
+ *     c * block_stride + h * head_stride + (row within the block) * row_stride
+ * The strides count elements (FA_CACHE_16BIT, FA_CACHE_E4M3) or bytes (FA_CACHE_U4) and are
+ * multiples of 16 bytes; a row is contiguous.  K and V share them.  Pages are those of
+ * fa_decode_gqa: page_size a power of two >= 16, block_table[b * block_table_stride + r / page_size]
+ * the page of row r.  Entries past a sequence's end are not read.  A page number outside
+ * [0, num_pages) names no page: rows in it are not written and read as zero.
+ * seq_lens [B] (device, optional): length of each sequence, clamped to [0, seq_len_kv]; without it
+ * every sequence has seq_len_kv rows.
+ *
+ * FA_CACHE_U4, a cache in 4 bits: two codes to a byte, the even element of the row in the low
+ * half; every 64 elements have a pair (scale, offset) of fp16, value = offset + scale * code, code
+ * 0..15.  4.5 bits an element.  The pairs of a row are contiguous (d_head / 64 of them); the
+ * param strides count pairs and are multiples of d_head / 64.  What fa_cache_append stores, with
+ * x the 16-bit element (clamped to +-65504, a NaN makes its 64 elements NaN):
+ *     offset = fp16(min x), scale = fp16((max x - offset) / 15),
+ *     code = round((x - offset) * (1 / scale)) in 0..15, ties to even (0 where scale = 0)
+ * all in 32-bit arithmetic with one rounding an operation, the division by 15 a product with
+ * fp32(1/15).
+ * ------------------------------------------------------------------------- */
+enum { FA_CACHE_16BIT = 0, FA_CACHE_E4M3 = 1, FA_CACHE_U4 = 2 };
+typedef struct fa_cache_layout {
+    long long  block_stride, head_stride, row_stride;
+    long long  param_block_stride, param_head_stride, param_row_stride;   /* FA_CACHE_U4 only */
+    const int* block_table;        /* device; NULL = a block is a sequence */
+    int        block_table_stride;
+    int        page_size;
+    int        num_pages;
+    const int* seq_lens;           /* device, optional */
+} fa_cache_layout;
+
+/*
+ * fa_cache_append: the newest num_tokens = T tokens of each sequence into its KV cache, with the
+ * rotation of q and k on the way; the step before fa_decode_gqa / fa_decode_gqa_u4, whose tokens
+ * are likewise the last T rows of each sequence: token t goes to row len - T + t, and that is its
+ * position unless `positions` gives another.  A token without a row (len < T), or before the
+ * last num_new[b] tokens of its sequence (a left-padded batch), is not stored.
+ *
+ *   q (optional) [B, T, Hq, D], k, v [B, T, Hkv, D] in `dtype` (f16 or bf16); the heads of a token are
+ *       contiguous, tokens lie token_stride elements apart (multiples of 8, 0 = dense), so that the three
+ *       can be parts of one projection's output.
+ *   q_out [B, T, Hq, D] dense: rotated q, in `dtype`; for an e4m3 cache its codes, rounded from the
+ *       rotated 16-bit value times 1 / q_scale[b * Hkv + kv head].  Zero for tokens that are not
+ *       stored.  May be q itself if q is dense and the cache is not e4m3.
+ *   k rotated and v go into the caches: FA_CACHE_16BIT in `dtype`; FA_CACHE_E4M3 (d_head 128) as codes of
+ *       the 16-bit value times 1 / {k,v}_scale[b * Hkv + kv head], saturating; FA_CACHE_U4 as above.
+ * Everything else in the caches stays as it is.
+ */
+typedef struct fa_cache_append_args {
+    const void*     q;
+    const void*     k;
+    const void*     v;
+    void*           q_out;
+    void*           k_cache;
+    void*           v_cache;
+    void*           k_params;      /* FA_CACHE_U4: fp16 pairs */
+    void*           v_params;
+    long long       q_token_stride, k_token_stride, v_token_stride;
+    int             batch_size;
+    int             num_tokens;
+    int             num_q_heads;   /* 0 without q; a multiple of num_kv_heads */
+    int             num_kv_heads;
+    int             seq_len_kv;
+    int             d_head;        /* 64 or 128 */
+    int             dtype;
+    int             cache;         /* FA_CACHE_* */
+    fa_cache_layout layout;
+    const int*      num_new;       /* device [B], optional */
+    const int*      positions;     /* device [B, T], optional */
+    fa_rotary       rotary;
+    const float*    q_scale;       /* FA_CACHE_E4M3 only */
+    const float*    k_scale;
+    const float*    v_scale;
+    void*           stream;
+} fa_cache_append_args;
+
+int fa_cache_append(const fa_cache_append_args* args);
+
+/*
+ * fa_cache_read_u4: num_rows rows of each sequence from a 4-bit cache as 16-bit values,
+ * offset + scale * code rounded once (f16: at most 65504).  k_out, v_out: [B, num_rows, Hkv, D] dense in `dtype`; row n is the
+ * cache's row first_rows[b] + n (device [B]; NULL = 0), zero where the sequence has no such row.
+ * For a prefix that the 16-bit entry points take, a cache that moves, or a check.
+ */
+typedef struct fa_cache_read_args {
+    const void*     k_cache;
+    const void*     k_params;
+    const void*     v_cache;
+    const void*     v_params;
+    void*           k_out;
+    void*           v_out;
+    int             batch_size;
+    int             num_kv_heads;
+    int             seq_len_kv;
+    int             d_head;        /* 64 or 128 */
+    int             num_rows;
+    int             dtype;         /* of the outputs: f16 or bf16 */
+    fa_cache_layout layout;
+    const int*      first_rows;
+    void*           stream;
+} fa_cache_read_args;
+
+int fa_cache_read_u4(const fa_cache_read_args* args);
+
 /*
  * LSE merge of n_parts partial results (the exchange step of KV-sequence
  * sharded decode: each rank's (o_f32, lse) gathered into one local buffer).
