@@ -46,7 +46,8 @@ EXPORTED_SYMBOLS = (
     "fa_clear_device_status", "fa_error_string", "fa_last_cuda_error", "fa_version",
     "fa_set_prefill_variant", "fa_combine_packed", "fa_decode_kv_sharded", "fa_decode_kv_sharded_gather_bytes",
     "fa_nccl_unique_id", "fa_nccl_comm_create", "fa_nccl_comm_destroy", "fa_status_word_to_error",
-    "fa_rope", "fa_rope_inv_freq", "fa_cache_append", "fa_cache_read_u4",
+    "fa_rope", "fa_rope_inv_freq", "fa_cache_append", "fa_cache_read_u4", "fa_decode_gqa_u4",
+    "fa_decode_gqa_u4_workspace_bytes",
 )
 
 
@@ -174,6 +175,18 @@ class CacheReadArgs(ctypes.Structure):
     ]
 
 
+class DecodeGqaU4Args(ctypes.Structure):
+    """Mirror of ``fa_decode_gqa_u4_args`` (include/fa_b200.h)."""
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k_cache", ctypes.c_void_p), ("k_params", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p), ("v_params", ctypes.c_void_p), ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("batch_size", ctypes.c_int), ("num_q_heads", ctypes.c_int), ("num_kv_heads", ctypes.c_int),
+        ("num_q_tokens", ctypes.c_int), ("seq_len_kv", ctypes.c_int), ("d_head", ctypes.c_int), ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int), ("layout", CacheLayout),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
+    ]
+
+
 class FaError(RuntimeError):
     def __init__(self, code: int, what: str):
         super().__init__(f"{what}: {error_string(code)} ({code})"
@@ -253,6 +266,10 @@ def lib() -> ctypes.CDLL:
         l.fa_cache_append.argtypes = [ctypes.POINTER(CacheAppendArgs)]
         l.fa_cache_read_u4.restype = ctypes.c_int
         l.fa_cache_read_u4.argtypes = [ctypes.POINTER(CacheReadArgs)]
+        l.fa_decode_gqa_u4.restype = ctypes.c_int
+        l.fa_decode_gqa_u4.argtypes = [ctypes.POINTER(DecodeGqaU4Args)]
+        l.fa_decode_gqa_u4_workspace_bytes.restype = ctypes.c_size_t
+        l.fa_decode_gqa_u4_workspace_bytes.argtypes = [ctypes.c_int] * 6
         _lib = l
     return _lib
 
@@ -475,6 +492,29 @@ def cache_read_u4(*args, **kw) -> None:
     rc = cache_read_u4_raw(*args, **kw)
     if rc != FA_OK:
         raise FaError(rc, "fa_cache_read_u4")
+
+
+def decode_gqa_u4_workspace_bytes(batch_size, num_q_heads, num_kv_heads, num_q_tokens, seq_len_kv, d_head) -> int:
+    return lib().fa_decode_gqa_u4_workspace_bytes(batch_size, num_q_heads, num_kv_heads, num_q_tokens, seq_len_kv, d_head)
+
+
+def decode_gqa_u4_raw(q, k_cache, k_params, v_cache, v_params, o, lse, batch_size, num_q_heads, num_kv_heads, seq_len_kv,
+                      d_head, scale, dtype="f16", num_q_tokens=0, kv_strides=(0, 0, 0), param_strides=(0, 0, 0),
+                      block_table=None, block_table_stride=0, page_size=0, num_pages=0, seq_lens=None, workspace=None,
+                      workspace_bytes=0, stream=None) -> int:
+    """fa_decode_gqa_u4; the cache is described as for cache_append.  Returns the status code."""
+    a = DecodeGqaU4Args(_ptr(q), _ptr(k_cache), _ptr(k_params), _ptr(v_cache), _ptr(v_params), _ptr(o), _ptr(lse), batch_size,
+                        num_q_heads, num_kv_heads, num_q_tokens, seq_len_kv, d_head, scale,
+                        DTYPES[dtype] if isinstance(dtype, str) else dtype,
+                        _layout(kv_strides, param_strides, block_table, block_table_stride, page_size, num_pages, seq_lens),
+                        _ptr(workspace), workspace_bytes, _stream_handle(stream))
+    return lib().fa_decode_gqa_u4(ctypes.byref(a))
+
+
+def decode_gqa_u4(*args, **kw) -> None:
+    rc = decode_gqa_u4_raw(*args, **kw)
+    if rc != FA_OK:
+        raise FaError(rc, "fa_decode_gqa_u4")
 
 
 def combine(o_parts, lse_parts, n_parts, rows, d_head, o, lse, dtype="f16", stream=None) -> None:

@@ -1,0 +1,810 @@
+// Grouped-query attention of the newest token(s) over a KV cache held in 4 bits (u4.cuh).
+//
+// The reference has no cache; the definition is its attention (src/demo.cu:28-70) over the values
+// K^ = z + s c, V^ = z + s c of the cache, for query rows that see the keys up to their own position.
+//
+// Mathematics.  With codes c in 0..15 and a (scale s, offset z) for each 64 elements of a key (group g of the row):
+//     S = scale * sum_g [ s_g sum_d q_d (c_d - 8) + (z_g + 8 s_g) sum_d q_d ]
+//     O = sum_k P_k V^_k  with  V^_k = s_kg (c_kd - 8) + (z_kg + 8 s_kg)
+//       = 2^E sum_k [P_k s_kg 2^-E] (c_kd - 8)  +  sum_k P_k (z_kg + 8 s_kg)
+// The sums over d and over k with c run on the tensor core: c - 8 is a whole number, exact in both 16-bit types, q is
+// the caller's 16-bit q, and the bracket is rounded to fp16, the one rounding on the way to O (2^-12 of a term, half
+// a step; 2^E follows the scales so that no bracket leaves fp16).  Everything else is held in 32 bits.
+//
+// What bounds it.  With a few query rows a key (T * group) HBM does: 4.5 bits an element.  The codes must be unpacked
+// between memory and tensor core, and the registers are where that costs no second trip through shared memory;
+// tcgen05.mma takes no operand from registers, and unpacked keys in shared memory would be 4 times the bytes that
+// came in, written and read back.  So the products are mma.sync m16n8k16 with the unpacked codes as the register operand A:
+// keys are the rows of S^T = K Q^T, head elements the rows of O^T = V^T P^T, and a query row takes one of 8 columns.
+//
+// Work split.  All (sequence, KV head, row block) items are laid out one after the other in tiles of 32 keys, and the
+// resulting line is cut into equal parts, one for each warp of the GPU, whatever the lengths of the sequences: a warp may
+// finish one item, do several and begin the next.  A warp streams its tiles through a cp.async ring of its own and meets
+// the others only once, at the end, where the CTA merges what its warps have of the same item.  Items that lie in
+// several CTAs go through the workspace and a second small kernel.
+#include <cmath>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "host_common.h"
+#include "ptx.cuh"
+#include "u4.cuh"
+
+namespace fa {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kKeys = 32;                      // keys of a tile
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kGrow = 8.0f;                  // a running max may be exceeded by this much (in powers of two) before it is raised
+
+struct U4Args {
+    const uint16_t* q;
+    const uint8_t *k, *v;
+    const __half2 *kp, *vp;
+    uint16_t* o;
+    float* lse;
+    float* scratch;                            // head records of the warps, then two records a CTA
+    int2* meta;                                // per CTA: item of the tail record or -1; head record: 0 none, 1 ends here, 2 goes on
+    long long block_stride, head_stride, row_stride;          // bytes
+    long long p_block_stride, p_head_stride, p_row_stride;    // pairs
+    CacheMap map;
+    const int* seq_lens;
+    int batch, hq, hkv, group, n_tok, rows, row_blocks, kv_len;
+    float scale_log2;
+};
+
+// Shapes of an instance: D, row columns of 8.
+template <int D, int NT>
+struct Shape {
+    static constexpr int G = D / kU4Group;                     // groups of a row
+    static constexpr int RowBytes = D / 2;
+    static constexpr int Stages = NT == 4 ? 4 : 3;
+    static constexpr int CodeBytes = kKeys * RowBytes;
+    static constexpr int ParamBytes = kKeys * G * 4;
+    static constexpr int StageBytes = 2 * CodeBytes + 2 * ParamBytes;
+    static constexpr int WarpBytes = Stages * StageBytes;
+    static constexpr int Rows = 8 * NT;
+    static constexpr int Record = Rows * (D + 2);              // floats: O [row][D], then m [row], l [row]
+    static_assert(Record * 4 <= WarpBytes, "a record fits the ring it replaces");
+    static constexpr int CtasPerSm = NT == 1 ? 2 : 1;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(valid ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t r;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(a));
+    return r;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 r;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
+    return r;
+}
+
+// D = A B + C, m16n8k16, fp32 accumulation.
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// An 8 x 8 tile of 16-bit values, rows to columns, across the warp.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// Nibble N (0..3) of both halves of `x` as the 16-bit value 16 + code: the code lies in the top four bits of the
+// mantissa of 16.0.
+template <bool BF16, int N>
+__device__ __forceinline__ uint32_t code16(uint32_t x) {
+    constexpr int at = BF16 ? 3 : 6, shift = at - 4 * N;
+    constexpr uint32_t mask = 0x000F000Fu << at, one = BF16 ? 0x41804180u : 0x4C004C00u;
+    const uint32_t y = shift >= 0 ? x << (shift >= 0 ? shift : 0) : x >> (shift >= 0 ? 0 : -shift);
+    return (y & mask) | one;
+}
+// The same minus 24: code - 8, exact.
+__device__ __forceinline__ uint32_t centred(uint32_t x) {
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(24.0f, 24.0f));
+    return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// Place of key r's row in a tile of V codes: a permutation of rows (and of 32-byte halves, d_head 128) under which the
+// reads below touch every bank once.  Within 8 keys the rows 0, 2, 4, 6 | 1, 3, 5, 7 follow one another.
+__device__ __forceinline__ int v_row(int r) { return (r & ~7) | ((r & 1) << 2) | ((r >> 1) & 3); }
+
+struct Item {
+    int b, h, rb, len, tiles;      // sequence, KV head, row block, its keys, tiles of 32 of them (at least one)
+};
+__device__ __forceinline__ int tiles_of(int len) { return max(1, (len + kKeys - 1) / kKeys); }
+
+template <int D, bool BF16, int NT>
+__global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kernel(const __grid_constant__ U4Args a) {
+    using S = Shape<D, NT>;
+    constexpr int G = S::G;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ long long s_prefix[kWarps * 32];                // tiles (of one head and row block) before a thread's sequences
+    __shared__ long long s_total;
+    __shared__ int s_head_item[kWarps], s_tail_item[kWarps], s_before[kWarps], s_after[kWarps];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    grid_dependency_wait();
+    grid_launch_dependents();
+
+    // ---- the line of tiles, and this warp's part of it
+    const int per_b = a.hkv * a.row_blocks;                    // items of a sequence
+    const int per_thread = (a.batch + kWarps * 32 - 1) / (kWarps * 32);   // sequences of a thread
+    if (a.seq_lens != nullptr) {
+        long long sum = 0;
+        for (int i = 0; i < per_thread; i++) {
+            const int b = tid * per_thread + i;
+            if (b < a.batch) sum += tiles_of(sequence_length(a.seq_lens, b, a.kv_len));
+        }
+        long long inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        __shared__ long long s_warp[kWarps];
+        if (lane == 31) s_warp[warp] = inc;
+        __syncthreads();
+        long long base = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            if (w < warp) base += s_warp[w];
+            total += s_warp[w];
+        }
+        s_prefix[tid] = base + inc - sum;
+        if (tid == 0) s_total = total;
+    } else if (tid == 0) {
+        s_total = (long long)a.batch * tiles_of(a.kv_len);
+    }
+    __syncthreads();
+    const long long total = s_total * per_b;
+    // equal parts of at least one tile a warp: CTAs without tiles come last, so those of an item follow one another
+    const long long chunk = max((total + gridDim.x - 1) / gridDim.x, (long long)kWarps);
+    const long long c_begin = min(total, chunk * blockIdx.x), c_end = min(total, c_begin + chunk);
+    const long long w_begin = c_begin + (c_end - c_begin) * warp / kWarps, w_end = c_begin + (c_end - c_begin) * (warp + 1) / kWarps;
+
+    const uint32_t ring = smem_u32(smem) + warp * S::WarpBytes;
+    float* tail_record = reinterpret_cast<float*>(smem + warp * S::WarpBytes);
+    float* head_record = a.scratch + (size_t)(blockIdx.x * kWarps + warp) * S::Record;
+    int head_item = -1, tail_item = -1, before = 0, after = 0;
+
+    Item it{0, 0, 0, 0, 0};
+    long long item_start = 0;
+    if (w_begin < w_end) {
+        long long b_start;                                     // first tile of sequence it.b
+        if (a.seq_lens == nullptr) {
+            it.tiles = tiles_of(a.kv_len);
+            it.len = a.kv_len;
+            it.b = (int)(w_begin / ((long long)it.tiles * per_b));
+            b_start = (long long)it.b * it.tiles * per_b;
+        } else {
+            int lo = 0, hi = kWarps * 32 - 1;                  // last thread whose sequences begin at or before w_begin
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (s_prefix[mid] * per_b <= w_begin && mid * per_thread < a.batch) lo = mid;
+                else hi = mid - 1;
+            }
+            it.b = lo * per_thread;
+            b_start = s_prefix[lo] * per_b;
+            for (;;) {
+                it.len = sequence_length(a.seq_lens, it.b, a.kv_len);
+                it.tiles = tiles_of(it.len);
+                const long long end = b_start + (long long)it.tiles * per_b;
+                if (w_begin < end || it.b + 1 >= a.batch) break;
+                b_start = end;
+                it.b++;
+            }
+        }
+        const int i = (int)((w_begin - b_start) / it.tiles);   // item of the sequence
+        it.h = i / a.row_blocks;
+        it.rb = i - it.h * a.row_blocks;
+        item_start = b_start + (long long)i * it.tiles;
+    }
+
+    // ---- item by item
+    for (long long x = w_begin; x < w_end;) {
+        const int tile0 = (int)(x - item_start);
+        const int tile1 = (int)min((long long)it.tiles, tile0 + (w_end - x));
+        const int row0 = it.rb * S::Rows;
+
+        // q as operand B: column g of the n-th 8 rows; a word of 8 codes is two steps of k, its pairs (i, i + 4)
+        uint32_t qf[NT][G][2][4];
+        float q_sum[NT][G][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int r = row0 + n * 8 + g;
+            const int tok = r / a.group, hh = r - tok * a.group;
+            const uint16_t* qp = a.q + (((long long)it.b * a.n_tok + tok) * a.hq + (long long)it.h * a.group + hh) * D;
+#pragma unroll
+            for (int gi = 0; gi < G; gi++) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    uint4 u = make_uint4(0, 0, 0, 0);
+                    if (r < a.rows) u = *reinterpret_cast<const uint4*>(qp + gi * kU4Group + t * 16 + w * 8);
+                    const float2 f0 = unpack16<BF16>(u.x), f1 = unpack16<BF16>(u.y), f2 = unpack16<BF16>(u.z), f3 = unpack16<BF16>(u.w);
+                    sum += ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
+                    qf[n][gi][w][0] = __byte_perm(u.x, u.z, 0x5410);
+                    qf[n][gi][w][1] = __byte_perm(u.x, u.z, 0x7632);
+                    qf[n][gi][w][2] = __byte_perm(u.y, u.w, 0x5410);
+                    qf[n][gi][w][3] = __byte_perm(u.y, u.w, 0x7632);
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                q_sum[n][gi][0] = __shfl_sync(0xffffffffu, sum, 8 * t);          // of the columns that this thread has in S^T
+                q_sum[n][gi][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+            }
+        }
+
+        // ---- loads of a tile
+        const long long h_off = (long long)it.h * a.head_stride, hp_off = (long long)it.h * a.p_head_stride;
+        auto page_of = [&](int key) -> int {                   // -1: names none, or past the end
+            if (key >= it.len) return -1;
+            if (a.map.page_shift < 0) return it.b;
+            const int p = a.map.block_table[(long long)it.b * a.map.table_stride + (key >> a.map.page_shift)];
+            return (unsigned)p < (unsigned)a.map.n_pages ? p : -1;
+        };
+        const int in_page = a.map.page_shift < 0 ? 0x7FFFFFFF : (1 << a.map.page_shift) - 1;
+        auto load_tile = [&](int tile, int stage, int p0, int p1) {
+            const int k0 = tile * kKeys;
+            const uint32_t dst = ring + stage * S::StageBytes;
+            constexpr int CPR = S::RowBytes / 16, RPI = 32 / CPR;              // 16-byte pieces of a row, rows an instruction
+#pragma unroll
+            for (int i = 0; i < kKeys / RPI; i++) {
+                const int r = i * RPI + lane / CPR, c = lane % CPR, key = k0 + r;
+                const int p = r < 16 ? p0 : p1;
+                const bool ok = key < it.len && p >= 0;
+                const long long off = ok ? p * a.block_stride + h_off + (long long)(key & in_page) * a.row_stride + c * 16 : 0;
+                const int ck = D == 128 ? c ^ (((r >> 1) & 1) << 1) : c, cv = D == 128 ? c ^ (((r >> 2) & 1) << 1) : c;
+                cp_async_16(dst + r * S::RowBytes + ck * 16, a.k + off, ok);
+                cp_async_16(dst + S::CodeBytes + v_row(r) * S::RowBytes + cv * 16, a.v + off, ok);
+            }
+            const int key = k0 + lane, p = lane < 16 ? p0 : p1;
+            const bool ok = key < it.len && p >= 0;
+            const long long off = ok ? p * a.p_block_stride + hp_off + (long long)(key & in_page) * a.p_row_stride : 0;
+            cp_async_small<4 * G>(dst + 2 * S::CodeBytes + lane * 4 * G, a.kp + off, ok);
+            cp_async_small<4 * G>(dst + 2 * S::CodeBytes + S::ParamBytes + lane * 4 * G, a.vp + off, ok);
+        };
+
+        float o[NT][G][4][4], l[NT][2], m[NT][2], zs[NT][G][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int gi = 0; gi < G; gi++) {
+                zs[n][gi][0] = zs[n][gi][1] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[n][gi][i][e] = 0.0f;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; c++) { l[n][c] = 0.0f; m[n][c] = -INFINITY; }
+        }
+        float s_limit = 0.0f, s_down = 0.0f;                   // 128 * 2^E, 2^-E of V's scales
+
+        int next_p0 = page_of(tile0 * kKeys), next_p1 = page_of(tile0 * kKeys + 16);
+#pragma unroll
+        for (int i = 0; i < S::Stages - 1; i++) {
+            if (tile0 + i < tile1) {
+                const int p0 = next_p0, p1 = next_p1;
+                if (tile0 + i + 1 < tile1) { next_p0 = page_of((tile0 + i + 1) * kKeys); next_p1 = page_of((tile0 + i + 1) * kKeys + 16); }
+                load_tile(tile0 + i, i, p0, p1);
+            }
+            cp_async_commit();
+        }
+        const int first_hidden = it.len - a.n_tok + row0 / a.group + 1;       // first key that the block's first token does not see
+        int stage = 0, load_stage = S::Stages - 1;
+        for (int tile = tile0; tile < tile1; tile++) {
+            cp_async_wait<S::Stages - 2>();
+            __syncwarp();                                      // every lane's copies have landed, and nobody reads the oldest stage any more
+            if (tile + S::Stages - 1 < tile1) {
+                const int p0 = next_p0, p1 = next_p1;
+                if (tile + S::Stages < tile1) { next_p0 = page_of((tile + S::Stages) * kKeys); next_p1 = page_of((tile + S::Stages) * kKeys + 16); }
+                load_tile(tile + S::Stages - 1, load_stage, p0, p1);
+            }
+            cp_async_commit();
+            load_stage = load_stage + 1 == S::Stages ? 0 : load_stage + 1;
+            const uint32_t kb = ring + stage * S::StageBytes, vb = kb + S::CodeBytes, kpb = kb + 2 * S::CodeBytes, vpb = kpb + S::ParamBytes;
+            stage = stage + 1 == S::Stages ? 0 : stage + 1;
+
+            // S^T: keys j * 16 + g and + 8, columns 2t and 2t + 1 of each 8 rows
+            float s[2][NT][4];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float acc[G][NT][4];
+#pragma unroll
+                for (int gi = 0; gi < G; gi++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[gi][n][e] = -24.0f * q_sum[n][gi][e & 1];
+                const int r0 = j * 16 + g, r1 = r0 + 8;
+                const uint32_t swap = D == 128 ? ((g >> 1) & 1) * 32 : 0;
+#pragma unroll
+                for (int gi = 0; gi < G; gi++) {
+                    const uint2 x0 = lds64(kb + r0 * S::RowBytes + ((gi * 32) ^ swap) + t * 8), x1 = lds64(kb + r1 * S::RowBytes + ((gi * 32) ^ swap) + t * 8);
+#pragma unroll
+                    for (int w = 0; w < 2; w++) {
+                        const uint32_t w0 = w ? x0.y : x0.x, w1 = w ? x1.y : x1.x;
+                        const uint32_t a0[4] = {code16<BF16, 0>(w0), code16<BF16, 0>(w1), code16<BF16, 1>(w0), code16<BF16, 1>(w1)};
+                        const uint32_t a1[4] = {code16<BF16, 2>(w0), code16<BF16, 2>(w1), code16<BF16, 3>(w0), code16<BF16, 3>(w1)};
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            mma<BF16>(acc[gi][n], a0, qf[n][gi][w][0], qf[n][gi][w][1]);
+                            mma<BF16>(acc[gi][n], a1, qf[n][gi][w][2], qf[n][gi][w][3]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int e2 = 0; e2 < 2; e2++) {               // keys r0, r1
+                    uint2 pr;
+                    if constexpr (G == 2) pr = lds64(kpb + (e2 ? r1 : r0) * 8);
+                    else pr = make_uint2(lds32(kpb + (e2 ? r1 : r0) * 4), 0u);
+                    float ks[G], kz[G];
+#pragma unroll
+                    for (int gi = 0; gi < G; gi++) {
+                        const uint32_t u = gi ? pr.y : pr.x;
+                        const float2 f = unpack16<false>(u);
+                        ks[gi] = f.x;
+                        kz[gi] = fmaf(8.0f, f.x, f.y);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            float v = kz[0] * q_sum[n][0][c];
+                            if constexpr (G == 2) v = fmaf(kz[1], q_sum[n][1][c], v);
+                            v = fmaf(ks[0], acc[0][n][e2 * 2 + c], v);
+                            if constexpr (G == 2) v = fmaf(ks[1], acc[G - 1][n][e2 * 2 + c], v);
+                            s[j][n][e2 * 2 + c] = v;
+                        }
+                }
+            }
+            // masked keys: past what the row's token sees (only the last tiles have any)
+            if ((tile + 1) * kKeys > first_hidden) {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const int limit = it.len - a.n_tok + (row0 + n * 8 + 2 * t + c) / a.group + 1 - tile * kKeys;
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+#pragma unroll
+                            for (int e2 = 0; e2 < 2; e2++)
+                                if (j * 16 + e2 * 8 + g >= limit || tile * kKeys + j * 16 + e2 * 8 + g >= it.len) s[j][n][e2 * 2 + c] = -INFINITY;
+                    }
+            }
+            // V's scales and offsets of this thread's keys
+            float vs[2][2][G], vz[2][2][G], s_max = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int e2 = 0; e2 < 2; e2++) {
+                    uint2 pr;
+                    if constexpr (G == 2) pr = lds64(vpb + (j * 16 + e2 * 8 + g) * 8);
+                    else pr = make_uint2(lds32(vpb + (j * 16 + e2 * 8 + g) * 4), 0u);
+#pragma unroll
+                    for (int gi = 0; gi < G; gi++) {
+                        const float2 f = unpack16<false>(gi ? pr.y : pr.x);
+                        vs[j][e2][gi] = f.x;
+                        vz[j][e2][gi] = fmaf(8.0f, f.x, f.y);
+                        s_max = fmaxf(s_max, f.x);
+                    }
+                }
+            // the running max may be exceeded by 2^8, the scales' reference by 2^3, before the sums are brought to new ones
+            float t_max[NT][2];
+            bool raise = s_max > s_limit;
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    t_max[n][c] = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
+                    raise |= (t_max[n][c] - m[n][c]) * a.scale_log2 > kGrow || (m[n][c] == -INFINITY && t_max[n][c] > -INFINITY);
+                }
+            if (__any_sync(0xffffffffu, raise)) {
+                float ratio = 1.0f;
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) s_max = fmaxf(s_max, __shfl_xor_sync(0xffffffffu, s_max, off));
+                if (s_max > s_limit) {
+                    // 2^-E such that the largest scale becomes 16 .. 32: with P up to 2^8 and scales up to 2^7 a bracket stays below 2^15
+                    const float down = __uint_as_float(((254u + 4u) << 23) - (__float_as_uint(s_max) & 0x7F800000u));
+                    ratio = s_down == 0.0f ? 1.0f : down / s_down;
+                    s_down = down;
+                    s_limit = 128.0f / down;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        float mx = t_max[n][c];
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                        mx = fmaxf(mx, m[n][c]);
+                        const float alpha = m[n][c] == -INFINITY ? 1.0f : ex2((m[n][c] - mx) * a.scale_log2);   // nothing summed so far: leave it
+                        m[n][c] = mx;
+                        l[n][c] *= alpha;
+#pragma unroll
+                        for (int gi = 0; gi < G; gi++) {
+                            zs[n][gi][c] *= alpha;
+#pragma unroll
+                            for (int i = 0; i < 4; i++) { o[n][gi][i][c] *= alpha * ratio; o[n][gi][i][2 + c] *= alpha * ratio; }
+                        }
+                    }
+            }
+            // P, its sums, and the brackets as operand B: columns to rows across the warp
+            uint32_t pf[2][NT][G][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const float mc0 = m[n][0] == -INFINITY ? 0.0f : m[n][0] * a.scale_log2, mc1 = m[n][1] == -INFINITY ? 0.0f : m[n][1] * a.scale_log2;
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int e2 = 0; e2 < 2; e2++) {
+                        const float p0 = ex2(fmaf(s[j][n][e2 * 2], a.scale_log2, -mc0)), p1 = ex2(fmaf(s[j][n][e2 * 2 + 1], a.scale_log2, -mc1));
+                        l[n][0] += p0;
+                        l[n][1] += p1;
+#pragma unroll
+                        for (int gi = 0; gi < G; gi++) {
+                            zs[n][gi][0] = fmaf(p0, vz[j][e2][gi], zs[n][gi][0]);
+                            zs[n][gi][1] = fmaf(p1, vz[j][e2][gi], zs[n][gi][1]);
+                            const float sd = vs[j][e2][gi] * s_down;
+                            pf[j][n][gi][e2] = transpose8x8(pack16<false>(p0 * sd, p1 * sd));
+                        }
+                    }
+            }
+            // O^T: elements 8g .. 8g + 7 of each group, a pair of them per product of 16 rows
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int ra = j * 16 + 2 * t;
+                const uint32_t row_a = vb + v_row(ra) * S::RowBytes, row_b = vb + v_row(ra + 1) * S::RowBytes;
+                const uint32_t row_c = vb + v_row(ra + 8) * S::RowBytes, row_d = vb + v_row(ra + 9) * S::RowBytes;
+#pragma unroll
+                for (int gi = 0; gi < G; gi++) {
+                    const uint32_t at = (D == 128 ? ((gi ^ (t >> 1)) & 1) * 32 : 0) + g * 4;
+                    const uint32_t xa = lds32(row_a + at), xb = lds32(row_b + at), xc = lds32(row_c + at), xd = lds32(row_d + at);
+#pragma unroll
+                    for (int hf = 0; hf < 2; hf++) {           // elements 0..3, 4..7
+                        const uint32_t y0 = __byte_perm(xa, xb, hf ? 0x7632 : 0x5410), y1 = __byte_perm(xc, xd, hf ? 0x7632 : 0x5410);
+                        const uint32_t a0[4] = {centred(code16<false, 0>(y0)), centred(code16<false, 1>(y0)), centred(code16<false, 0>(y1)), centred(code16<false, 1>(y1))};
+                        const uint32_t a1[4] = {centred(code16<false, 2>(y0)), centred(code16<false, 3>(y0)), centred(code16<false, 2>(y1)), centred(code16<false, 3>(y1))};
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            mma<false>(o[n][gi][2 * hf], a0, pf[j][n][gi][0], pf[j][n][gi][1]);
+                            mma<false>(o[n][gi][2 * hf + 1], a1, pf[j][n][gi][0], pf[j][n][gi][1]);
+                        }
+                    }
+                }
+            }
+        }
+        cp_async_wait<0>();
+        __syncwarp();
+
+        // ---- the item's sums, or this warp's part of them
+        const float up = s_down == 0.0f ? 0.0f : 1.0f / s_down;
+        const bool whole = tile0 == 0 && tile1 == it.tiles;
+        const bool last = x + (tile1 - tile0) >= w_end;
+        const int item = (it.b * a.hkv + it.h) * a.row_blocks + it.rb;
+        float* record = last ? tail_record : head_record;
+        if (!whole) {
+            if (last) tail_item = item;
+            else head_item = item;
+            if (item_start < c_begin) before = 1;     // only the CTA's first item can begin before it, only its last end after it
+            if (item_start + it.tiles > c_end) after = 1;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) {
+                    l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], off);
+#pragma unroll
+                    for (int gi = 0; gi < G; gi++) zs[n][gi][c] += __shfl_xor_sync(0xffffffffu, zs[n][gi][c], off);
+                }
+                const int r = n * 8 + 2 * t + c;
+#pragma unroll
+                for (int gi = 0; gi < G; gi++) {
+                    float f[8];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        f[2 * i] = fmaf(o[n][gi][i][c], up, zs[n][gi][c]);
+                        f[2 * i + 1] = fmaf(o[n][gi][i][2 + c], up, zs[n][gi][c]);
+                    }
+                    if (!whole) {
+                        float4* p = reinterpret_cast<float4*>(record + r * D + gi * kU4Group + g * 8);
+                        p[0] = make_float4(f[0], f[1], f[2], f[3]);
+                        p[1] = make_float4(f[4], f[5], f[6], f[7]);
+                    } else if (row0 + r < a.rows) {
+                        const float inv = l[n][c] == 0.0f ? 0.0f : 1.0f / l[n][c];
+                        const int tok = (row0 + r) / a.group, hh = (row0 + r) - tok * a.group;
+                        const long long row = ((long long)it.b * a.n_tok + tok) * a.hq + (long long)it.h * a.group + hh;
+                        uint4 y;
+                        y.x = pack16<BF16>(f[0] * inv, f[1] * inv);
+                        y.y = pack16<BF16>(f[2] * inv, f[3] * inv);
+                        y.z = pack16<BF16>(f[4] * inv, f[5] * inv);
+                        y.w = pack16<BF16>(f[6] * inv, f[7] * inv);
+                        *reinterpret_cast<uint4*>(a.o + row * D + gi * kU4Group + g * 8) = y;
+                        if (gi == 0 && g == 0 && a.lse != nullptr)
+                            a.lse[row] = l[n][c] == 0.0f ? -INFINITY : kLn2 * (m[n][c] * a.scale_log2 + log2f(l[n][c]));
+                    }
+                }
+                if (!whole && g == 0) {
+                    record[S::Rows * D + r] = m[n][c] == -INFINITY ? -INFINITY : m[n][c] * a.scale_log2;
+                    record[S::Rows * (D + 1) + r] = l[n][c];
+                }
+            }
+        // ---- the next item
+        x += tile1 - tile0;
+        item_start += it.tiles;
+        if (x < w_end) {
+            if (++it.rb == a.row_blocks) {
+                it.rb = 0;
+                if (++it.h == a.hkv) {
+                    it.h = 0;
+                    it.b++;
+                    it.len = sequence_length(a.seq_lens, it.b, a.kv_len);
+                    it.tiles = tiles_of(it.len);
+                }
+            }
+        }
+    }
+
+    // ---- the CTA's records, in the order of the line: head and tail of warp 0, of warp 1, ...
+    if (lane == 0) { s_head_item[warp] = head_item; s_tail_item[warp] = tail_item; s_before[warp] = before; s_after[warp] = after; }
+    __threadfence_block();
+    __syncthreads();
+    int tail_of_cta = -1, head_of_cta = 0;
+    auto item_at = [&](int k) { return k & 1 ? s_tail_item[k >> 1] : s_head_item[k >> 1]; };
+    auto record_at = [&](int k) -> const float* {
+        return k & 1 ? reinterpret_cast<const float*>(smem + (k >> 1) * S::WarpBytes) : a.scratch + (size_t)(blockIdx.x * kWarps + (k >> 1)) * S::Record;
+    };
+    for (int k = 0; k < 2 * kWarps;) {
+        const int item = item_at(k);
+        if (item < 0) { k++; continue; }
+        int end = k + 1;                                       // records of this item: k .. end - 1, with gaps
+        for (int i = k + 1; i < 2 * kWarps; i++) {
+            const int y = item_at(i);
+            if (y == item) end = i + 1;
+            else if (y >= 0) break;
+        }
+        const int rb = item % a.row_blocks, bh = item / a.row_blocks, b = bh / a.hkv, h = bh - b * a.hkv;
+        // it begins before this CTA's part if its first warp says so of its first record, and ends after it likewise
+        const bool starts_before = s_before[k >> 1] != 0 && item == (s_head_item[k >> 1] >= 0 ? s_head_item[k >> 1] : s_tail_item[k >> 1]);
+        const bool ends_after = s_after[(end - 1) >> 1] != 0 && item == (s_tail_item[(end - 1) >> 1] >= 0 ? s_tail_item[(end - 1) >> 1] : s_head_item[(end - 1) >> 1]);
+        float* slot = a.scratch + ((size_t)gridDim.x * kWarps + 2 * blockIdx.x + (starts_before ? 0 : 1)) * S::Record;
+        const bool final_here = !starts_before && !ends_after;
+        if (starts_before) head_of_cta = ends_after ? 2 : 1;
+        else if (ends_after) tail_of_cta = item;
+        for (int i = tid; i < S::Rows * (D / 4); i += kWarps * 32) {
+            const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+            float mx = -INFINITY;
+            for (int y = k; y < end; y++)
+                if (item_at(y) == item) mx = fmaxf(mx, record_at(y)[S::Rows * D + r]);
+            float sum = 0.0f;
+            float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int y = k; y < end; y++)
+                if (item_at(y) == item) {
+                    const float* rec = record_at(y);
+                    const float ym = rec[S::Rows * D + r];
+                    const float w = ym == -INFINITY ? (rec[S::Rows * (D + 1) + r] == 0.0f ? 0.0f : 1.0f) : ex2(ym - mx);
+                    const float4 z = *reinterpret_cast<const float4*>(rec + r * D + d);
+                    sum = fmaf(w, rec[S::Rows * (D + 1) + r], sum);
+                    f.x = fmaf(w, z.x, f.x); f.y = fmaf(w, z.y, f.y); f.z = fmaf(w, z.z, f.z); f.w = fmaf(w, z.w, f.w);
+                }
+            if (!final_here) {
+                *reinterpret_cast<float4*>(slot + r * D + d) = f;
+                if (d == 0) { slot[S::Rows * D + r] = mx; slot[S::Rows * (D + 1) + r] = sum; }
+            } else if (rb * S::Rows + r < a.rows) {
+                const int tok = (rb * S::Rows + r) / a.group, hh = rb * S::Rows + r - tok * a.group;
+                const long long row = ((long long)b * a.n_tok + tok) * a.hq + (long long)h * a.group + hh;
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                uint2 y;
+                y.x = pack16<BF16>(f.x * inv, f.y * inv);
+                y.y = pack16<BF16>(f.z * inv, f.w * inv);
+                *reinterpret_cast<uint2*>(a.o + row * D + d) = y;
+                if (d == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? -INFINITY : kLn2 * (mx + log2f(sum));
+            }
+        }
+        k = end;
+    }
+    if (tid == 0) a.meta[blockIdx.x] = make_int2(tail_of_cta, head_of_cta);
+}
+
+// Items that lie in several CTAs: block (c, row) merges, for the item that CTA c is the first of, its tail record and the
+// head records of the CTAs after it, up to the one where the item ends.
+template <int D, bool BF16, int NT>
+__global__ void __launch_bounds__(kWarps * 32) u4_merge_kernel(const __grid_constant__ U4Args a, int n_ctas) {
+    using S = Shape<D, NT>;
+    __shared__ float part[kWarps][D], part_l[kWarps];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int c = blockIdx.x / S::Rows, r = blockIdx.x - c * S::Rows;
+    const int item = a.meta[c].x;
+    if (item < 0) return;
+    const int rb = item % a.row_blocks, bh = item / a.row_blocks, b = bh / a.hkv, h = bh - b * a.hkv;
+    if (rb * S::Rows + r >= a.rows) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the CTAs of the item: those after c whose head record is part of it, up to the first that says it ends
+    int last = n_ctas;
+    for (int i0 = c + 1; i0 < n_ctas; i0 += 32) {
+        const int i = i0 + lane;
+        const bool ends = i < n_ctas && a.meta[i].y != 2;
+        const unsigned who = __ballot_sync(0xffffffffu, ends);
+        if (who) {
+            const int e = i0 + __ffs(who) - 1;
+            last = a.meta[e].y == 1 ? e + 1 : e;
+            break;
+        }
+    }
+    const float* base = a.scratch + (size_t)n_ctas * kWarps * S::Record;
+    auto record = [&](int i) { return base + (size_t)(2 * i + (i == c ? 1 : 0)) * S::Record; };
+    float mx = -INFINITY;
+    for (int i = c + lane; i < last; i += 32) mx = fmaxf(mx, record(i)[S::Rows * D + r]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    constexpr int E = D / 32;
+    float f[E], sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; e++) f[e] = 0.0f;
+#pragma unroll 4
+    for (int i = c + warp; i < last; i += kWarps) {
+        const float* rec = record(i);
+        const float ym = rec[S::Rows * D + r], yl = rec[S::Rows * (D + 1) + r];
+        const float w = ym == -INFINITY ? (yl == 0.0f ? 0.0f : 1.0f) : ex2(ym - mx);
+        sum = fmaf(w, yl, sum);
+#pragma unroll
+        for (int e = 0; e < E; e++) f[e] = fmaf(w, rec[r * D + e * 32 + lane], f[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) part[warp][e * 32 + lane] = f[e];
+    if (lane == 0) part_l[warp] = sum;
+    __syncthreads();
+    float total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) total += part_l[w];
+    const int tok = (rb * S::Rows + r) / a.group, hh = rb * S::Rows + r - tok * a.group;
+    const long long row = ((long long)b * a.n_tok + tok) * a.hq + (long long)h * a.group + hh;
+    for (int d = threadIdx.x; d < D; d += kWarps * 32) {
+        float y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) y += part[w][d];
+        y = total == 0.0f ? 0.0f : y / total;
+        if constexpr (BF16) a.o[row * D + d] = __bfloat16_as_ushort(__float2bfloat16_rn(y));
+        else a.o[row * D + d] = __half_as_ushort(__float2half_rn(y));
+        if (d == 0 && a.lse != nullptr) a.lse[row] = total == 0.0f ? -INFINITY : kLn2 * (mx + log2f(total));
+    }
+}
+
+// ------------------------------------------------------------------------------------------ host
+struct Plan {
+    int nt;                 // 8-row columns of a block
+    int row_blocks;
+    int ctas;
+    size_t record;          // bytes
+    size_t bytes;           // of the workspace
+};
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+Plan make_plan(int batch, int hq, int hkv, int n_tok, int kv_len, int d_head, int sm_count) {
+    Plan p;
+    const long long rows = (long long)n_tok * (hq / hkv);
+    p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    p.row_blocks = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
+    const long long tiles = (long long)batch * hkv * p.row_blocks * ((kv_len + kKeys - 1) / kKeys);
+    const long long most = (long long)sm_count * (p.nt == 1 ? 2 : 1);
+    const long long want = (tiles + kWarps - 1) / kWarps;
+    p.ctas = (int)(want < most ? want : most);
+    p.record = (size_t)8 * p.nt * (d_head + 2) * sizeof(float);
+    p.bytes = align256(p.record * p.ctas * (kWarps + 2)) + align256((size_t)p.ctas * sizeof(int2));
+    return p;
+}
+
+template <int D, bool BF16, int NT>
+int run_u4(const U4Args& a, int ctas, DeviceState* st, cudaStream_t stream) {
+    using S = Shape<D, NT>;
+    static bool configured[64] = {};
+    const int smem = kWarps * S::WarpBytes;
+    if (!configured[st->device]) {
+        FA_CUDA_TRY(cudaFuncSetAttribute(u4_kernel<D, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        configured[st->device] = true;
+    }
+    int rc = launch_dependent(u4_kernel<D, BF16, NT>, ctas, kWarps * 32, smem, stream, 1, a);
+    if (rc != FA_OK || ctas == 1) return rc;
+    return launch_dependent(u4_merge_kernel<D, BF16, NT>, ctas * S::Rows, kWarps * 32, 0, stream, 1, a, ctas);
+}
+template <int D, bool BF16>
+int run_u4_rows(const U4Args& a, const Plan& p, DeviceState* st, cudaStream_t stream) {
+    if (p.nt == 1) return run_u4<D, BF16, 1>(a, p.ctas, st, stream);
+    if (p.nt == 2) return run_u4<D, BF16, 2>(a, p.ctas, st, stream);
+    return run_u4<D, BF16, 4>(a, p.ctas, st, stream);
+}
+
+}  // namespace
+}  // namespace fa
+
+using namespace fa;
+
+FA_EXPORT size_t fa_decode_gqa_u4_workspace_bytes(int batch_size, int num_q_heads, int num_kv_heads, int num_q_tokens,
+                                                  int seq_len_kv, int d_head) {
+    if (batch_size <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || num_q_tokens < 0 || seq_len_kv <= 0)
+        return 0;
+    if (d_head != 64 && d_head != 128) return 0;
+    DeviceState* st = device_state();
+    return make_plan(batch_size, num_q_heads, num_kv_heads, num_q_tokens > 0 ? num_q_tokens : 1, seq_len_kv, d_head, st ? st->sm_count : 148).bytes;
+}
+
+FA_EXPORT int fa_decode_gqa_u4(const fa_decode_gqa_u4_args* p) {
+    if (!p || !p->q || !p->k_cache || !p->k_params || !p->v_cache || !p->v_params || !p->o) return FA_ERR_INVALID_ARGUMENT;
+    if (p->batch_size <= 0 || p->num_q_heads <= 0 || p->num_kv_heads <= 0 || p->seq_len_kv <= 0) return FA_ERR_INVALID_ARGUMENT;
+    if (p->num_q_heads % p->num_kv_heads != 0) return FA_ERR_INVALID_ARGUMENT;
+    if (!(p->scale > 0.0f) || !std::isfinite(p->scale)) return FA_ERR_INVALID_ARGUMENT;
+    const int n_tok = p->num_q_tokens > 0 ? p->num_q_tokens : 1;
+    if (p->num_q_tokens < 0 || n_tok > p->seq_len_kv) return FA_ERR_INVALID_ARGUMENT;
+    if (p->d_head != 64 && p->d_head != 128) return FA_ERR_UNSUPPORTED;
+    if (p->dtype != FA_DTYPE_F16 && p->dtype != FA_DTYPE_BF16) return FA_ERR_UNSUPPORTED;
+    if ((long long)p->batch_size * n_tok * p->num_q_heads > 0x7FFFFFFFll || p->seq_len_kv > 0x7FFFFFFF - 64) return FA_ERR_INVALID_ARGUMENT;
+    U4Args a;
+    int rc = check_layout(p->layout, FA_CACHE_U4, p->d_head, p->seq_len_kv, 0, &a.map);
+    if (rc != FA_OK) return rc;
+    if (!aligned16(p->q) || !aligned16(p->k_cache) || !aligned16(p->v_cache) || !aligned16(p->k_params) || !aligned16(p->v_params) || !aligned16(p->o))
+        return FA_ERR_MISALIGNED;
+    if (reinterpret_cast<uintptr_t>(p->lse) & 3u) return FA_ERR_MISALIGNED;
+    DeviceState* st = device_state();
+    if (!st) return FA_ERR_CUDA;
+    if (st->cc_major != 10) return FA_ERR_NOT_SM100;
+    const Plan plan = make_plan(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->d_head, st->sm_count);
+    if (!p->workspace || p->workspace_bytes < plan.bytes || !aligned16(p->workspace)) return FA_ERR_WORKSPACE;
+    a.q = static_cast<const uint16_t*>(p->q);
+    a.k = static_cast<const uint8_t*>(p->k_cache);
+    a.v = static_cast<const uint8_t*>(p->v_cache);
+    a.kp = static_cast<const __half2*>(p->k_params);
+    a.vp = static_cast<const __half2*>(p->v_params);
+    a.o = static_cast<uint16_t*>(p->o);
+    a.lse = p->lse;
+    a.scratch = static_cast<float*>(p->workspace);
+    a.meta = reinterpret_cast<int2*>(static_cast<uint8_t*>(p->workspace) + align256(plan.record * plan.ctas * (kWarps + 2)));
+    a.block_stride = p->layout.block_stride;
+    a.head_stride = p->layout.head_stride;
+    a.row_stride = p->layout.row_stride;
+    a.p_block_stride = p->layout.param_block_stride;
+    a.p_head_stride = p->layout.param_head_stride;
+    a.p_row_stride = p->layout.param_row_stride;
+    a.seq_lens = p->layout.seq_lens;
+    a.batch = p->batch_size;
+    a.hq = p->num_q_heads;
+    a.hkv = p->num_kv_heads;
+    a.group = p->num_q_heads / p->num_kv_heads;
+    a.n_tok = n_tok;
+    a.rows = n_tok * a.group;
+    a.row_blocks = plan.row_blocks;
+    a.kv_len = p->seq_len_kv;
+    a.scale_log2 = p->scale * 1.4426950408889634f;
+    cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
+    const bool bf = p->dtype == FA_DTYPE_BF16;
+    if (p->d_head == 64) return bf ? run_u4_rows<64, true>(a, plan, st, stream) : run_u4_rows<64, false>(a, plan, st, stream);
+    return bf ? run_u4_rows<128, true>(a, plan, st, stream) : run_u4_rows<128, false>(a, plan, st, stream);
+}

@@ -1,5 +1,6 @@
 """PyTorch custom operators over the C ABI: ``torch.ops.fa_b200.prefill`` / ``decode`` /
-``decode_gqa`` / ``prefill_backward`` / ``rope`` / ``cache_append`` / ``cache_read_u4``.
+``decode_gqa`` / ``prefill_backward`` / ``rope`` / ``cache_append`` / ``cache_read_u4`` /
+``decode_gqa_u4``.
 
 ``prefill`` is differentiable with respect to q, k and v (``fa_backward``); the gradient of its LSE
 output is not supported.  ``rope`` is differentiable with respect to q and k.  The others are forward
@@ -413,6 +414,41 @@ def _(k_cache, k_params, v_cache, v_params, batch, num_rows, dtype, first_rows=N
     return k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
 
 
+@torch.library.custom_op("fa_b200::decode_gqa_u4", mutates_args=())
+def decode_gqa_u4(q: torch.Tensor, k_cache: torch.Tensor, k_params: torch.Tensor, v_cache: torch.Tensor,
+                  v_params: torch.Tensor, scale: float, seq_lens: torch.Tensor | None = None,
+                  block_table: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``decode_gqa`` over a 4-bit cache (``fa_decode_gqa_u4``): codes uint8 ``[B, Skv, Hkv, D/2]`` or page pools
+    ``[P, page_size, Hkv, D/2]``, params fp16 ``[..., D/64, 2]``, of any strides (``u4_cache``).
+
+    q ``[B, T, Hq, D]``; returns (O ``[B, T, Hq, D]``, LSE ``[B, T, Hq]``)."""
+    if q.dtype not in _DTYPES:
+        raise TypeError("fa_b200::decode_gqa_u4: q is float16 or bfloat16")
+    if not all(t.is_cuda and t.device == q.device for t in (q, k_cache, k_params, v_cache, v_params)):
+        raise RuntimeError("fa_b200: tensors must be on one CUDA device (there is no CPU path)")
+    if q.dim() != 4:
+        raise ValueError("fa_b200::decode_gqa_u4: expected q [B,T,Hq,D]")
+    b, t, hq, d = q.shape
+    skv, kw = _cache_kw(k_cache, v_cache, d, b, seq_lens, block_table, k_params, v_params)
+    hkv = k_cache.shape[2]
+    q, _ = _rows(q.contiguous(), "q", copy=True)
+    o = torch.empty_like(q)
+    lse = torch.empty((b, t, hq), device=q.device, dtype=torch.float32)
+    with torch.cuda.device(q.device):
+        ws_bytes = _fa.decode_gqa_u4_workspace_bytes(b, hq, hkv, t, skv, d)
+        ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8)
+        _fa.decode_gqa_u4(q, k_cache, k_params, v_cache, v_params, o, lse, b, hq, hkv, skv, d, float(scale),
+                          dtype=_DTYPES[q.dtype], num_q_tokens=t, workspace=ws, workspace_bytes=ws_bytes,
+                          stream=torch.cuda.current_stream(q.device), **kw)
+    return o, lse
+
+
+@decode_gqa_u4.register_fake
+def _(q, k_cache, k_params, v_cache, v_params, scale, seq_lens=None, block_table=None):
+    b, t, hq, _ = q.shape
+    return q.new_empty(q.shape), q.new_empty((b, t, hq), dtype=torch.float32)
+
+
 def sdpa(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, attn_mask=None,
          dropout_p: float = 0.0, is_causal: bool = False, scale: float | None = None) -> torch.Tensor:
     """``scaled_dot_product_attention`` for the cases the library covers (no mask, no dropout).
@@ -431,4 +467,4 @@ def sdpa(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, attn_mask=
 
 
 __all__ = ["prefill", "prefill_backward", "decode", "decode_gqa", "rope", "rope_frequencies", "cache_append",
-           "cache_read_u4", "u4_cache", "sdpa", "FaError"]
+           "cache_read_u4", "decode_gqa_u4", "u4_cache", "sdpa", "FaError"]

@@ -487,6 +487,39 @@ typedef struct fa_cache_read_args {
 int fa_cache_read_u4(const fa_cache_read_args* args);
 
 /*
+ * fa_decode_gqa_u4: fa_decode_gqa over a 4-bit cache.  q, o [B, T, Hq, D] in `dtype`, lse [B, T, Hq]
+ * (optional); T = num_q_tokens newest tokens per sequence (0 = 1), token t sees keys
+ * [0, len - T + t]; a token that sees no key yields O = 0, LSE = -inf.  workspace: at least
+ * fa_decode_gqa_u4_workspace_bytes(...) of the same sizes; two calls that may run at the same
+ * time need one each.
+ */
+typedef struct fa_decode_gqa_u4_args {
+    const void*     q;
+    const void*     k_cache;
+    const void*     k_params;
+    const void*     v_cache;
+    const void*     v_params;
+    void*           o;
+    float*          lse;           /* optional */
+    int             batch_size;
+    int             num_q_heads;
+    int             num_kv_heads;  /* divides num_q_heads */
+    int             num_q_tokens;
+    int             seq_len_kv;
+    int             d_head;        /* 64 or 128 */
+    float           scale;
+    int             dtype;         /* FA_DTYPE_F16 or FA_DTYPE_BF16 */
+    fa_cache_layout layout;
+    void*           workspace;
+    size_t          workspace_bytes;
+    void*           stream;
+} fa_decode_gqa_u4_args;
+
+size_t fa_decode_gqa_u4_workspace_bytes(int batch_size, int num_q_heads, int num_kv_heads, int num_q_tokens,
+                                        int seq_len_kv, int d_head);
+int fa_decode_gqa_u4(const fa_decode_gqa_u4_args* args);
+
+/*
  * LSE merge of n_parts partial results (the exchange step of KV-sequence
  * sharded decode: each rank's (o_f32, lse) gathered into one local buffer).
  *   o_parts  : fp32 [n_parts, rows, d_head]   lse_parts: fp32 [n_parts, rows]

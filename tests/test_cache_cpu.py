@@ -95,9 +95,35 @@ def test_read_refusals(fa, change, code):
     assert fa.cache_read_u4_raw(*[base.pop(n) for n in names], **base) == getattr(fa, "FA_ERR_" + code)
 
 
+@pytest.mark.parametrize("change,code", [
+    (dict(q=None), "INVALID_ARGUMENT"), (dict(v_params=None), "INVALID_ARGUMENT"), (dict(o=None), "INVALID_ARGUMENT"),
+    (dict(num_q_heads=3), "INVALID_ARGUMENT"), (dict(batch_size=0), "INVALID_ARGUMENT"), (dict(seq_len_kv=0), "INVALID_ARGUMENT"),
+    (dict(seq_len_kv=2 ** 31 - 1), "INVALID_ARGUMENT"), (dict(scale=0.0), "INVALID_ARGUMENT"),
+    (dict(scale=float("inf")), "INVALID_ARGUMENT"), (dict(num_q_tokens=-1), "INVALID_ARGUMENT"),
+    (dict(num_q_tokens=65), "INVALID_ARGUMENT"), (dict(d_head=96), "UNSUPPORTED"), (dict(dtype="e4m3"), "UNSUPPORTED"),
+    (dict(kv_strides=(64 * 128, 64 * 64 + 8, 64)), "MISALIGNED"), (dict(param_strides=(257, 128, 2)), "MISALIGNED"),
+    (dict(param_strides=(256, 0, 2)), "INVALID_ARGUMENT"), (dict(PAGED, page_size=100), "INVALID_ARGUMENT"),
+    (dict(q=24), "MISALIGNED"), (dict(lse=18), "MISALIGNED"),
+])
+def test_attention_refusals(fa, change, code):
+    base = dict(q=16, k_cache=16, k_params=16, v_cache=16, v_params=16, o=16, lse=16, batch_size=2, num_q_heads=4,
+                num_kv_heads=2, seq_len_kv=64, d_head=128, scale=0.1, kv_strides=U4["kv_strides"],
+                param_strides=U4["param_strides"])
+    base.update(change)
+    names = ("q", "k_cache", "k_params", "v_cache", "v_params", "o", "lse", "batch_size", "num_q_heads", "num_kv_heads",
+             "seq_len_kv", "d_head", "scale")
+    assert fa.decode_gqa_u4_raw(*[base.pop(n) for n in names], **base) == getattr(fa, "FA_ERR_" + code)
+
+
+def test_attention_workspace(fa):
+    size = fa.decode_gqa_u4_workspace_bytes
+    assert size(0, 4, 2, 1, 64, 128) == size(1, 3, 2, 1, 64, 128) == size(1, 4, 2, 1, 64, 96) == 0
+    assert 0 < size(1, 4, 2, 1, 64, 128) <= size(8, 4, 2, 1, 4096, 128) == size(8, 4, 2, 0, 4096, 128)
+
+
 def test_null_arguments(fa):
     lib = fa.lib()
-    for name in ("fa_rope", "fa_cache_append", "fa_cache_read_u4"):
+    for name in ("fa_rope", "fa_cache_append", "fa_cache_read_u4", "fa_decode_gqa_u4"):
         assert getattr(lib, name)(None) == fa.FA_ERR_INVALID_ARGUMENT
     assert lib.fa_rope_inv_freq(None, 64, None, None) == fa.FA_ERR_INVALID_ARGUMENT
 
@@ -155,6 +181,8 @@ def test_operators_registered_and_fake_shapes(fa):
         assert torch.ops.fa_b200.cache_append(q, k, k, codes, codes, params, params, f).shape == q.shape
         e = torch.empty((2, 64, 3, 128), dtype=torch.float8_e4m3fn)
         assert torch.ops.fa_b200.cache_append(q, k, k, e, e, None, None, f).dtype == torch.float8_e4m3fn
+        o, lse = torch.ops.fa_b200.decode_gqa_u4(q, codes, params, codes, params, 0.1)
+        assert o.shape == q.shape and o.dtype == q.dtype and lse.shape == (2, 5, 6) and lse.dtype == torch.float32
         kk, vv = torch.ops.fa_b200.cache_read_u4(codes, params, codes, params, 2, 7, torch.float16)
         assert kk.shape == vv.shape == (2, 7, 3, 128) and kk.dtype == torch.float16
 
