@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # FA_B200_LIB points the binding at another build of the same library (development only).
@@ -187,6 +188,32 @@ class DecodeGqaU4Args(ctypes.Structure):
     ]
 
 
+def _packer(cls):
+    """``struct.Struct(...).pack`` with the memory layout of a ctypes structure, nested ones flattened.  An argument block
+    packed this way takes a serving step's call a third of the time that building the ctypes object takes (40 fields:
+    1.5 us against 5)."""
+    codes = {ctypes.c_void_p: "Q", ctypes.c_int: "i", ctypes.c_longlong: "q", ctypes.c_size_t: "Q", ctypes.c_float: "f",
+             ctypes.c_double: "d"}
+    fmt, at = ["="], 0
+
+    def walk(c, base):
+        nonlocal at
+        for name, t in c._fields_:
+            off = base + getattr(c, name).offset
+            if issubclass(t, ctypes.Structure):
+                walk(t, off)
+            else:
+                fmt.append(f"{off - at}x{codes[t]}" if off > at else codes[t])
+                at = off + ctypes.sizeof(t)
+
+    walk(cls, 0)
+    fmt.append(f"{ctypes.sizeof(cls) - at}x")
+    return struct.Struct("".join(fmt)).pack
+
+
+_pack_rope, _pack_append, _pack_read, _pack_decode_u4 = map(_packer, (RopeArgs, CacheAppendArgs, CacheReadArgs, DecodeGqaU4Args))
+
+
 class FaError(RuntimeError):
     def __init__(self, code: int, what: str):
         super().__init__(f"{what}: {error_string(code)} ({code})"
@@ -257,17 +284,12 @@ def lib() -> ctypes.CDLL:
         l.fa_status_word_to_error.argtypes = [ctypes.c_int]
         l.fa_set_prefill_variant.restype = ctypes.c_int
         l.fa_set_prefill_variant.argtypes = [ctypes.c_int]
-        l.fa_rope.restype = ctypes.c_int
-        l.fa_rope.argtypes = [ctypes.POINTER(RopeArgs)]
+        for name in ("fa_rope", "fa_cache_append", "fa_cache_read_u4", "fa_decode_gqa_u4"):
+            getattr(l, name).restype = ctypes.c_int
+            getattr(l, name).argtypes = [ctypes.c_void_p]              # a packed block, or byref() of the mirror
         l.fa_rope_inv_freq.restype = ctypes.c_int
         l.fa_rope_inv_freq.argtypes = [ctypes.POINTER(RopeScaling), ctypes.c_int, ctypes.POINTER(ctypes.c_double),
                                        ctypes.POINTER(ctypes.c_float)]
-        l.fa_cache_append.restype = ctypes.c_int
-        l.fa_cache_append.argtypes = [ctypes.POINTER(CacheAppendArgs)]
-        l.fa_cache_read_u4.restype = ctypes.c_int
-        l.fa_cache_read_u4.argtypes = [ctypes.POINTER(CacheReadArgs)]
-        l.fa_decode_gqa_u4.restype = ctypes.c_int
-        l.fa_decode_gqa_u4.argtypes = [ctypes.POINTER(DecodeGqaU4Args)]
         l.fa_decode_gqa_u4_workspace_bytes.restype = ctypes.c_size_t
         l.fa_decode_gqa_u4_workspace_bytes.argtypes = [ctypes.c_int] * 6
         _lib = l
@@ -408,11 +430,13 @@ def backward(*args, **kw) -> None:
         raise FaError(rc, "fa_backward")
 
 
-def _rotary(inv_freq, rotary_dim, interleaved, amplitude) -> Rotary:
-    """``inv_freq``: doubles in host memory - a CPU tensor, a ctypes array or an address."""
-    if isinstance(inv_freq, ctypes.Array):
-        inv_freq = ctypes.addressof(inv_freq)
-    return Rotary(_ptr(inv_freq), rotary_dim, int(interleaved), amplitude)
+def _adr(x) -> int:
+    """Address of a tensor or a ctypes array, or the address given; 0 for None."""
+    if x is None:
+        return 0
+    if x.__class__ is int:
+        return x
+    return ctypes.addressof(x) if isinstance(x, ctypes.Array) else x.data_ptr()
 
 
 def rope_inv_freq(rotary_dim, base=10000.0, scaling="plain", factor=1.0, original_length=0.0, slow=0.0, fast=0.0):
@@ -431,23 +455,18 @@ def rope_raw(q, k, q_out, k_out, batch_size, num_q_heads, num_kv_heads, seq_len,
              interleaved=False, amplitude=1.0, dtype="f16", positions=None, positions_stride=0, position_offset=0,
              inverse=False, q_strides=(0, 0, 0), k_strides=(0, 0, 0), q_out_strides=(0, 0, 0), k_out_strides=(0, 0, 0),
              stream=None) -> int:
-    """fa_rope; strides are (batch, head, row) in elements ((0, 0, 0) = dense [B, H, S, D]).  Returns the status code."""
-    a = RopeArgs(_ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), Strides(*q_strides), Strides(*k_strides),
-                 Strides(*q_out_strides), Strides(*k_out_strides), batch_size, num_q_heads, num_kv_heads, seq_len, d_head,
-                 DTYPES[dtype] if isinstance(dtype, str) else dtype, _ptr(positions), positions_stride, position_offset,
-                 int(inverse), _rotary(inv_freq, rotary_dim, interleaved, amplitude), _stream_handle(stream))
-    return lib().fa_rope(ctypes.byref(a))
+    """fa_rope; ``inv_freq``: doubles in host memory (a CPU tensor, a ctypes array or an address); strides are (batch, head,
+    row) in elements ((0, 0, 0) = dense [B, H, S, D]).  Returns the status code."""
+    return (_lib or lib()).fa_rope(_pack_rope(
+        _adr(q), _adr(k), _adr(q_out), _adr(k_out), *q_strides, *k_strides, *q_out_strides, *k_out_strides, batch_size,
+        num_q_heads, num_kv_heads, seq_len, d_head, DTYPES.get(dtype, dtype), _adr(positions), positions_stride,
+        position_offset, inverse, _adr(inv_freq), rotary_dim, interleaved, amplitude, _stream_handle(stream) or 0))
 
 
 def rope(*args, **kw) -> None:
     rc = rope_raw(*args, **kw)
     if rc != FA_OK:
         raise FaError(rc, "fa_rope")
-
-
-def _layout(kv_strides, param_strides, block_table, block_table_stride, page_size, num_pages, seq_lens) -> CacheLayout:
-    return CacheLayout(*kv_strides, *param_strides, _ptr(block_table), block_table_stride, page_size, num_pages,
-                       _ptr(seq_lens))
 
 
 def cache_append_raw(k, v, k_cache, v_cache, batch_size, num_tokens, num_kv_heads, seq_len_kv, d_head, dtype="f16",
@@ -461,14 +480,12 @@ def cache_append_raw(k, v, k_cache, v_cache, batch_size, num_tokens, num_kv_head
     the tokens of q, k, v.  Returns the status code."""
     if cache_dtype in ("f16", "bf16") and cache_dtype != dtype:
         return FA_ERR_UNSUPPORTED
-    a = CacheAppendArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), _ptr(k_params),
-                        _ptr(v_params), *token_strides, batch_size, num_tokens, num_q_heads, num_kv_heads, seq_len_kv,
-                        d_head, DTYPES[dtype] if isinstance(dtype, str) else dtype,
-                        CACHES[cache_dtype] if isinstance(cache_dtype, str) else cache_dtype,
-                        _layout(kv_strides, param_strides, block_table, block_table_stride, page_size, num_pages, seq_lens),
-                        _ptr(num_new), _ptr(positions), _rotary(inv_freq, rotary_dim, interleaved, amplitude),
-                        _ptr(q_scale), _ptr(k_scale), _ptr(v_scale), _stream_handle(stream))
-    return lib().fa_cache_append(ctypes.byref(a))
+    return (_lib or lib()).fa_cache_append(_pack_append(
+        _adr(q), _adr(k), _adr(v), _adr(q_out), _adr(k_cache), _adr(v_cache), _adr(k_params), _adr(v_params),
+        *token_strides, batch_size, num_tokens, num_q_heads, num_kv_heads, seq_len_kv, d_head, DTYPES.get(dtype, dtype),
+        CACHES.get(cache_dtype, cache_dtype), *kv_strides, *param_strides, _adr(block_table), block_table_stride, page_size,
+        num_pages, _adr(seq_lens), _adr(num_new), _adr(positions), _adr(inv_freq), rotary_dim, interleaved, amplitude,
+        _adr(q_scale), _adr(k_scale), _adr(v_scale), _stream_handle(stream) or 0))
 
 
 def cache_append(*args, **kw) -> None:
@@ -481,11 +498,10 @@ def cache_read_u4_raw(k_cache, k_params, v_cache, v_params, k_out, v_out, batch_
                       num_rows, dtype="f16", first_rows=None, kv_strides=(0, 0, 0), param_strides=(0, 0, 0),
                       block_table=None, block_table_stride=0, page_size=0, num_pages=0, seq_lens=None, stream=None) -> int:
     """fa_cache_read_u4; the cache is described as for cache_append.  Returns the status code."""
-    a = CacheReadArgs(_ptr(k_cache), _ptr(k_params), _ptr(v_cache), _ptr(v_params), _ptr(k_out), _ptr(v_out), batch_size,
-                      num_kv_heads, seq_len_kv, d_head, num_rows, DTYPES[dtype] if isinstance(dtype, str) else dtype,
-                      _layout(kv_strides, param_strides, block_table, block_table_stride, page_size, num_pages, seq_lens),
-                      _ptr(first_rows), _stream_handle(stream))
-    return lib().fa_cache_read_u4(ctypes.byref(a))
+    return (_lib or lib()).fa_cache_read_u4(_pack_read(
+        _adr(k_cache), _adr(k_params), _adr(v_cache), _adr(v_params), _adr(k_out), _adr(v_out), batch_size, num_kv_heads,
+        seq_len_kv, d_head, num_rows, DTYPES.get(dtype, dtype), *kv_strides, *param_strides, _adr(block_table),
+        block_table_stride, page_size, num_pages, _adr(seq_lens), _adr(first_rows), _stream_handle(stream) or 0))
 
 
 def cache_read_u4(*args, **kw) -> None:
@@ -503,12 +519,11 @@ def decode_gqa_u4_raw(q, k_cache, k_params, v_cache, v_params, o, lse, batch_siz
                       block_table=None, block_table_stride=0, page_size=0, num_pages=0, seq_lens=None, workspace=None,
                       workspace_bytes=0, stream=None) -> int:
     """fa_decode_gqa_u4; the cache is described as for cache_append.  Returns the status code."""
-    a = DecodeGqaU4Args(_ptr(q), _ptr(k_cache), _ptr(k_params), _ptr(v_cache), _ptr(v_params), _ptr(o), _ptr(lse), batch_size,
-                        num_q_heads, num_kv_heads, num_q_tokens, seq_len_kv, d_head, scale,
-                        DTYPES[dtype] if isinstance(dtype, str) else dtype,
-                        _layout(kv_strides, param_strides, block_table, block_table_stride, page_size, num_pages, seq_lens),
-                        _ptr(workspace), workspace_bytes, _stream_handle(stream))
-    return lib().fa_decode_gqa_u4(ctypes.byref(a))
+    return (_lib or lib()).fa_decode_gqa_u4(_pack_decode_u4(
+        _adr(q), _adr(k_cache), _adr(k_params), _adr(v_cache), _adr(v_params), _adr(o), _adr(lse), batch_size, num_q_heads,
+        num_kv_heads, num_q_tokens, seq_len_kv, d_head, scale, DTYPES.get(dtype, dtype), *kv_strides, *param_strides,
+        _adr(block_table), block_table_stride, page_size, num_pages, _adr(seq_lens), _adr(workspace), workspace_bytes,
+        _stream_handle(stream) or 0))
 
 
 def decode_gqa_u4(*args, **kw) -> None:

@@ -106,6 +106,19 @@ int make_tensor_map_4d(CUtensorMap* out, const void* base, int dtype, uint64_t r
     return FA_OK;
 }
 
+int make_tensor_map_u4(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t n_rows, uint64_t n_heads, uint64_t n_blocks,
+                       uint64_t row_stride, uint64_t head_stride, uint64_t block_stride, uint32_t box_rows) {
+    cuuint64_t dims[4]    = {row_bytes, n_rows, n_heads, n_blocks};
+    cuuint64_t strides[3] = {row_stride, head_stride, block_stride};
+    cuuint32_t box[4]     = {(cuuint32_t)row_bytes, box_rows, 1, 1};
+    cuuint32_t estr[4]    = {1, 1, 1, 1};
+    CUresult r = g_encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return note_driver_error(r, "cuTensorMapEncodeTiled");
+    return FA_OK;
+}
+
 int make_tensor_map_q5(CUtensorMap* out, const void* base, int dtype, uint64_t d_head, uint64_t group,
                        uint64_t n_tok, uint64_t n_kv_heads, uint64_t batch, uint32_t box_cols) {
     const uint64_t es = (dtype == FA_DTYPE_E4M3) ? 1 : 2;

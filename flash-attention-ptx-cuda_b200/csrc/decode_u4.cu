@@ -39,14 +39,14 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kGrow = 8.0f;                  // a running max may be exceeded by this much (in powers of two) before it is raised
 
 struct U4Args {
+    CUtensorMap tk, tv;                        // codes: (bytes of a row, rows of a block, KV heads, blocks), boxes of up to 32 rows
     const uint16_t* q;
-    const uint8_t *k, *v;
     const __half2 *kp, *vp;
     uint16_t* o;
     float* lse;
     float* scratch;                            // head records of the warps, then two records a CTA
+    int* status;
     int2* meta;                                // per CTA: item of the tail record or -1; head record: 0 none, 1 ends here, 2 goes on
-    long long block_stride, head_stride, row_stride;          // bytes
     long long p_block_stride, p_head_stride, p_row_stride;    // pairs
     CacheMap map;
     const int* seq_lens;
@@ -75,11 +75,9 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
+// BYTES of `src`, or zeros.
 template <int BYTES>
-__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bool valid) {
+__device__ __forceinline__ void cp_async_or_zero(uint32_t dst, const void* src, bool valid) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(valid ? BYTES : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -87,26 +85,30 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-    uint32_t r;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(a));
-    return r;
+// The pairs of a key.
+template <int G>
+__device__ __forceinline__ void lds_pairs(uint32_t a, uint32_t (&p)[G]) {
+    if constexpr (G == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(p[0]), "=r"(p[G - 1]) : "r"(a));
+    else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(p[0]) : "r"(a));
 }
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-    uint2 r;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
-    return r;
+// Four 8 x 8 tiles of 16-bit values, whose rows the lanes' addresses name (8 lanes a tile); TRANS: by columns.
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t a, uint32_t (&r)[4]) {
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
 }
 
-// D = A B + C, m16n8k16, fp32 accumulation.
-template <bool BF16>
+// D = A B + C, m16n8k16, fp16 operands, fp32 accumulation.
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (BF16)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same with C the same in both halves of the rows: c0 in the first column of a thread, c1 in the second.
+__device__ __forceinline__ void mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 // An 8 x 8 tile of 16-bit values, rows to columns, across the warp.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -114,25 +116,30 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
+__device__ __forceinline__ uint32_t hadd2(uint32_t x, float y) {
+    const __half2 z = __hadd2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(y));
+    return *reinterpret_cast<const uint32_t*>(&z);
+}
 
-// Nibble N (0..3) of both halves of `x` as the 16-bit value 16 + code: the code lies in the top four bits of the
-// mantissa of 16.0.
-template <bool BF16, int N>
+// Nibble N (0..3) of both halves of a word as code + BIAS in fp16.  A nibble in bits 0-3 of the mantissa of 1024.0 is
+// 1024 + code, one in bits 4-7 of that of 64.0 is 64 + code: a logic instruction each, the word shifted once for
+// nibbles 2 and 3, and an exact addition where the bias wanted is another.  (Shifting every nibble to the same place costs
+// three shifts a word on the integer pipe, which runs at half the rate and was the kernel's limit.)
+template <int N, int BIAS>
 __device__ __forceinline__ uint32_t code16(uint32_t x) {
-    constexpr int at = BF16 ? 3 : 6, shift = at - 4 * N;
-    constexpr uint32_t mask = 0x000F000Fu << at, one = BF16 ? 0x41804180u : 0x4C004C00u;
-    const uint32_t y = shift >= 0 ? x << (shift >= 0 ? shift : 0) : x >> (shift >= 0 ? 0 : -shift);
-    return (y & mask) | one;
-}
-// The same minus 24: code - 8, exact.
-__device__ __forceinline__ uint32_t centred(uint32_t x) {
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(24.0f, 24.0f));
-    return *reinterpret_cast<const uint32_t*>(&y);
+    constexpr bool odd = N & 1;
+    const uint32_t y = N < 2 ? x : x >> 8;
+    // (y & mask) | one as one instruction, which takes one of the two constants from a register
+    uint32_t c;
+    if constexpr (odd) asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(c) : "r"(y), "n"(0x00F000F0), "r"(0x54005400));
+    else asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(c) : "r"(y), "n"(0x000F000F), "r"(0x64006400));
+    return (odd ? 64 : 1024) == BIAS ? c : hadd2(c, (float)(BIAS - (odd ? 64 : 1024)));
 }
 
-// Place of key r's row in a tile of V codes: a permutation of rows (and of 32-byte halves, d_head 128) under which the
-// reads below touch every bank once.  Within 8 keys the rows 0, 2, 4, 6 | 1, 3, 5, 7 follow one another.
-__device__ __forceinline__ int v_row(int r) { return (r & ~7) | ((r & 1) << 2) | ((r >> 1) & 3); }
+// The 16-byte piece of row r in which piece c of the row lies: the exchange of TMA's 64-byte (d_head 128) and 32-byte swizzle,
+// under which the eight rows of a tile of ldmatrix touch every bank once.
+template <int D>
+__device__ __forceinline__ int piece(int r, int c) { return D == 128 ? c ^ ((r >> 1) & 3) : c ^ ((r >> 2) & 1); }
 
 struct Item {
     int b, h, rb, len, tiles;      // sequence, KV head, row block, its keys, tiles of 32 of them (at least one)
@@ -143,11 +150,20 @@ template <int D, bool BF16, int NT>
 __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kernel(const __grid_constant__ U4Args a) {
     using S = Shape<D, NT>;
     constexpr int G = S::G;
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);      // the swizzle goes by the address
+    __shared__ __align__(8) uint64_t s_full[kWarps][S::Stages];
+    __shared__ int s_abort, s_never;
     __shared__ long long s_prefix[kWarps * 32];                // tiles (of one head and row block) before a thread's sequences
     __shared__ long long s_total;
     __shared__ int s_head_item[kWarps], s_tail_item[kWarps], s_before[kWarps], s_after[kWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    if (tid == 0) {
+        s_abort = s_never = 0;
+        for (int i = 0; i < kWarps * S::Stages; i++) mbar_init(smem_u32(&s_full[0][0] + i), 1);
+        fence_mbar_init();
+    }
+    const WaitCtl ctl{&s_abort, a.status};
     grid_dependency_wait();
     grid_launch_dependents();
 
@@ -225,84 +241,134 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
         item_start = b_start + (long long)i * it.tiles;
     }
 
+    // ---- the warp's ring: a barrier a stage, which TMA's copies of the codes complete; scale and offset pairs, 4 or 8 bytes
+    // of any row stride, come by cp.async
+    constexpr int P = D / 32;                                  // pieces of a row as the products see them: 32 elements, 16 bytes
+    const uint32_t full0 = smem_u32(&s_full[warp][0]);
+    const bool two_boxes = a.map.page_shift == 4;              // pages of 16 rows: half a tile each
+    const int in_page = a.map.page_shift < 0 ? 0x7FFFFFFF : (1 << a.map.page_shift) - 1;
+    int stage = 0, load_stage = 0, in_flight = 0;
+    uint32_t phase = 0;
+    bool alive = true;
+    // row and first piece of the lane's address for ldmatrix: keys 0-7, 8-15 of piece c, then of piece c + 1
+    const int m_row = lane & 15;
+    uint32_t m_at[P / 2];
+#pragma unroll
+    for (int c = 0; c < P / 2; c++) m_at[c] = ring + m_row * S::RowBytes + piece<D>(m_row, 2 * c + (lane >> 4)) * 16;
+
     // ---- item by item
-    for (long long x = w_begin; x < w_end;) {
+    for (long long x = w_begin; x < w_end && alive;) {
         const int tile0 = (int)(x - item_start);
         const int tile1 = (int)min((long long)it.tiles, tile0 + (w_end - x));
         const int row0 = it.rb * S::Rows;
 
-        // q as operand B: column g of the n-th 8 rows; a word of 8 codes is two steps of k, its pairs (i, i + 4)
-        uint32_t qf[NT][G][2][4];
-        float q_sum[NT][G][2];
+        // q as operand B: column g of the n-th 8 rows; 8 elements of a 16-byte piece of codes are two steps of k, in pairs
+        // (i, i + 4) as the codes lie in a word.  bf16 rows are brought to fp16 by a power of two that puts their
+        // largest element at 2^14: exact for elements down to 2^-28 of that one, and the rest is below its 32-bit rounding.
+        uint32_t qf[NT][P][4];
+        float q_init[NT][G][2];                                // -72 sum of q over the group
+        float sc[NT][2];                                       // softmax scale (log2) of the columns that this thread has in S^T
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const int r = row0 + n * 8 + g;
             const int tok = r / a.group, hh = r - tok * a.group;
             const uint16_t* qp = a.q + (((long long)it.b * a.n_tok + tok) * a.hq + (long long)it.h * a.group + hh) * D;
+            uint4 u[P];
+#pragma unroll
+            for (int c = 0; c < P; c++) u[c] = r < a.rows ? *reinterpret_cast<const uint4*>(qp + c * 32 + t * 8) : make_uint4(0, 0, 0, 0);
+            if constexpr (BF16) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int c = 0; c < P; c++) {
+                    const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+                }
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const uint32_t e = max(top >> 7, 15u);         // exponent field of the largest element
+                const float up = __uint_as_float((268u - e) << 23), down = __uint_as_float((e - 14u) << 23);
+#pragma unroll
+                for (int c = 0; c < P; c++) {
+                    uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float2 f = unpack16<true>(w[i]);
+                        w[i] = pack16<false>(f.x * up, f.y * up);
+                    }
+                    u[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                sc[n][0] = a.scale_log2 * __shfl_sync(0xffffffffu, down, 8 * t);
+                sc[n][1] = a.scale_log2 * __shfl_sync(0xffffffffu, down, 8 * t + 4);
+            } else {
+                sc[n][0] = sc[n][1] = a.scale_log2;
+            }
 #pragma unroll
             for (int gi = 0; gi < G; gi++) {
                 float sum = 0.0f;
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    uint4 u = make_uint4(0, 0, 0, 0);
-                    if (r < a.rows) u = *reinterpret_cast<const uint4*>(qp + gi * kU4Group + t * 16 + w * 8);
-                    const float2 f0 = unpack16<BF16>(u.x), f1 = unpack16<BF16>(u.y), f2 = unpack16<BF16>(u.z), f3 = unpack16<BF16>(u.w);
+                for (int c = 2 * gi; c < 2 * gi + 2; c++) {
+                    const float2 f0 = unpack16<false>(u[c].x), f1 = unpack16<false>(u[c].y), f2 = unpack16<false>(u[c].z), f3 = unpack16<false>(u[c].w);
                     sum += ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
-                    qf[n][gi][w][0] = __byte_perm(u.x, u.z, 0x5410);
-                    qf[n][gi][w][1] = __byte_perm(u.x, u.z, 0x7632);
-                    qf[n][gi][w][2] = __byte_perm(u.y, u.w, 0x5410);
-                    qf[n][gi][w][3] = __byte_perm(u.y, u.w, 0x7632);
+                    qf[n][c][0] = __byte_perm(u[c].x, u[c].z, 0x5410);
+                    qf[n][c][1] = __byte_perm(u[c].x, u[c].z, 0x7632);
+                    qf[n][c][2] = __byte_perm(u[c].y, u[c].w, 0x5410);
+                    qf[n][c][3] = __byte_perm(u[c].y, u[c].w, 0x7632);
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                q_sum[n][gi][0] = __shfl_sync(0xffffffffu, sum, 8 * t);          // of the columns that this thread has in S^T
-                q_sum[n][gi][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+                q_init[n][gi][0] = -72.0f * __shfl_sync(0xffffffffu, sum, 8 * t);
+                q_init[n][gi][1] = -72.0f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
             }
         }
 
         // ---- loads of a tile
-        const long long h_off = (long long)it.h * a.head_stride, hp_off = (long long)it.h * a.p_head_stride;
+        const long long hp_off = (long long)it.h * a.p_head_stride;
         auto page_of = [&](int key) -> int {                   // -1: names none, or past the end
             if (key >= it.len) return -1;
             if (a.map.page_shift < 0) return it.b;
             const int p = a.map.block_table[(long long)it.b * a.map.table_stride + (key >> a.map.page_shift)];
             return (unsigned)p < (unsigned)a.map.n_pages ? p : -1;
         };
-        const int in_page = a.map.page_shift < 0 ? 0x7FFFFFFF : (1 << a.map.page_shift) - 1;
-        auto load_tile = [&](int tile, int stage, int p0, int p1) {
+        auto load_tile = [&](int tile, int p0, int p1) {
             const int k0 = tile * kKeys;
-            const uint32_t dst = ring + stage * S::StageBytes;
-            constexpr int CPR = S::RowBytes / 16, RPI = 32 / CPR;              // 16-byte pieces of a row, rows an instruction
-#pragma unroll
-            for (int i = 0; i < kKeys / RPI; i++) {
-                const int r = i * RPI + lane / CPR, c = lane % CPR, key = k0 + r;
-                const int p = r < 16 ? p0 : p1;
-                const bool ok = key < it.len && p >= 0;
-                const long long off = ok ? p * a.block_stride + h_off + (long long)(key & in_page) * a.row_stride + c * 16 : 0;
-                const int ck = D == 128 ? c ^ (((r >> 1) & 1) << 1) : c, cv = D == 128 ? c ^ (((r >> 2) & 1) << 1) : c;
-                cp_async_16(dst + r * S::RowBytes + ck * 16, a.k + off, ok);
-                cp_async_16(dst + S::CodeBytes + v_row(r) * S::RowBytes + cv * 16, a.v + off, ok);
+            const uint32_t dst = ring + load_stage * S::StageBytes, bar = full0 + load_stage * 8;
+            load_stage = load_stage + 1 == S::Stages ? 0 : load_stage + 1;
+            in_flight++;
+            if (elect_one()) {
+                // rows past the block and pages that name none read as zero; rows past the sequence's end hold any codes, and are masked
+                mbar_arrive_expect_tx(bar, 2 * S::CodeBytes);
+                tma_load_4d(dst, &a.tk, bar, 0, k0 & in_page, it.h, p0);
+                tma_load_4d(dst + S::CodeBytes, &a.tv, bar, 0, k0 & in_page, it.h, p0);
+                if (two_boxes) {
+                    tma_load_4d(dst + S::CodeBytes / 2, &a.tk, bar, 0, 0, it.h, p1);
+                    tma_load_4d(dst + S::CodeBytes + S::CodeBytes / 2, &a.tv, bar, 0, 0, it.h, p1);
+                }
             }
+            const uint32_t pdst = dst + 2 * S::CodeBytes + lane * 4 * G;
             const int key = k0 + lane, p = lane < 16 ? p0 : p1;
             const bool ok = key < it.len && p >= 0;
             const long long off = ok ? p * a.p_block_stride + hp_off + (long long)(key & in_page) * a.p_row_stride : 0;
-            cp_async_small<4 * G>(dst + 2 * S::CodeBytes + lane * 4 * G, a.kp + off, ok);
-            cp_async_small<4 * G>(dst + 2 * S::CodeBytes + S::ParamBytes + lane * 4 * G, a.vp + off, ok);
+            cp_async_or_zero<4 * G>(pdst, a.kp + off, ok);
+            cp_async_or_zero<4 * G>(pdst + S::ParamBytes, a.vp + off, ok);
         };
 
-        float o[NT][G][4][4], l[NT][2], m[NT][2], zs[NT][G][2];
+        float o[NT][P][2][4], l[NT][2], m[NT][2], mc[NT][2], zs[NT][G][2];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
-            for (int gi = 0; gi < G; gi++) {
-                zs[n][gi][0] = zs[n][gi][1] = 0.0f;
+            for (int c = 0; c < P; c++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int i = 0; i < 2; i++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[n][gi][i][e] = 0.0f;
+                    for (int e = 0; e < 4; e++) o[n][c][i][e] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                l[n][c] = mc[n][c] = 0.0f;                     // mc: the max as it is taken off, scaled; 0 as long as there is none
+                m[n][c] = -INFINITY;
+#pragma unroll
+                for (int gi = 0; gi < G; gi++) zs[n][gi][c] = 0.0f;
             }
-#pragma unroll
-            for (int c = 0; c < 2; c++) { l[n][c] = 0.0f; m[n][c] = -INFINITY; }
         }
         float s_limit = 0.0f, s_down = 0.0f;                   // 128 * 2^E, 2^-E of V's scales
 
@@ -312,24 +378,25 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
             if (tile0 + i < tile1) {
                 const int p0 = next_p0, p1 = next_p1;
                 if (tile0 + i + 1 < tile1) { next_p0 = page_of((tile0 + i + 1) * kKeys); next_p1 = page_of((tile0 + i + 1) * kKeys + 16); }
-                load_tile(tile0 + i, i, p0, p1);
+                load_tile(tile0 + i, p0, p1);
             }
             cp_async_commit();
         }
         const int first_hidden = it.len - a.n_tok + row0 / a.group + 1;       // first key that the block's first token does not see
-        int stage = 0, load_stage = S::Stages - 1;
-        for (int tile = tile0; tile < tile1; tile++) {
+        for (int tile = tile0; tile < tile1 && alive; tile++) {
             cp_async_wait<S::Stages - 2>();
+            alive = mbar_wait(full0 + stage * 8, phase, ctl, 1);       // the warp votes
+            if (!alive) break;
+            in_flight--;
             __syncwarp();                                      // every lane's copies have landed, and nobody reads the oldest stage any more
             if (tile + S::Stages - 1 < tile1) {
                 const int p0 = next_p0, p1 = next_p1;
                 if (tile + S::Stages < tile1) { next_p0 = page_of((tile + S::Stages) * kKeys); next_p1 = page_of((tile + S::Stages) * kKeys + 16); }
-                load_tile(tile + S::Stages - 1, load_stage, p0, p1);
+                load_tile(tile + S::Stages - 1, p0, p1);
             }
             cp_async_commit();
-            load_stage = load_stage + 1 == S::Stages ? 0 : load_stage + 1;
-            const uint32_t kb = ring + stage * S::StageBytes, vb = kb + S::CodeBytes, kpb = kb + 2 * S::CodeBytes, vpb = kpb + S::ParamBytes;
-            stage = stage + 1 == S::Stages ? 0 : stage + 1;
+            const uint32_t at = stage * S::StageBytes, kpb = ring + at + 2 * S::CodeBytes + g * 4 * G, vpb = kpb + S::ParamBytes;
+            if (++stage == S::Stages) { stage = 0; phase ^= 1; }
 
             // S^T: keys j * 16 + g and + 8, columns 2t and 2t + 1 of each 8 rows
             float s[2][NT][4];
@@ -337,49 +404,41 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
             for (int j = 0; j < 2; j++) {
                 float acc[G][NT][4];
 #pragma unroll
-                for (int gi = 0; gi < G; gi++)
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) acc[gi][n][e] = -24.0f * q_sum[n][gi][e & 1];
-                const int r0 = j * 16 + g, r1 = r0 + 8;
-                const uint32_t swap = D == 128 ? ((g >> 1) & 1) * 32 : 0;
-#pragma unroll
                 for (int gi = 0; gi < G; gi++) {
-                    const uint2 x0 = lds64(kb + r0 * S::RowBytes + ((gi * 32) ^ swap) + t * 8), x1 = lds64(kb + r1 * S::RowBytes + ((gi * 32) ^ swap) + t * 8);
+                    uint32_t w[4];                             // keys g, g + 8 of piece 2 gi, then of piece 2 gi + 1
+                    ldmatrix4<false>(m_at[gi] + at + j * 16 * S::RowBytes, w);
 #pragma unroll
-                    for (int w = 0; w < 2; w++) {
-                        const uint32_t w0 = w ? x0.y : x0.x, w1 = w ? x1.y : x1.x;
-                        const uint32_t a0[4] = {code16<BF16, 0>(w0), code16<BF16, 0>(w1), code16<BF16, 1>(w0), code16<BF16, 1>(w1)};
-                        const uint32_t a1[4] = {code16<BF16, 2>(w0), code16<BF16, 2>(w1), code16<BF16, 3>(w0), code16<BF16, 3>(w1)};
+                    for (int c = 0; c < 2; c++) {
+                        const uint32_t w0 = w[2 * c], w1 = w[2 * c + 1];
+                        const uint32_t a0[4] = {code16<0, 64>(w0), code16<0, 64>(w1), code16<1, 64>(w0), code16<1, 64>(w1)};
+                        const uint32_t a1[4] = {code16<2, 64>(w0), code16<2, 64>(w1), code16<3, 64>(w0), code16<3, 64>(w1)};
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
-                            mma<BF16>(acc[gi][n], a0, qf[n][gi][w][0], qf[n][gi][w][1]);
-                            mma<BF16>(acc[gi][n], a1, qf[n][gi][w][2], qf[n][gi][w][3]);
+                            if (c == 0) mma_from(acc[gi][n], a0, qf[n][2 * gi][0], qf[n][2 * gi][1], q_init[n][gi][0], q_init[n][gi][1]);
+                            else mma(acc[gi][n], a0, qf[n][2 * gi + c][0], qf[n][2 * gi + c][1]);
+                            mma(acc[gi][n], a1, qf[n][2 * gi + c][2], qf[n][2 * gi + c][3]);
                         }
                     }
                 }
 #pragma unroll
-                for (int e2 = 0; e2 < 2; e2++) {               // keys r0, r1
-                    uint2 pr;
-                    if constexpr (G == 2) pr = lds64(kpb + (e2 ? r1 : r0) * 8);
-                    else pr = make_uint2(lds32(kpb + (e2 ? r1 : r0) * 4), 0u);
-                    float ks[G], kz[G];
+                for (int e2 = 0; e2 < 2; e2++) {
+                    uint32_t pr[G];
+                    lds_pairs<G>(kpb + (j * 16 + e2 * 8) * 4 * G, pr);
+                    float ks[G], kz[G];                        // scale; offset of code 8 over -72, as it meets q_init
 #pragma unroll
                     for (int gi = 0; gi < G; gi++) {
-                        const uint32_t u = gi ? pr.y : pr.x;
-                        const float2 f = unpack16<false>(u);
+                        const float2 f = unpack16<false>(pr[gi]);
                         ks[gi] = f.x;
-                        kz[gi] = fmaf(8.0f, f.x, f.y);
+                        kz[gi] = fmaf(8.0f, f.x, f.y) * (-1.0f / 72.0f);
                     }
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
                         for (int c = 0; c < 2; c++) {
-                            float v = kz[0] * q_sum[n][0][c];
-                            if constexpr (G == 2) v = fmaf(kz[1], q_sum[n][1][c], v);
+                            float v = kz[0] * q_init[n][0][c];
+                            if constexpr (G == 2) v = fmaf(kz[G - 1], q_init[n][G - 1][c], v);
                             v = fmaf(ks[0], acc[0][n][e2 * 2 + c], v);
-                            if constexpr (G == 2) v = fmaf(ks[1], acc[G - 1][n][e2 * 2 + c], v);
+                            if constexpr (G == 2) v = fmaf(ks[G - 1], acc[G - 1][n][e2 * 2 + c], v);
                             s[j][n][e2 * 2 + c] = v;
                         }
                 }
@@ -404,12 +463,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
             for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int e2 = 0; e2 < 2; e2++) {
-                    uint2 pr;
-                    if constexpr (G == 2) pr = lds64(vpb + (j * 16 + e2 * 8 + g) * 8);
-                    else pr = make_uint2(lds32(vpb + (j * 16 + e2 * 8 + g) * 4), 0u);
+                    uint32_t pr[G];
+                    lds_pairs<G>(vpb + (j * 16 + e2 * 8) * 4 * G, pr);
 #pragma unroll
                     for (int gi = 0; gi < G; gi++) {
-                        const float2 f = unpack16<false>(gi ? pr.y : pr.x);
+                        const float2 f = unpack16<false>(pr[gi]);
                         vs[j][e2][gi] = f.x;
                         vz[j][e2][gi] = fmaf(8.0f, f.x, f.y);
                         s_max = fmaxf(s_max, f.x);
@@ -423,7 +481,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     t_max[n][c] = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
-                    raise |= (t_max[n][c] - m[n][c]) * a.scale_log2 > kGrow || (m[n][c] == -INFINITY && t_max[n][c] > -INFINITY);
+                    raise |= (t_max[n][c] - m[n][c]) * sc[n][c] > kGrow;       // no max yet: inf, unless every key is masked
                 }
             if (__any_sync(0xffffffffu, raise)) {
                 float ratio = 1.0f;
@@ -444,63 +502,68 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
 #pragma unroll
                         for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
                         mx = fmaxf(mx, m[n][c]);
-                        const float alpha = m[n][c] == -INFINITY ? 1.0f : ex2((m[n][c] - mx) * a.scale_log2);   // nothing summed so far: leave it
+                        const float alpha = m[n][c] == -INFINITY ? 1.0f : ex2((m[n][c] - mx) * sc[n][c]);   // nothing summed so far: leave it
                         m[n][c] = mx;
+                        mc[n][c] = mx == -INFINITY ? 0.0f : mx * sc[n][c];
                         l[n][c] *= alpha;
 #pragma unroll
-                        for (int gi = 0; gi < G; gi++) {
-                            zs[n][gi][c] *= alpha;
+                        for (int gi = 0; gi < G; gi++) zs[n][gi][c] *= alpha;
 #pragma unroll
-                            for (int i = 0; i < 4; i++) { o[n][gi][i][c] *= alpha * ratio; o[n][gi][i][2 + c] *= alpha * ratio; }
-                        }
+                        for (int i = 0; i < 2 * P; i++) { o[n][i / 2][i % 2][c] *= alpha * ratio; o[n][i / 2][i % 2][2 + c] *= alpha * ratio; }
                     }
             }
             // P, its sums, and the brackets as operand B: columns to rows across the warp
             uint32_t pf[2][NT][G][2];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const float mc0 = m[n][0] == -INFINITY ? 0.0f : m[n][0] * a.scale_log2, mc1 = m[n][1] == -INFINITY ? 0.0f : m[n][1] * a.scale_log2;
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int j = 0; j < 2; j++)
+                for (int e2 = 0; e2 < 2; e2++) {
+                    float sd[G];
 #pragma unroll
-                    for (int e2 = 0; e2 < 2; e2++) {
-                        const float p0 = ex2(fmaf(s[j][n][e2 * 2], a.scale_log2, -mc0)), p1 = ex2(fmaf(s[j][n][e2 * 2 + 1], a.scale_log2, -mc1));
+                    for (int gi = 0; gi < G; gi++) sd[gi] = vs[j][e2][gi] * s_down;
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const float p0 = ex2(fmaf(s[j][n][e2 * 2], sc[n][0], -mc[n][0])), p1 = ex2(fmaf(s[j][n][e2 * 2 + 1], sc[n][1], -mc[n][1]));
                         l[n][0] += p0;
                         l[n][1] += p1;
 #pragma unroll
                         for (int gi = 0; gi < G; gi++) {
                             zs[n][gi][0] = fmaf(p0, vz[j][e2][gi], zs[n][gi][0]);
                             zs[n][gi][1] = fmaf(p1, vz[j][e2][gi], zs[n][gi][1]);
-                            const float sd = vs[j][e2][gi] * s_down;
-                            pf[j][n][gi][e2] = transpose8x8(pack16<false>(p0 * sd, p1 * sd));
-                        }
-                    }
-            }
-            // O^T: elements 8g .. 8g + 7 of each group, a pair of them per product of 16 rows
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int ra = j * 16 + 2 * t;
-                const uint32_t row_a = vb + v_row(ra) * S::RowBytes, row_b = vb + v_row(ra + 1) * S::RowBytes;
-                const uint32_t row_c = vb + v_row(ra + 8) * S::RowBytes, row_d = vb + v_row(ra + 9) * S::RowBytes;
-#pragma unroll
-                for (int gi = 0; gi < G; gi++) {
-                    const uint32_t at = (D == 128 ? ((gi ^ (t >> 1)) & 1) * 32 : 0) + g * 4;
-                    const uint32_t xa = lds32(row_a + at), xb = lds32(row_b + at), xc = lds32(row_c + at), xd = lds32(row_d + at);
-#pragma unroll
-                    for (int hf = 0; hf < 2; hf++) {           // elements 0..3, 4..7
-                        const uint32_t y0 = __byte_perm(xa, xb, hf ? 0x7632 : 0x5410), y1 = __byte_perm(xc, xd, hf ? 0x7632 : 0x5410);
-                        const uint32_t a0[4] = {centred(code16<false, 0>(y0)), centred(code16<false, 1>(y0)), centred(code16<false, 0>(y1)), centred(code16<false, 1>(y1))};
-                        const uint32_t a1[4] = {centred(code16<false, 2>(y0)), centred(code16<false, 3>(y0)), centred(code16<false, 2>(y1)), centred(code16<false, 3>(y1))};
-#pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            mma<false>(o[n][gi][2 * hf], a0, pf[j][n][gi][0], pf[j][n][gi][1]);
-                            mma<false>(o[n][gi][2 * hf + 1], a1, pf[j][n][gi][0], pf[j][n][gi][1]);
+                            pf[j][n][gi][e2] = transpose8x8(pack16<false>(p0 * sd[gi], p1 * sd[gi]));
                         }
                     }
                 }
-            }
+            // O^T: elements 4g .. 4g + 3 of each piece, two of them per product of 16 rows
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int gi = 0; gi < G; gi++) {
+                    uint32_t y[4];                             // keys 2t, 2t + 1 and 2t + 8, 2t + 9 of piece 2 gi, then of piece 2 gi + 1
+                    ldmatrix4<true>(m_at[gi] + at + S::CodeBytes + j * 16 * S::RowBytes, y);
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const uint32_t y0 = y[2 * c], y1 = y[2 * c + 1];
+                        const uint32_t a0[4] = {code16<0, -8>(y0), code16<1, -8>(y0), code16<0, -8>(y1), code16<1, -8>(y1)};
+                        const uint32_t a1[4] = {code16<2, -8>(y0), code16<3, -8>(y0), code16<2, -8>(y1), code16<3, -8>(y1)};
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            mma(o[n][2 * gi + c][0], a0, pf[j][n][gi][0], pf[j][n][gi][1]);
+                            mma(o[n][2 * gi + c][1], a1, pf[j][n][gi][0], pf[j][n][gi][1]);
+                        }
+                    }
+                }
         }
         cp_async_wait<0>();
+        if (!alive) {
+            // a copy did not arrive: the status word says so.  Give those under way as long again, so that none lands in the
+            // shared memory of another CTA, and leave the results as they are.
+            const WaitCtl last{&s_never, a.status};
+            for (; in_flight > 0; in_flight--) {
+                mbar_wait(full0 + stage * 8, phase, last, 2);
+                if (++stage == S::Stages) { stage = 0; phase ^= 1; }
+            }
+        }
         __syncwarp();
 
         // ---- the item's sums, or this warp's part of them
@@ -526,34 +589,23 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
                     for (int gi = 0; gi < G; gi++) zs[n][gi][c] += __shfl_xor_sync(0xffffffffu, zs[n][gi][c], off);
                 }
                 const int r = n * 8 + 2 * t + c;
+                const float inv = l[n][c] == 0.0f ? 0.0f : 1.0f / l[n][c];
+                const int tok = (row0 + r) / a.group, hh = (row0 + r) - tok * a.group;
+                const long long row = ((long long)it.b * a.n_tok + tok) * a.hq + (long long)it.h * a.group + hh;
 #pragma unroll
-                for (int gi = 0; gi < G; gi++) {
-                    float f[8];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        f[2 * i] = fmaf(o[n][gi][i][c], up, zs[n][gi][c]);
-                        f[2 * i + 1] = fmaf(o[n][gi][i][2 + c], up, zs[n][gi][c]);
-                    }
+                for (int i = 0; i < P; i++) {
+                    const float z = zs[n][i / 2][c];
+                    const float4 f = make_float4(fmaf(o[n][i][0][c], up, z), fmaf(o[n][i][0][2 + c], up, z), fmaf(o[n][i][1][c], up, z), fmaf(o[n][i][1][2 + c], up, z));
                     if (!whole) {
-                        float4* p = reinterpret_cast<float4*>(record + r * D + gi * kU4Group + g * 8);
-                        p[0] = make_float4(f[0], f[1], f[2], f[3]);
-                        p[1] = make_float4(f[4], f[5], f[6], f[7]);
+                        *reinterpret_cast<float4*>(record + r * D + i * 32 + g * 4) = f;
                     } else if (row0 + r < a.rows) {
-                        const float inv = l[n][c] == 0.0f ? 0.0f : 1.0f / l[n][c];
-                        const int tok = (row0 + r) / a.group, hh = (row0 + r) - tok * a.group;
-                        const long long row = ((long long)it.b * a.n_tok + tok) * a.hq + (long long)it.h * a.group + hh;
-                        uint4 y;
-                        y.x = pack16<BF16>(f[0] * inv, f[1] * inv);
-                        y.y = pack16<BF16>(f[2] * inv, f[3] * inv);
-                        y.z = pack16<BF16>(f[4] * inv, f[5] * inv);
-                        y.w = pack16<BF16>(f[6] * inv, f[7] * inv);
-                        *reinterpret_cast<uint4*>(a.o + row * D + gi * kU4Group + g * 8) = y;
-                        if (gi == 0 && g == 0 && a.lse != nullptr)
-                            a.lse[row] = l[n][c] == 0.0f ? -INFINITY : kLn2 * (m[n][c] * a.scale_log2 + log2f(l[n][c]));
+                        *reinterpret_cast<uint2*>(a.o + row * D + i * 32 + g * 4) = make_uint2(pack16<BF16>(f.x * inv, f.y * inv), pack16<BF16>(f.z * inv, f.w * inv));
                     }
                 }
+                if (whole && row0 + r < a.rows && g == 0 && a.lse != nullptr)
+                    a.lse[row] = l[n][c] == 0.0f ? -INFINITY : kLn2 * (mc[n][c] + log2f(l[n][c]));
                 if (!whole && g == 0) {
-                    record[S::Rows * D + r] = m[n][c] == -INFINITY ? -INFINITY : m[n][c] * a.scale_log2;
+                    record[S::Rows * D + r] = m[n][c] == -INFINITY ? -INFINITY : mc[n][c];
                     record[S::Rows * (D + 1) + r] = l[n][c];
                 }
             }
@@ -727,7 +779,7 @@ template <int D, bool BF16, int NT>
 int run_u4(const U4Args& a, int ctas, DeviceState* st, cudaStream_t stream) {
     using S = Shape<D, NT>;
     static bool configured[64] = {};
-    const int smem = kWarps * S::WarpBytes;
+    const int smem = kWarps * S::WarpBytes + 1024;
     if (!configured[st->device]) {
         FA_CUDA_TRY(cudaFuncSetAttribute(u4_kernel<D, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         configured[st->device] = true;
@@ -778,18 +830,21 @@ FA_EXPORT int fa_decode_gqa_u4(const fa_decode_gqa_u4_args* p) {
     if (st->cc_major != 10) return FA_ERR_NOT_SM100;
     const Plan plan = make_plan(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->d_head, st->sm_count);
     if (!p->workspace || p->workspace_bytes < plan.bytes || !aligned16(p->workspace)) return FA_ERR_WORKSPACE;
+    const bool paged = p->layout.block_table != nullptr;
+    const int block_rows = paged ? p->layout.page_size : p->seq_len_kv, blocks = paged ? p->layout.num_pages : p->batch_size;
+    for (int i = 0; i < 2; i++) {
+        rc = make_tensor_map_u4(i ? &a.tv : &a.tk, i ? p->v_cache : p->k_cache, p->d_head / 2, block_rows, p->num_kv_heads, blocks,
+                                p->layout.row_stride, p->layout.head_stride, p->layout.block_stride, paged && block_rows < kKeys ? block_rows : kKeys);
+        if (rc != FA_OK) return rc;
+    }
+    a.status = st->status;
     a.q = static_cast<const uint16_t*>(p->q);
-    a.k = static_cast<const uint8_t*>(p->k_cache);
-    a.v = static_cast<const uint8_t*>(p->v_cache);
     a.kp = static_cast<const __half2*>(p->k_params);
     a.vp = static_cast<const __half2*>(p->v_params);
     a.o = static_cast<uint16_t*>(p->o);
     a.lse = p->lse;
     a.scratch = static_cast<float*>(p->workspace);
     a.meta = reinterpret_cast<int2*>(static_cast<uint8_t*>(p->workspace) + align256(plan.record * plan.ctas * (kWarps + 2)));
-    a.block_stride = p->layout.block_stride;
-    a.head_stride = p->layout.head_stride;
-    a.row_stride = p->layout.row_stride;
     a.p_block_stride = p->layout.param_block_stride;
     a.p_head_stride = p->layout.param_head_stride;
     a.p_row_stride = p->layout.param_row_stride;

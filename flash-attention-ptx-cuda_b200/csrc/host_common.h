@@ -100,6 +100,11 @@ int make_tensor_map_4d(CUtensorMap* out, const void* base, int dtype, uint64_t r
 int make_tensor_map_q5(CUtensorMap* out, const void* base, int dtype, uint64_t d_head, uint64_t group,
                        uint64_t n_tok, uint64_t n_kv_heads, uint64_t batch, uint32_t box_cols);
 
+// Rank-4 tensor map over the codes of a 4-bit cache: dims (row_bytes, n_rows, n_heads, n_blocks), strides in bytes (multiples
+// of 16); a box is `box_rows` whole rows of 32 or 64 bytes, in shared memory swizzled as wide as the row.
+int make_tensor_map_u4(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t n_rows, uint64_t n_heads, uint64_t n_blocks,
+                       uint64_t row_stride, uint64_t head_stride, uint64_t block_stride, uint32_t box_rows);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Implemented next to their kernels.

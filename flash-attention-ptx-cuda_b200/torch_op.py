@@ -22,11 +22,13 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.utils._python_dispatch import is_in_torch_dispatch_mode
 
 import fa_b200 as _fa
 from fa_b200 import FaError
 
 _DTYPES = {torch.float16: "f16", torch.bfloat16: "bf16"}
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def _check(q, k, v):
@@ -210,13 +212,7 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "pla
     return torch.tensor(list(out), dtype=torch.float64), amp
 
 
-@torch.library.custom_op("fa_b200::rope", mutates_args=())
-def rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,
-         interleaved: bool = False, amplitude: float = 1.0, inverse: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
-    """Rotary positions (``fa_rope``) of q ``[B, Hq, S, D]`` and k ``[B, Hkv, S, D]`` (any strides; Hkv may be 0).
-
-    ``inv_freq`` float64 ``[rotary_dim / 2]`` in CPU memory; ``positions`` integer ``[S]`` or ``[B, S]`` on the device,
-    default 0 .. S-1; ``inverse`` turns back.  Returns the rotated (q, k), contiguous."""
+def _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse):
     if q.dtype not in _DTYPES or k.dtype != q.dtype:
         raise TypeError("fa_b200: q and k must share dtype float16 or bfloat16")
     if not (q.is_cuda and k.is_cuda):
@@ -241,7 +237,13 @@ def rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, positions: to
     return q_out, k_out
 
 
-@rope.register_fake
+@torch.library.custom_op("fa_b200::rope", mutates_args=())
+def _rope_op(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,
+             interleaved: bool = False, amplitude: float = 1.0, inverse: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    return _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse)
+
+
+@_rope_op.register_fake
 def _(q, k, inv_freq, positions=None, interleaved=False, amplitude=1.0, inverse=False):
     return q.new_empty(q.shape), k.new_empty(k.shape)
 
@@ -260,6 +262,28 @@ def _rope_backward(ctx, d_q, d_k):
 
 
 torch.library.register_autograd("fa_b200::rope", _rope_backward, setup_context=_rope_setup_context)
+
+
+class _Rope(torch.autograd.Function):
+    forward = staticmethod(_run_rope)
+    setup_context = staticmethod(_rope_setup_context)
+    backward = staticmethod(_rope_backward)
+
+
+def rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,
+         interleaved: bool = False, amplitude: float = 1.0, inverse: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rotary positions (``fa_rope``) of q ``[B, Hq, S, D]`` and k ``[B, Hkv, S, D]`` (any strides; Hkv may be 0).
+
+    ``inv_freq`` float64 ``[rotary_dim / 2]`` in CPU memory; ``positions`` integer ``[S]`` or ``[B, S]`` on the device,
+    default 0 .. S-1; ``inverse`` turns back.  Returns the rotated (q, k), contiguous.
+
+    ``torch.ops.fa_b200.rope`` is the same; plain tensors in eager mode go to the kernel without the dispatcher, whose
+    20 us a call a short prompt would feel."""
+    if type(q) in _PLAIN and type(k) in _PLAIN and not torch.compiler.is_compiling() and not is_in_torch_dispatch_mode():
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+            return _Rope.apply(q, k, inv_freq, positions, interleaved, amplitude, inverse)
+        return _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse)
+    return torch.ops.fa_b200.rope(q, k, inv_freq, positions, interleaved, amplitude, inverse)
 
 
 def u4_cache(blocks: int, rows: int, num_kv_heads: int, d_head: int, device="cuda") -> tuple[torch.Tensor, torch.Tensor]:

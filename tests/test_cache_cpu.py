@@ -121,6 +121,24 @@ def test_attention_workspace(fa):
     assert 0 < size(1, 4, 2, 1, 64, 128) <= size(8, 4, 2, 1, 4096, 128) == size(8, 4, 2, 0, 4096, 128)
 
 
+@pytest.mark.parametrize("name", ["RopeArgs", "CacheAppendArgs", "CacheReadArgs", "DecodeGqaU4Args"])
+def test_packed_arguments_have_the_structures_layout(fa, name):
+    cls, values, at = getattr(fa, name), [], [0]
+
+    def fill(obj):
+        for field, t in obj._fields_:
+            if issubclass(t, ctypes.Structure):
+                fill(getattr(obj, field))
+            else:
+                at[0] += 1
+                v = at[0] + 0.5 if t in (ctypes.c_float, ctypes.c_double) else at[0]
+                setattr(obj, field, v)
+                values.append(v)
+    obj = cls()
+    fill(obj)
+    assert fa._packer(cls)(*values) == bytes(obj)
+
+
 def test_null_arguments(fa):
     lib = fa.lib()
     for name in ("fa_rope", "fa_cache_append", "fa_cache_read_u4", "fa_decode_gqa_u4"):
