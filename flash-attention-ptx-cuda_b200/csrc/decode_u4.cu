@@ -19,13 +19,15 @@
 //
 // Work split.  All (sequence, KV head, row block) items are laid out one after the other in tiles of 32 keys, and the
 // resulting line is cut into equal parts, one for each warp of the GPU, whatever the lengths of the sequences: a warp may
-// finish one item, do several and begin the next.  A warp streams its tiles through a cp.async ring of its own and meets
-// the others only once, at the end, where the CTA merges what its warps have of the same item.  Items that lie in
-// several CTAs go through the workspace and a second small kernel.
+// finish one item, do several and begin the next.  A warp streams its tiles through a ring of its own and meets the others
+// only once, at the end, where the CTA merges what its warps have of the same item.  Items that lie in several CTAs go
+// through the workspace and a second small kernel.  Short jobs are done in one launch instead: a cluster of up to 8 CTAs an
+// item, which merges through distributed shared memory (plan.cluster says when).
 #include <cmath>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "fast_div.h"
 #include "host_common.h"
 #include "ptx.cuh"
 #include "u4.cuh"
@@ -34,8 +36,10 @@ namespace fa {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kMaxCluster = 8;                 // portable cluster size
 constexpr int kKeys = 32;                      // keys of a tile
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kClusterTiles = 8;               // see make_plan
 constexpr float kGrow = 8.0f;                  // a running max may be exceeded by this much (in powers of two) before it is raised
 
 struct U4Args {
@@ -46,13 +50,21 @@ struct U4Args {
     float* lse;
     float* scratch;                            // head records of the warps, then two records a CTA
     int* status;
-    int2* meta;                                // per CTA: item of the tail record or -1; head record: 0 none, 1 ends here, 2 goes on
+    int2* meta;                                // per CTA: item that begins in it and goes on (or -1), one past the last CTA of that item
     long long p_block_stride, p_head_stride, p_row_stride;    // pairs
     CacheMap map;
     const int* seq_lens;
     int batch, hq, hkv, group, n_tok, rows, row_blocks, kv_len;
+    int cluster;                               // CTAs of an item's cluster; 0: the line
+    FastDiv by_group, by_row_blocks, by_hkv, by_cluster;
     float scale_log2;
 };
+
+// Output row of query row r of a (sequence, KV head): token r / group, head r % group of the group.
+__device__ __forceinline__ long long out_row(const U4Args& a, int b, int h, int r) {
+    const int tok = a.by_group.quot(r);
+    return ((long long)b * a.n_tok + tok) * a.hq + (long long)h * a.group + (r - tok * a.group);
+}
 
 // Shapes of an instance: D, row columns of 8.
 template <int D, int NT>
@@ -141,6 +153,38 @@ __device__ __forceinline__ uint32_t code16(uint32_t x) {
 template <int D>
 __device__ __forceinline__ int piece(int r, int c) { return D == 128 ? c ^ ((r >> 1) & 3) : c ^ ((r >> 2) & 1); }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// What CTA `rank` of the cluster has at this CTA's shared address `p`.
+__device__ __forceinline__ uint32_t cluster_address(const float* p, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster(const float* p, int rank) {
+    float x;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(cluster_address(p, rank)) : "memory");
+    return x;
+}
+__device__ __forceinline__ float4 ld_cluster4(const float* p, int rank) {
+    float4 x;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(cluster_address(p, rank)) : "memory");
+    return x;
+}
+
+// Weight of a record (its max in powers of two, its sum) in a merge with maximum `mx`: none if it is empty; a NaN sum without a
+// max is kept.
+__device__ __forceinline__ float record_weight(float m, float l, float mx) { return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : ex2(m - mx); }
+
+// Four elements of an output row from its sums, and the row's LSE with the first of them.
+template <int D, bool BF16>
+__device__ __forceinline__ void store_quad(const U4Args& a, long long row, int d, const float4& f, float m, float l) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<uint2*>(a.o + row * D + d) = make_uint2(pack16<BF16>(f.x * inv, f.y * inv), pack16<BF16>(f.z * inv, f.w * inv));
+    if (d == 0 && a.lse != nullptr) a.lse[row] = l == 0.0f ? -INFINITY : kLn2 * (m + log2f(l));
+}
+
 struct Item {
     int b, h, rb, len, tiles;      // sequence, KV head, row block, its keys, tiles of 32 of them (at least one)
 };
@@ -152,13 +196,16 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
     constexpr int G = S::G;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);      // the swizzle goes by the address
+    constexpr int kRecords = 2 * kWarps;                       // of a CTA, in the order of the line: head and tail of warp 0, of warp 1, ...
     __shared__ __align__(8) uint64_t s_full[kWarps][S::Stages];
     __shared__ int s_abort, s_never;
-    __shared__ long long s_prefix[kWarps * 32];                // tiles (of one head and row block) before a thread's sequences
-    __shared__ long long s_total;
-    __shared__ int s_head_item[kWarps], s_tail_item[kWarps], s_before[kWarps], s_after[kWarps];
+    __shared__ int s_prefix[kWarps * 32], s_warp[kWarps];      // tiles (of one head and row block) before a thread's sequences
+    __shared__ int s_item[kRecords], s_before[kWarps], s_after[kWarps];
+    __shared__ float s_m[kRecords][S::Rows], s_l[kRecords][S::Rows], s_w[kRecords][S::Rows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     if (tid == 0) {
+        prefetch_tensormap(&a.tk);
+        prefetch_tensormap(&a.tv);
         s_abort = s_never = 0;
         for (int i = 0; i < kWarps * S::Stages; i++) mbar_init(smem_u32(&s_full[0][0] + i), 1);
         fence_mbar_init();
@@ -167,57 +214,69 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
     grid_dependency_wait();
     grid_launch_dependents();
 
-    // ---- the line of tiles, and this warp's part of it
+    // ---- this warp's part of the line, and the item that it begins in
     const int per_b = a.hkv * a.row_blocks;                    // items of a sequence
-    const int per_thread = (a.batch + kWarps * 32 - 1) / (kWarps * 32);   // sequences of a thread
-    if (a.seq_lens != nullptr) {
-        long long sum = 0;
-        for (int i = 0; i < per_thread; i++) {
-            const int b = tid * per_thread + i;
-            if (b < a.batch) sum += tiles_of(sequence_length(a.seq_lens, b, a.kv_len));
-        }
-        long long inc = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += y;
-        }
-        __shared__ long long s_warp[kWarps];
-        if (lane == 31) s_warp[warp] = inc;
-        __syncthreads();
-        long long base = 0, total = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) {
-            if (w < warp) base += s_warp[w];
-            total += s_warp[w];
-        }
-        s_prefix[tid] = base + inc - sum;
-        if (tid == 0) s_total = total;
-    } else if (tid == 0) {
-        s_total = (long long)a.batch * tiles_of(a.kv_len);
-    }
-    __syncthreads();
-    const long long total = s_total * per_b;
-    // equal parts of at least one tile a warp: CTAs without tiles come last, so those of an item follow one another
-    const long long chunk = max((total + gridDim.x - 1) / gridDim.x, (long long)kWarps);
-    const long long c_begin = min(total, chunk * blockIdx.x), c_end = min(total, c_begin + chunk);
-    const long long w_begin = c_begin + (c_end - c_begin) * warp / kWarps, w_end = c_begin + (c_end - c_begin) * (warp + 1) / kWarps;
-
-    const uint32_t ring = smem_u32(smem) + warp * S::WarpBytes;
-    float* tail_record = reinterpret_cast<float*>(smem + warp * S::WarpBytes);
-    float* head_record = a.scratch + (size_t)(blockIdx.x * kWarps + warp) * S::Record;
-    int head_item = -1, tail_item = -1, before = 0, after = 0;
-
     Item it{0, 0, 0, 0, 0};
-    long long item_start = 0;
-    if (w_begin < w_end) {
-        long long b_start;                                     // first tile of sequence it.b
+    int item_start = 0, chunk = 0, rank = 0;
+    int c_begin, c_end, w_begin, w_end;
+    if (a.cluster > 0) {                                       // an item of its own: the line is that item
+        const int item = a.by_cluster.quot(blockIdx.x), bh = a.by_row_blocks.quot(item);
+        rank = blockIdx.x - item * a.cluster;
+        it.rb = item - bh * a.row_blocks;
+        it.b = a.by_hkv.quot(bh);
+        it.h = bh - it.b * a.hkv;
+        it.len = sequence_length(a.seq_lens, it.b, a.kv_len);
+        it.tiles = tiles_of(it.len);
+        c_begin = a.by_cluster.quot(it.tiles * rank);
+        c_end = a.by_cluster.quot(it.tiles * (rank + 1));
+        __syncthreads();                                       // the barriers are ready
+    } else {
+        const int per_thread = (a.batch + kWarps * 32 - 1) / (kWarps * 32);   // sequences of a thread
+        int total = a.batch * tiles_of(a.kv_len);
+        if (a.seq_lens != nullptr) {
+            int sum = 0;
+            for (int i = 0; i < per_thread; i++) {
+                const int b = tid * per_thread + i;
+                if (b < a.batch) sum += tiles_of(sequence_length(a.seq_lens, b, a.kv_len));
+            }
+            int inc = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += y;
+            }
+            if (lane == 31) s_warp[warp] = inc;
+            __syncthreads();
+            int base = 0;
+            total = 0;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                if (w < warp) base += s_warp[w];
+                total += s_warp[w];
+            }
+            s_prefix[tid] = base + inc - sum;
+        }
+        __syncthreads();
+        total *= per_b;
+        // equal parts of at least one tile a warp: CTAs without tiles come last, so those of an item follow one another
+        chunk = max((total + (int)gridDim.x - 1) / (int)gridDim.x, kWarps);
+        c_begin = (int)min((long long)total, (long long)chunk * blockIdx.x);
+        c_end = min(total - c_begin, chunk) + c_begin;
+    }
+    {
+        const int n = c_end - c_begin, q = n / kWarps, rest = n % kWarps;
+        w_begin = c_begin + warp * q + min(warp, rest);
+        w_end = w_begin + q + (warp < rest ? 1 : 0);
+    }
+    if (a.cluster == 0 && w_begin < w_end) {
+        int b_start;                                           // first tile of sequence it.b
         if (a.seq_lens == nullptr) {
             it.tiles = tiles_of(a.kv_len);
             it.len = a.kv_len;
-            it.b = (int)(w_begin / ((long long)it.tiles * per_b));
-            b_start = (long long)it.b * it.tiles * per_b;
+            it.b = w_begin / (it.tiles * per_b);
+            b_start = it.b * it.tiles * per_b;
         } else {
+            const int per_thread = (a.batch + kWarps * 32 - 1) / (kWarps * 32);
             int lo = 0, hi = kWarps * 32 - 1;                  // last thread whose sequences begin at or before w_begin
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
@@ -229,17 +288,22 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
             for (;;) {
                 it.len = sequence_length(a.seq_lens, it.b, a.kv_len);
                 it.tiles = tiles_of(it.len);
-                const long long end = b_start + (long long)it.tiles * per_b;
+                const int end = b_start + it.tiles * per_b;
                 if (w_begin < end || it.b + 1 >= a.batch) break;
                 b_start = end;
                 it.b++;
             }
         }
-        const int i = (int)((w_begin - b_start) / it.tiles);   // item of the sequence
-        it.h = i / a.row_blocks;
+        const int i = (w_begin - b_start) / it.tiles;          // item of the sequence
+        it.h = a.by_row_blocks.quot(i);
         it.rb = i - it.h * a.row_blocks;
-        item_start = b_start + (long long)i * it.tiles;
+        item_start = b_start + i * it.tiles;
     }
+
+    const uint32_t ring = smem_u32(smem) + warp * S::WarpBytes;
+    float* tail_record = reinterpret_cast<float*>(smem + warp * S::WarpBytes);
+    float* head_record = a.scratch + (size_t)(blockIdx.x * kWarps + warp) * S::Record;
+    int head_item = -1, tail_item = -1, before = 0, after = 0;
 
     // ---- the warp's ring: a barrier a stage, which TMA's copies of the codes complete; scale and offset pairs, 4 or 8 bytes
     // of any row stride, come by cp.async
@@ -257,11 +321,51 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
     for (int c = 0; c < P / 2; c++) m_at[c] = ring + m_row * S::RowBytes + piece<D>(m_row, 2 * c + (lane >> 4)) * 16;
 
     // ---- item by item
-    for (long long x = w_begin; x < w_end && alive;) {
-        const int tile0 = (int)(x - item_start);
-        const int tile1 = (int)min((long long)it.tiles, tile0 + (w_end - x));
+    for (int x = w_begin; x < w_end && alive;) {
+        const int tile0 = x - item_start, tile1 = min(it.tiles, tile0 + w_end - x);
         const int row0 = it.rb * S::Rows;
 
+        // ---- loads of a tile
+        const long long hp_off = (long long)it.h * a.p_head_stride;
+        auto page_of = [&](int key) -> int {                   // -1: names none, or past the end
+            if (key >= it.len) return -1;
+            if (a.map.page_shift < 0) return it.b;
+            const int p = a.map.block_table[(long long)it.b * a.map.table_stride + (key >> a.map.page_shift)];
+            return (unsigned)p < (unsigned)a.map.n_pages ? p : -1;
+        };
+        auto load_tile = [&](int tile, int p0, int p1) {
+            const int k0 = tile * kKeys;
+            const uint32_t dst = ring + load_stage * S::StageBytes, bar = full0 + load_stage * 8;
+            load_stage = load_stage + 1 == S::Stages ? 0 : load_stage + 1;
+            in_flight++;
+            if (elect_one()) {
+                // rows past the block and pages that name none read as zero; rows past the sequence's end hold any codes, and are masked
+                mbar_arrive_expect_tx(bar, 2 * S::CodeBytes);
+                tma_load_4d(dst, &a.tk, bar, 0, k0 & in_page, it.h, p0);
+                tma_load_4d(dst + S::CodeBytes, &a.tv, bar, 0, k0 & in_page, it.h, p0);
+                if (two_boxes) {
+                    tma_load_4d(dst + S::CodeBytes / 2, &a.tk, bar, 0, 0, it.h, p1);
+                    tma_load_4d(dst + S::CodeBytes + S::CodeBytes / 2, &a.tv, bar, 0, 0, it.h, p1);
+                }
+            }
+            const uint32_t pdst = dst + 2 * S::CodeBytes + lane * 4 * G;
+            const int key = k0 + lane, p = lane < 16 ? p0 : p1;
+            const bool ok = key < it.len && p >= 0;
+            const long long off = ok ? p * a.p_block_stride + hp_off + (long long)(key & in_page) * a.p_row_stride : 0;
+            cp_async_or_zero<4 * G>(pdst, a.kp + off, ok);
+            cp_async_or_zero<4 * G>(pdst + S::ParamBytes, a.vp + off, ok);
+        };
+
+        int next_p0 = page_of(tile0 * kKeys), next_p1 = page_of(tile0 * kKeys + 16);
+#pragma unroll
+        for (int i = 0; i < S::Stages - 1; i++) {
+            if (tile0 + i < tile1) {
+                const int p0 = next_p0, p1 = next_p1;
+                if (tile0 + i + 1 < tile1) { next_p0 = page_of((tile0 + i + 1) * kKeys); next_p1 = page_of((tile0 + i + 1) * kKeys + 16); }
+                load_tile(tile0 + i, p0, p1);
+            }
+            cp_async_commit();
+        }
         // q as operand B: column g of the n-th 8 rows; 8 elements of a 16-byte piece of codes are two steps of k, in pairs
         // (i, i + 4) as the codes lie in a word.  bf16 rows are brought to fp16 by a power of two that puts their
         // largest element at 2^14: exact for elements down to 2^-28 of that one, and the rest is below its 32-bit rounding.
@@ -271,8 +375,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const int r = row0 + n * 8 + g;
-            const int tok = r / a.group, hh = r - tok * a.group;
-            const uint16_t* qp = a.q + (((long long)it.b * a.n_tok + tok) * a.hq + (long long)it.h * a.group + hh) * D;
+            const uint16_t* qp = a.q + out_row(a, it.b, it.h, r) * D;
             uint4 u[P];
 #pragma unroll
             for (int c = 0; c < P; c++) u[c] = r < a.rows ? *reinterpret_cast<const uint4*>(qp + c * 32 + t * 8) : make_uint4(0, 0, 0, 0);
@@ -322,37 +425,6 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
             }
         }
 
-        // ---- loads of a tile
-        const long long hp_off = (long long)it.h * a.p_head_stride;
-        auto page_of = [&](int key) -> int {                   // -1: names none, or past the end
-            if (key >= it.len) return -1;
-            if (a.map.page_shift < 0) return it.b;
-            const int p = a.map.block_table[(long long)it.b * a.map.table_stride + (key >> a.map.page_shift)];
-            return (unsigned)p < (unsigned)a.map.n_pages ? p : -1;
-        };
-        auto load_tile = [&](int tile, int p0, int p1) {
-            const int k0 = tile * kKeys;
-            const uint32_t dst = ring + load_stage * S::StageBytes, bar = full0 + load_stage * 8;
-            load_stage = load_stage + 1 == S::Stages ? 0 : load_stage + 1;
-            in_flight++;
-            if (elect_one()) {
-                // rows past the block and pages that name none read as zero; rows past the sequence's end hold any codes, and are masked
-                mbar_arrive_expect_tx(bar, 2 * S::CodeBytes);
-                tma_load_4d(dst, &a.tk, bar, 0, k0 & in_page, it.h, p0);
-                tma_load_4d(dst + S::CodeBytes, &a.tv, bar, 0, k0 & in_page, it.h, p0);
-                if (two_boxes) {
-                    tma_load_4d(dst + S::CodeBytes / 2, &a.tk, bar, 0, 0, it.h, p1);
-                    tma_load_4d(dst + S::CodeBytes + S::CodeBytes / 2, &a.tv, bar, 0, 0, it.h, p1);
-                }
-            }
-            const uint32_t pdst = dst + 2 * S::CodeBytes + lane * 4 * G;
-            const int key = k0 + lane, p = lane < 16 ? p0 : p1;
-            const bool ok = key < it.len && p >= 0;
-            const long long off = ok ? p * a.p_block_stride + hp_off + (long long)(key & in_page) * a.p_row_stride : 0;
-            cp_async_or_zero<4 * G>(pdst, a.kp + off, ok);
-            cp_async_or_zero<4 * G>(pdst + S::ParamBytes, a.vp + off, ok);
-        };
-
         float o[NT][P][2][4], l[NT][2], m[NT][2], mc[NT][2], zs[NT][G][2];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
@@ -372,17 +444,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
         }
         float s_limit = 0.0f, s_down = 0.0f;                   // 128 * 2^E, 2^-E of V's scales
 
-        int next_p0 = page_of(tile0 * kKeys), next_p1 = page_of(tile0 * kKeys + 16);
-#pragma unroll
-        for (int i = 0; i < S::Stages - 1; i++) {
-            if (tile0 + i < tile1) {
-                const int p0 = next_p0, p1 = next_p1;
-                if (tile0 + i + 1 < tile1) { next_p0 = page_of((tile0 + i + 1) * kKeys); next_p1 = page_of((tile0 + i + 1) * kKeys + 16); }
-                load_tile(tile0 + i, p0, p1);
-            }
-            cp_async_commit();
-        }
-        const int first_hidden = it.len - a.n_tok + row0 / a.group + 1;       // first key that the block's first token does not see
+        const int first_hidden = it.len - a.n_tok + a.by_group.quot(row0) + 1;       // first key that the block's first token does not see
         for (int tile = tile0; tile < tile1 && alive; tile++) {
             cp_async_wait<S::Stages - 2>();
             alive = mbar_wait(full0 + stage * 8, phase, ctl, 1);       // the warp votes
@@ -449,7 +511,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
-                        const int limit = it.len - a.n_tok + (row0 + n * 8 + 2 * t + c) / a.group + 1 - tile * kKeys;
+                        const int limit = it.len - a.n_tok + a.by_group.quot(row0 + n * 8 + 2 * t + c) + 1 - tile * kKeys;
 #pragma unroll
                         for (int j = 0; j < 2; j++)
 #pragma unroll
@@ -568,15 +630,15 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
 
         // ---- the item's sums, or this warp's part of them
         const float up = s_down == 0.0f ? 0.0f : 1.0f / s_down;
-        const bool whole = tile0 == 0 && tile1 == it.tiles;
-        const bool last = x + (tile1 - tile0) >= w_end;
+        const bool whole = tile0 == 0 && tile1 == it.tiles && a.cluster <= 1;     // a cluster's result is its last step's
+        const bool last = x + tile1 - tile0 >= w_end;
         const int item = (it.b * a.hkv + it.h) * a.row_blocks + it.rb;
         float* record = last ? tail_record : head_record;
         if (!whole) {
             if (last) tail_item = item;
             else head_item = item;
-            if (item_start < c_begin) before = 1;     // only the CTA's first item can begin before it, only its last end after it
-            if (item_start + it.tiles > c_end) after = 1;
+            if (item_start < c_begin) before = 1;              // only the CTA's first item can begin before it, only its last end after it
+            if (item_start + it.tiles > c_end) after = item_start + it.tiles;
         }
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -590,8 +652,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
                 }
                 const int r = n * 8 + 2 * t + c;
                 const float inv = l[n][c] == 0.0f ? 0.0f : 1.0f / l[n][c];
-                const int tok = (row0 + r) / a.group, hh = (row0 + r) - tok * a.group;
-                const long long row = ((long long)it.b * a.n_tok + tok) * a.hq + (long long)it.h * a.group + hh;
+                const long long row = out_row(a, it.b, it.h, row0 + r);
 #pragma unroll
                 for (int i = 0; i < P; i++) {
                     const float z = zs[n][i / 2][c];
@@ -605,8 +666,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
                 if (whole && row0 + r < a.rows && g == 0 && a.lse != nullptr)
                     a.lse[row] = l[n][c] == 0.0f ? -INFINITY : kLn2 * (mc[n][c] + log2f(l[n][c]));
                 if (!whole && g == 0) {
-                    record[S::Rows * D + r] = m[n][c] == -INFINITY ? -INFINITY : mc[n][c];
-                    record[S::Rows * (D + 1) + r] = l[n][c];
+                    s_m[2 * warp + last][r] = m[n][c] == -INFINITY ? -INFINITY : mc[n][c];
+                    s_l[2 * warp + last][r] = l[n][c];
                 }
             }
         // ---- the next item
@@ -625,129 +686,159 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
         }
     }
 
-    // ---- the CTA's records, in the order of the line: head and tail of warp 0, of warp 1, ...
-    if (lane == 0) { s_head_item[warp] = head_item; s_tail_item[warp] = tail_item; s_before[warp] = before; s_after[warp] = after; }
+    // ---- the CTA's records
+    if (lane == 0) {
+        s_item[2 * warp] = head_item;
+        s_item[2 * warp + 1] = tail_item;
+        s_before[warp] = before;
+        s_after[warp] = after;
+    }
     __threadfence_block();
     __syncthreads();
-    int tail_of_cta = -1, head_of_cta = 0;
-    auto item_at = [&](int k) { return k & 1 ? s_tail_item[k >> 1] : s_head_item[k >> 1]; };
-    auto record_at = [&](int k) -> const float* {
-        return k & 1 ? reinterpret_cast<const float*>(smem + (k >> 1) * S::WarpBytes) : a.scratch + (size_t)(blockIdx.x * kWarps + (k >> 1)) * S::Record;
-    };
-    for (int k = 0; k < 2 * kWarps;) {
-        const int item = item_at(k);
+    for (int i = tid; i < kRecords * S::Rows; i += kWarps * 32) {          // each one's weight in its item
+        const int y = i / S::Rows, r = i % S::Rows, item = s_item[y];
+        if (item >= 0) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int z = 0; z < kRecords; z++)
+                if (s_item[z] == item) mx = fmaxf(mx, s_m[z][r]);
+            s_w[y][r] = record_weight(s_m[y][r], s_l[y][r], mx);
+        }
+    }
+    __syncthreads();
+    int2 carried = make_int2(-1, 0);
+    constexpr int kQuads = S::Rows * (D / 4), kEach = (kQuads + kWarps * 32 - 1) / (kWarps * 32);
+    float4 mine[kEach];                                        // cluster: the CTA's sums
+    float mine_m[kEach], mine_l[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; j++) { mine[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f); mine_m[j] = -INFINITY; mine_l[j] = 0.0f; }
+    for (int k = 0; k < kRecords;) {
+        const int item = s_item[k];
         if (item < 0) { k++; continue; }
         int end = k + 1;                                       // records of this item: k .. end - 1, with gaps
-        for (int i = k + 1; i < 2 * kWarps; i++) {
-            const int y = item_at(i);
+        for (int i = k + 1; i < kRecords; i++) {
+            const int y = s_item[i];
             if (y == item) end = i + 1;
             else if (y >= 0) break;
         }
-        const int rb = item % a.row_blocks, bh = item / a.row_blocks, b = bh / a.hkv, h = bh - b * a.hkv;
-        // it begins before this CTA's part if its first warp says so of its first record, and ends after it likewise
-        const bool starts_before = s_before[k >> 1] != 0 && item == (s_head_item[k >> 1] >= 0 ? s_head_item[k >> 1] : s_tail_item[k >> 1]);
-        const bool ends_after = s_after[(end - 1) >> 1] != 0 && item == (s_tail_item[(end - 1) >> 1] >= 0 ? s_tail_item[(end - 1) >> 1] : s_head_item[(end - 1) >> 1]);
+        // it begins before this CTA's part if its first warp says so and this is that warp's first record, and ends after it likewise
+        const int w0 = k >> 1, w1 = (end - 1) >> 1;
+        const bool starts_before = s_before[w0] != 0 && item == (s_item[2 * w0] >= 0 ? s_item[2 * w0] : s_item[2 * w0 + 1]);
+        const bool ends_after = s_after[w1] != 0 && item == (s_item[2 * w1 + 1] >= 0 ? s_item[2 * w1 + 1] : s_item[2 * w1]);
         float* slot = a.scratch + ((size_t)gridDim.x * kWarps + 2 * blockIdx.x + (starts_before ? 0 : 1)) * S::Record;
-        const bool final_here = !starts_before && !ends_after;
-        if (starts_before) head_of_cta = ends_after ? 2 : 1;
-        else if (ends_after) tail_of_cta = item;
-        for (int i = tid; i < S::Rows * (D / 4); i += kWarps * 32) {
+        const int bh = a.by_row_blocks.quot(item), rb = item - bh * a.row_blocks, b = a.by_hkv.quot(bh), h = bh - b * a.hkv;
+        if (ends_after && !starts_before && a.cluster == 0) carried = make_int2(item, (s_after[w1] - 1) / chunk + 1);
+#pragma unroll
+        for (int j = 0; j < kEach; j++) {
+            const int i = tid + j * kWarps * 32;
+            if (i >= kQuads) break;
             const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-            float mx = -INFINITY;
-            for (int y = k; y < end; y++)
-                if (item_at(y) == item) mx = fmaxf(mx, record_at(y)[S::Rows * D + r]);
-            float sum = 0.0f;
+            float mx = -INFINITY, sum = 0.0f;
             float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             for (int y = k; y < end; y++)
-                if (item_at(y) == item) {
-                    const float* rec = record_at(y);
-                    const float ym = rec[S::Rows * D + r];
-                    const float w = ym == -INFINITY ? (rec[S::Rows * (D + 1) + r] == 0.0f ? 0.0f : 1.0f) : ex2(ym - mx);
+                if (s_item[y] == item) {
+                    const float* rec = y & 1 ? reinterpret_cast<const float*>(smem + (y >> 1) * S::WarpBytes) : a.scratch + (size_t)(blockIdx.x * kWarps + (y >> 1)) * S::Record;
+                    const float w = s_w[y][r];
                     const float4 z = *reinterpret_cast<const float4*>(rec + r * D + d);
-                    sum = fmaf(w, rec[S::Rows * (D + 1) + r], sum);
+                    mx = fmaxf(mx, s_m[y][r]);
+                    sum = fmaf(w, s_l[y][r], sum);
                     f.x = fmaf(w, z.x, f.x); f.y = fmaf(w, z.y, f.y); f.z = fmaf(w, z.z, f.z); f.w = fmaf(w, z.w, f.w);
                 }
-            if (!final_here) {
+            if (a.cluster > 1) {
+                mine[j] = f; mine_m[j] = mx; mine_l[j] = sum;
+            } else if (starts_before || ends_after) {
                 *reinterpret_cast<float4*>(slot + r * D + d) = f;
                 if (d == 0) { slot[S::Rows * D + r] = mx; slot[S::Rows * (D + 1) + r] = sum; }
             } else if (rb * S::Rows + r < a.rows) {
-                const int tok = (rb * S::Rows + r) / a.group, hh = rb * S::Rows + r - tok * a.group;
-                const long long row = ((long long)b * a.n_tok + tok) * a.hq + (long long)h * a.group + hh;
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                uint2 y;
-                y.x = pack16<BF16>(f.x * inv, f.y * inv);
-                y.y = pack16<BF16>(f.z * inv, f.w * inv);
-                *reinterpret_cast<uint2*>(a.o + row * D + d) = y;
-                if (d == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? -INFINITY : kLn2 * (mx + log2f(sum));
+                store_quad<D, BF16>(a, out_row(a, b, h, rb * S::Rows + r), d, f, mx, sum);
             }
         }
         k = end;
     }
-    if (tid == 0) a.meta[blockIdx.x] = make_int2(tail_of_cta, head_of_cta);
+    if (a.cluster == 0) {
+        if (tid == 0) a.meta[blockIdx.x] = carried;
+    } else if (a.cluster > 1) {
+        // ---- the item's CTAs: each leaves its sums in its shared memory, the first ones read them all
+        __syncthreads();                                       // the records have been read
+        float* rec = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int j = 0; j < kEach; j++) {
+            const int i = tid + j * kWarps * 32;
+            if (i >= kQuads) break;
+            *reinterpret_cast<float4*>(rec + i * 4) = mine[j];
+            if (i % (D / 4) == 0) { rec[S::Rows * D + i / (D / 4)] = mine_m[j]; rec[S::Rows * (D + 1) + i / (D / 4)] = mine_l[j]; }
+        }
+        cluster_sync();
+        for (int i = rank * kWarps * 32 + tid; i < kQuads; i += a.cluster * kWarps * 32) {
+            const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+            if (it.rb * S::Rows + r >= a.rows) break;
+            float cm[kMaxCluster], cl[kMaxCluster], mx = -INFINITY, sum = 0.0f;
+            float4 cz[kMaxCluster], f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int c = 0; c < kMaxCluster; c++)
+                if (c < a.cluster) {
+                    cm[c] = ld_cluster(rec + S::Rows * D + r, c);
+                    cl[c] = ld_cluster(rec + S::Rows * (D + 1) + r, c);
+                    cz[c] = ld_cluster4(rec + i * 4, c);
+                    mx = fmaxf(mx, cm[c]);
+                }
+#pragma unroll
+            for (int c = 0; c < kMaxCluster; c++)
+                if (c < a.cluster) {
+                    const float w = record_weight(cm[c], cl[c], mx);
+                    sum = fmaf(w, cl[c], sum);
+                    f.x = fmaf(w, cz[c].x, f.x); f.y = fmaf(w, cz[c].y, f.y); f.z = fmaf(w, cz[c].z, f.z); f.w = fmaf(w, cz[c].w, f.w);
+                }
+            store_quad<D, BF16>(a, out_row(a, it.b, it.h, it.rb * S::Rows + r), d, f, mx, sum);
+        }
+        cluster_sync();                                        // nobody leaves while its shared memory may be read
+    }
 }
 
-// Items that lie in several CTAs: block (c, row) merges, for the item that CTA c is the first of, its tail record and the
-// head records of the CTAs after it, up to the one where the item ends.
+// Items that lie in several CTAs: a block takes 8 rows of the item that begins in CTA c and goes on, four warps a row, and
+// merges c's second record and the first records of the CTAs up to the item's last.
 template <int D, bool BF16, int NT>
-__global__ void __launch_bounds__(kWarps * 32) u4_merge_kernel(const __grid_constant__ U4Args a, int n_ctas) {
+__global__ void __launch_bounds__(1024) u4_merge_kernel(const __grid_constant__ U4Args a, int n_ctas) {
     using S = Shape<D, NT>;
-    __shared__ float part[kWarps][D], part_l[kWarps];
+    constexpr int kSubs = 4;                                   // warps of a row
+    __shared__ float4 part[kSubs][8][32];
+    __shared__ float part_l[kSubs][8];
     grid_dependency_wait();
     grid_launch_dependents();
-    const int c = blockIdx.x / S::Rows, r = blockIdx.x - c * S::Rows;
-    const int item = a.meta[c].x;
-    if (item < 0) return;
-    const int rb = item % a.row_blocks, bh = item / a.row_blocks, b = bh / a.hkv, h = bh - b * a.hkv;
-    if (rb * S::Rows + r >= a.rows) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // the CTAs of the item: those after c whose head record is part of it, up to the first that says it ends
-    int last = n_ctas;
-    for (int i0 = c + 1; i0 < n_ctas; i0 += 32) {
-        const int i = i0 + lane;
-        const bool ends = i < n_ctas && a.meta[i].y != 2;
-        const unsigned who = __ballot_sync(0xffffffffu, ends);
-        if (who) {
-            const int e = i0 + __ffs(who) - 1;
-            last = a.meta[e].y == 1 ? e + 1 : e;
-            break;
-        }
-    }
+    const int c = blockIdx.x / NT, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp >> 3, r = blockIdx.x % NT * 8 + (warp & 7);
+    const int2 carried = a.meta[c];
+    if (carried.x < 0) return;
+    const int item = carried.x, last = carried.y;
+    const int bh = a.by_row_blocks.quot(item), rb = item - bh * a.row_blocks, b = a.by_hkv.quot(bh), h = bh - b * a.hkv;
+    const bool live = rb * S::Rows + r < a.rows;
     const float* base = a.scratch + (size_t)n_ctas * kWarps * S::Record;
     auto record = [&](int i) { return base + (size_t)(2 * i + (i == c ? 1 : 0)) * S::Record; };
-    float mx = -INFINITY;
-    for (int i = c + lane; i < last; i += 32) mx = fmaxf(mx, record(i)[S::Rows * D + r]);
+    float mx = -INFINITY, sum = 0.0f;
+    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (live) {
+        for (int i = c + lane; i < last; i += 32) mx = fmaxf(mx, record(i)[S::Rows * D + r]);
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-    constexpr int E = D / 32;
-    float f[E], sum = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; e++) f[e] = 0.0f;
+        for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
 #pragma unroll 4
-    for (int i = c + warp; i < last; i += kWarps) {
-        const float* rec = record(i);
-        const float ym = rec[S::Rows * D + r], yl = rec[S::Rows * (D + 1) + r];
-        const float w = ym == -INFINITY ? (yl == 0.0f ? 0.0f : 1.0f) : ex2(ym - mx);
-        sum = fmaf(w, yl, sum);
-#pragma unroll
-        for (int e = 0; e < E; e++) f[e] = fmaf(w, rec[r * D + e * 32 + lane], f[e]);
+        for (int i = c + sub; i < last; i += kSubs) {
+            const float* rec = record(i);
+            const float yl = rec[S::Rows * (D + 1) + r], w = record_weight(rec[S::Rows * D + r], yl, mx);
+            const float4 z = lane < D / 4 ? *reinterpret_cast<const float4*>(rec + r * D + lane * 4) : f;
+            sum = fmaf(w, yl, sum);
+            f.x = fmaf(w, z.x, f.x); f.y = fmaf(w, z.y, f.y); f.z = fmaf(w, z.z, f.z); f.w = fmaf(w, z.w, f.w);
+        }
+        part[sub][warp & 7][lane] = f;
+        if (lane == 0) part_l[sub][warp & 7] = sum;
     }
-#pragma unroll
-    for (int e = 0; e < E; e++) part[warp][e * 32 + lane] = f[e];
-    if (lane == 0) part_l[warp] = sum;
     __syncthreads();
-    float total = 0.0f;
+    if (sub == 0 && live && lane < D / 4) {
 #pragma unroll
-    for (int w = 0; w < kWarps; w++) total += part_l[w];
-    const int tok = (rb * S::Rows + r) / a.group, hh = rb * S::Rows + r - tok * a.group;
-    const long long row = ((long long)b * a.n_tok + tok) * a.hq + (long long)h * a.group + hh;
-    for (int d = threadIdx.x; d < D; d += kWarps * 32) {
-        float y = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) y += part[w][d];
-        y = total == 0.0f ? 0.0f : y / total;
-        if constexpr (BF16) a.o[row * D + d] = __bfloat16_as_ushort(__float2bfloat16_rn(y));
-        else a.o[row * D + d] = __half_as_ushort(__float2half_rn(y));
-        if (d == 0 && a.lse != nullptr) a.lse[row] = total == 0.0f ? -INFINITY : kLn2 * (mx + log2f(total));
+        for (int y = 1; y < kSubs; y++) {
+            const float4 z = part[y][warp][lane];
+            f.x += z.x; f.y += z.y; f.z += z.z; f.w += z.w;
+            sum += part_l[y][warp];
+        }
+        store_quad<D, BF16>(a, out_row(a, b, h, rb * S::Rows + r), lane * 4, f, mx, sum);
     }
 }
 
@@ -755,7 +846,9 @@ __global__ void __launch_bounds__(kWarps * 32) u4_merge_kernel(const __grid_cons
 struct Plan {
     int nt;                 // 8-row columns of a block
     int row_blocks;
+    int cluster;            // CTAs of an item; 0: equal parts of the line of all tiles
     int ctas;
+    long long tiles;        // at most, of all items
     size_t record;          // bytes
     size_t bytes;           // of the workspace
 };
@@ -766,12 +859,22 @@ Plan make_plan(int batch, int hq, int hkv, int n_tok, int kv_len, int d_head, in
     const long long rows = (long long)n_tok * (hq / hkv);
     p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
     p.row_blocks = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
-    const long long tiles = (long long)batch * hkv * p.row_blocks * ((kv_len + kKeys - 1) / kKeys);
-    const long long most = (long long)sm_count * (p.nt == 1 ? 2 : 1);
-    const long long want = (tiles + kWarps - 1) / kWarps;
-    p.ctas = (int)(want < most ? want : most);
+    const long long items = (long long)batch * hkv * p.row_blocks, item_tiles = (kv_len + kKeys - 1) / kKeys;
+    p.tiles = items * item_tiles;
+    const long long slots = (long long)sm_count * (p.nt == 1 ? 2 : 1);
+    // A cluster an item, if all are on the GPU at once and its warps get few tiles each beyond an equal share: that many
+    // cost less than the second launch.
+    p.cluster = 0;
+    if (items <= slots) {
+        const long long most = slots / items < kMaxCluster ? slots / items : kMaxCluster;
+        const long long want = (item_tiles + kWarps - 1) / kWarps, cl = want < most ? want : most;
+        const long long each = (item_tiles + cl * kWarps - 1) / (cl * kWarps), share = (p.tiles + slots * kWarps - 1) / (slots * kWarps);
+        if (each <= share + kClusterTiles) p.cluster = (int)cl;
+    }
+    const long long want = (p.tiles + kWarps - 1) / kWarps;
+    p.ctas = p.cluster ? (int)(items * p.cluster) : (int)(want < slots ? want : slots);
     p.record = (size_t)8 * p.nt * (d_head + 2) * sizeof(float);
-    p.bytes = align256(p.record * p.ctas * (kWarps + 2)) + align256((size_t)p.ctas * sizeof(int2));
+    p.bytes = p.cluster ? 256 : align256(p.record * p.ctas * (kWarps + 2)) + align256((size_t)p.ctas * sizeof(int2));
     return p;
 }
 
@@ -784,9 +887,9 @@ int run_u4(const U4Args& a, int ctas, DeviceState* st, cudaStream_t stream) {
         FA_CUDA_TRY(cudaFuncSetAttribute(u4_kernel<D, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         configured[st->device] = true;
     }
-    int rc = launch_dependent(u4_kernel<D, BF16, NT>, ctas, kWarps * 32, smem, stream, 1, a);
-    if (rc != FA_OK || ctas == 1) return rc;
-    return launch_dependent(u4_merge_kernel<D, BF16, NT>, ctas * S::Rows, kWarps * 32, 0, stream, 1, a, ctas);
+    const int rc = launch_dependent(u4_kernel<D, BF16, NT>, ctas, kWarps * 32, smem, stream, a.cluster > 1 ? a.cluster : 1, a);
+    if (rc != FA_OK || a.cluster > 0 || ctas == 1) return rc;
+    return launch_dependent(u4_merge_kernel<D, BF16, NT>, ctas * NT, 1024, 0, stream, 1, a, ctas);
 }
 template <int D, bool BF16>
 int run_u4_rows(const U4Args& a, const Plan& p, DeviceState* st, cudaStream_t stream) {
@@ -829,6 +932,7 @@ FA_EXPORT int fa_decode_gqa_u4(const fa_decode_gqa_u4_args* p) {
     if (!st) return FA_ERR_CUDA;
     if (st->cc_major != 10) return FA_ERR_NOT_SM100;
     const Plan plan = make_plan(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->d_head, st->sm_count);
+    if (plan.tiles > 0x7FFF0000ll) return FA_ERR_INVALID_ARGUMENT;
     if (!p->workspace || p->workspace_bytes < plan.bytes || !aligned16(p->workspace)) return FA_ERR_WORKSPACE;
     const bool paged = p->layout.block_table != nullptr;
     const int block_rows = paged ? p->layout.page_size : p->seq_len_kv, blocks = paged ? p->layout.num_pages : p->batch_size;
@@ -852,10 +956,15 @@ FA_EXPORT int fa_decode_gqa_u4(const fa_decode_gqa_u4_args* p) {
     a.batch = p->batch_size;
     a.hq = p->num_q_heads;
     a.hkv = p->num_kv_heads;
-    a.group = p->num_q_heads / p->num_kv_heads;
     a.n_tok = n_tok;
+    a.group = p->num_q_heads / p->num_kv_heads;
     a.rows = n_tok * a.group;
     a.row_blocks = plan.row_blocks;
+    a.cluster = plan.cluster;
+    a.by_group = FastDiv(a.group);
+    a.by_row_blocks = FastDiv(plan.row_blocks);
+    a.by_hkv = FastDiv(p->num_kv_heads);
+    a.by_cluster = FastDiv(plan.cluster > 0 ? plan.cluster : 1);
     a.kv_len = p->seq_len_kv;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
