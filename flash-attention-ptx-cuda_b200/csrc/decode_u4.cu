@@ -23,6 +23,7 @@
 // only once, at the end, where the CTA merges what its warps have of the same item.  Items that lie in several CTAs go
 // through the workspace and a second small kernel.  Short jobs are done in one launch instead: a cluster of up to 8 CTAs an
 // item, which merges through distributed shared memory (plan.cluster says when).
+#include <atomic>
 #include <cmath>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -37,9 +38,11 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kMaxCluster = 8;                 // portable cluster size
-constexpr int kKeys = 32;                      // keys of a tile
+// Keys of a tile.  The longer one has a third fewer instructions a key besides the products and twice the independent ones
+// to fill a product's latency with; with more than one column of 8 rows there are enough of those, and no registers.
+constexpr int tile_keys(int nt) { return nt == 1 ? 64 : 32; }
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kClusterTiles = 8;               // see make_plan
+constexpr int kClusterTiles = 1;               // see make_plan
 constexpr float kGrow = 8.0f;                  // a running max may be exceeded by this much (in powers of two) before it is raised
 
 struct U4Args {
@@ -56,6 +59,7 @@ struct U4Args {
     const int* seq_lens;
     int batch, hq, hkv, group, n_tok, rows, row_blocks, kv_len;
     int cluster;                               // CTAs of an item's cluster; 0: the line
+    int box_shift;                             // rows of a TMA box: a tile's, or a page's
     FastDiv by_group, by_row_blocks, by_hkv, by_cluster;
     float scale_log2;
 };
@@ -70,38 +74,54 @@ __device__ __forceinline__ long long out_row(const U4Args& a, int b, int h, int 
 template <int D, int NT>
 struct Shape {
     static constexpr int G = D / kU4Group;                     // groups of a row
+    static constexpr int Keys = tile_keys(NT), J = Keys / 16;  // of a tile, and its 16-key steps
     static constexpr int RowBytes = D / 2;
     static constexpr int Stages = NT == 4 ? 4 : 3;
-    static constexpr int CodeBytes = kKeys * RowBytes;
-    static constexpr int ParamBytes = kKeys * G * 4;
-    static constexpr int StageBytes = 2 * CodeBytes + 2 * ParamBytes;
-    static constexpr int WarpBytes = Stages * StageBytes;
+    static constexpr int CodeBytes = Keys * RowBytes;
+    static constexpr int StageBytes = 2 * CodeBytes;
+    static constexpr int FactorBytes = Keys * G * 16;         // of a tile: for each key K's (scale, offset) and V's, unpacked
+    static constexpr int WarpBytes = Stages * StageBytes + FactorBytes;
     static constexpr int Rows = 8 * NT;
     static constexpr int Record = Rows * (D + 2);              // floats: O [row][D], then m [row], l [row]
     static_assert(Record * 4 <= WarpBytes, "a record fits the ring it replaces");
-    static constexpr int CtasPerSm = NT == 1 ? 2 : 1;
 };
 
+// Two at a time: d = a b - c, a += b.
+__device__ __forceinline__ void fma2(float (&d)[2], const float* a, const float (&b)[2], const float (&c)[2]) {
+    asm("{\n\t.reg .b64 x, y, z, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 r, x, y, z;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]), "f"(-c[0]), "f"(-c[1]));
+}
+__device__ __forceinline__ void add2(float (&a)[2], const float (&b)[2]) {
+    asm("{\n\t.reg .b64 x, y, r;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 r, x, y;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "+f"(a[0]), "+f"(a[1]) : "f"(b[0]), "f"(b[1]));
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// BYTES of `src`, or zeros.
-template <int BYTES>
-__device__ __forceinline__ void cp_async_or_zero(uint32_t dst, const void* src, bool valid) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(valid ? BYTES : 0) : "memory");
+// Four floats (G = 2) or two.
+template <int G>
+__device__ __forceinline__ void lds_factors(uint32_t a, float (&f)[2 * G]) {
+    if constexpr (G == 2) asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[0]), "=f"(f[1]), "=f"(f[2 * G - 2]), "=f"(f[2 * G - 1]) : "r"(a));
+    else asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(f[0]), "=f"(f[1]) : "r"(a));
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+template <int G>
+__device__ __forceinline__ void sts_factors(uint32_t a, const float (&f)[2 * G]) {
+    if constexpr (G == 2) asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(f[0]), "f"(f[1]), "f"(f[2 * G - 2]), "f"(f[2 * G - 1]) : "memory");
+    else asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(f[0]), "f"(f[1]) : "memory");
 }
 // The pairs of a key.
 template <int G>
-__device__ __forceinline__ void lds_pairs(uint32_t a, uint32_t (&p)[G]) {
-    if constexpr (G == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(p[0]), "=r"(p[G - 1]) : "r"(a));
-    else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(p[0]) : "r"(a));
+__device__ __forceinline__ void ldg_pairs(const __half2* p, uint32_t (&u)[G]) {
+    if constexpr (G == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        u[0] = x.x;
+        u[G - 1] = x.y;
+    } else {
+        u[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
 }
 // Four 8 x 8 tiles of 16-bit values, whose rows the lanes' addresses name (8 lanes a tile); TRANS: by columns.
 template <bool TRANS>
@@ -188,10 +208,11 @@ __device__ __forceinline__ void store_quad(const U4Args& a, long long row, int d
 struct Item {
     int b, h, rb, len, tiles;      // sequence, KV head, row block, its keys, tiles of 32 of them (at least one)
 };
-__device__ __forceinline__ int tiles_of(int len) { return max(1, (len + kKeys - 1) / kKeys); }
+template <int KEYS>
+__device__ __forceinline__ int tiles_of(int len) { return max(1, (len + KEYS - 1) / KEYS); }
 
 template <int D, bool BF16, int NT>
-__global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kernel(const __grid_constant__ U4Args a) {
+__global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constant__ U4Args a) {
     using S = Shape<D, NT>;
     constexpr int G = S::G;
     extern __shared__ uint8_t smem_raw[];
@@ -226,18 +247,18 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
         it.b = a.by_hkv.quot(bh);
         it.h = bh - it.b * a.hkv;
         it.len = sequence_length(a.seq_lens, it.b, a.kv_len);
-        it.tiles = tiles_of(it.len);
+        it.tiles = tiles_of<S::Keys>(it.len);
         c_begin = a.by_cluster.quot(it.tiles * rank);
         c_end = a.by_cluster.quot(it.tiles * (rank + 1));
         __syncthreads();                                       // the barriers are ready
     } else {
         const int per_thread = (a.batch + kWarps * 32 - 1) / (kWarps * 32);   // sequences of a thread
-        int total = a.batch * tiles_of(a.kv_len);
+        int total = a.batch * tiles_of<S::Keys>(a.kv_len);
         if (a.seq_lens != nullptr) {
             int sum = 0;
             for (int i = 0; i < per_thread; i++) {
                 const int b = tid * per_thread + i;
-                if (b < a.batch) sum += tiles_of(sequence_length(a.seq_lens, b, a.kv_len));
+                if (b < a.batch) sum += tiles_of<S::Keys>(sequence_length(a.seq_lens, b, a.kv_len));
             }
             int inc = sum;
 #pragma unroll
@@ -271,7 +292,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
     if (a.cluster == 0 && w_begin < w_end) {
         int b_start;                                           // first tile of sequence it.b
         if (a.seq_lens == nullptr) {
-            it.tiles = tiles_of(a.kv_len);
+            it.tiles = tiles_of<S::Keys>(a.kv_len);
             it.len = a.kv_len;
             it.b = w_begin / (it.tiles * per_b);
             b_start = it.b * it.tiles * per_b;
@@ -287,7 +308,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
             b_start = s_prefix[lo] * per_b;
             for (;;) {
                 it.len = sequence_length(a.seq_lens, it.b, a.kv_len);
-                it.tiles = tiles_of(it.len);
+                it.tiles = tiles_of<S::Keys>(it.len);
                 const int end = b_start + it.tiles * per_b;
                 if (w_begin < end || it.b + 1 >= a.batch) break;
                 b_start = end;
@@ -305,11 +326,12 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
     float* head_record = a.scratch + (size_t)(blockIdx.x * kWarps + warp) * S::Record;
     int head_item = -1, tail_item = -1, before = 0, after = 0;
 
-    // ---- the warp's ring: a barrier a stage, which TMA's copies of the codes complete; scale and offset pairs, 4 or 8 bytes
-    // of any row stride, come by cp.async
+    // ---- the warp's ring: a barrier a stage, which TMA's copies of the codes complete.  The scales and offsets of a key, 4 or 8 bytes
+    // of any row stride, come by ordinary loads a tile ahead, a lane a key; it unpacks them once for the four that need them.
     constexpr int P = D / 32;                                  // pieces of a row as the products see them: 32 elements, 16 bytes
     const uint32_t full0 = smem_u32(&s_full[warp][0]);
-    const bool two_boxes = a.map.page_shift == 4;              // pages of 16 rows: half a tile each
+    const int box_shift = a.box_shift, boxes = S::Keys >> box_shift;        // rows of a TMA box; boxes of a tile
+    const uint32_t factors = ring + S::Stages * S::StageBytes;
     const int in_page = a.map.page_shift < 0 ? 0x7FFFFFFF : (1 << a.map.page_shift) - 1;
     int stage = 0, load_stage = 0, in_flight = 0;
     uint32_t phase = 0;
@@ -333,39 +355,60 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
             const int p = a.map.block_table[(long long)it.b * a.map.table_stride + (key >> a.map.page_shift)];
             return (unsigned)p < (unsigned)a.map.n_pages ? p : -1;
         };
-        auto load_tile = [&](int tile, int p0, int p1) {
-            const int k0 = tile * kKeys;
+        // pages of a tile's boxes, one a lane
+        auto pages_of = [&](int tile) { return lane < boxes ? page_of(tile * S::Keys + (lane << box_shift)) : -1; };
+        auto load_codes = [&](int tile, int pages) {
+            const int k0 = tile * S::Keys;
             const uint32_t dst = ring + load_stage * S::StageBytes, bar = full0 + load_stage * 8;
             load_stage = load_stage + 1 == S::Stages ? 0 : load_stage + 1;
             in_flight++;
-            if (elect_one()) {
-                // rows past the block and pages that name none read as zero; rows past the sequence's end hold any codes, and are masked
-                mbar_arrive_expect_tx(bar, 2 * S::CodeBytes);
-                tma_load_4d(dst, &a.tk, bar, 0, k0 & in_page, it.h, p0);
-                tma_load_4d(dst + S::CodeBytes, &a.tv, bar, 0, k0 & in_page, it.h, p0);
-                if (two_boxes) {
-                    tma_load_4d(dst + S::CodeBytes / 2, &a.tk, bar, 0, 0, it.h, p1);
-                    tma_load_4d(dst + S::CodeBytes + S::CodeBytes / 2, &a.tv, bar, 0, 0, it.h, p1);
+            if (boxes == 1) {
+                const int p = __shfl_sync(0xffffffffu, pages, 0);
+                if (elect_one()) {
+                    // rows past the block and pages that name none read as zero; rows past the sequence's end hold any codes, and are masked
+                    mbar_arrive_expect_tx(bar, 2 * S::CodeBytes);
+                    tma_load_4d(dst, &a.tk, bar, 0, k0 & in_page, it.h, p);
+                    tma_load_4d(dst + S::CodeBytes, &a.tv, bar, 0, k0 & in_page, it.h, p);
+                }
+            } else {
+                if (elect_one()) mbar_arrive_expect_tx(bar, 2 * S::CodeBytes);
+                __syncwarp();
+                if (lane < boxes) {
+                    const uint32_t at = dst + (lane << box_shift) * S::RowBytes;
+                    const int row = (k0 + (lane << box_shift)) & in_page;
+                    tma_load_4d(at, &a.tk, bar, 0, row, it.h, pages);
+                    tma_load_4d(at + S::CodeBytes, &a.tv, bar, 0, row, it.h, pages);
+                }
+                __syncwarp();
+            }
+        };
+        constexpr int KPL = (S::Keys + 31) / 32;                 // keys of a lane
+        uint32_t kraw[KPL][G], vraw[KPL][G];
+        auto load_pairs = [&](int tile, int pages) {
+#pragma unroll
+            for (int i = 0; i < KPL; i++) {
+                const int key = tile * S::Keys + i * 32 + lane, p = __shfl_sync(0xffffffffu, pages, (i * 32 + lane) >> box_shift);
+#pragma unroll
+                for (int gi = 0; gi < G; gi++) kraw[i][gi] = vraw[i][gi] = 0;
+                if (key < it.len && p >= 0 && (S::Keys >= 32 || lane < S::Keys)) {
+                    const long long off = p * a.p_block_stride + hp_off + (long long)(key & in_page) * a.p_row_stride;
+                    ldg_pairs<G>(a.kp + off, kraw[i]);
+                    ldg_pairs<G>(a.vp + off, vraw[i]);
                 }
             }
-            const uint32_t pdst = dst + 2 * S::CodeBytes + lane * 4 * G;
-            const int key = k0 + lane, p = lane < 16 ? p0 : p1;
-            const bool ok = key < it.len && p >= 0;
-            const long long off = ok ? p * a.p_block_stride + hp_off + (long long)(key & in_page) * a.p_row_stride : 0;
-            cp_async_or_zero<4 * G>(pdst, a.kp + off, ok);
-            cp_async_or_zero<4 * G>(pdst + S::ParamBytes, a.vp + off, ok);
         };
 
-        int next_p0 = page_of(tile0 * kKeys), next_p1 = page_of(tile0 * kKeys + 16);
+        int pages = pages_of(tile0), next_pages = -1;          // of the tile whose pairs are loaded next, and of the one whose codes are
+        load_pairs(tile0, pages);
 #pragma unroll
         for (int i = 0; i < S::Stages - 1; i++) {
             if (tile0 + i < tile1) {
-                const int p0 = next_p0, p1 = next_p1;
-                if (tile0 + i + 1 < tile1) { next_p0 = page_of((tile0 + i + 1) * kKeys); next_p1 = page_of((tile0 + i + 1) * kKeys + 16); }
-                load_tile(tile0 + i, p0, p1);
+                next_pages = i == 0 ? pages : pages_of(tile0 + i);
+                load_codes(tile0 + i, next_pages);
             }
-            cp_async_commit();
         }
+        int ahead = S::Stages - 1 == 2 ? next_pages : tile0 + 1 < tile1 ? pages_of(tile0 + 1) : -1;
+        next_pages = tile0 + S::Stages - 1 < tile1 ? pages_of(tile0 + S::Stages - 1) : -1;
         // q as operand B: column g of the n-th 8 rows; 8 elements of a 16-byte piece of codes are two steps of k, in pairs
         // (i, i + 4) as the codes lie in a word.  bf16 rows are brought to fp16 by a power of two that puts their
         // largest element at 2^14: exact for elements down to 2^-28 of that one, and the rest is below its 32-bit rounding.
@@ -446,24 +489,62 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
 
         const int first_hidden = it.len - a.n_tok + a.by_group.quot(row0) + 1;       // first key that the block's first token does not see
         for (int tile = tile0; tile < tile1 && alive; tile++) {
-            cp_async_wait<S::Stages - 2>();
+            // this tile's factors: K's scale and offset of code 8 over -72, as it meets q_init; V's offset of code 8, and its scale
+            // over 2^E, E such that the largest becomes 16 .. 32 when it is set: with P up to 2^8 and scales up to 2^7 times
+            // 2^E a bracket stays below 2^15
+            float s_max = 0.0f;
+#pragma unroll
+            for (int i = 0; i < KPL; i++)
+#pragma unroll
+                for (int gi = 0; gi < G; gi++) s_max = fmaxf(s_max, unpack16<false>(vraw[i][gi]).x);
+            if (__any_sync(0xffffffffu, s_max > s_limit)) {
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) s_max = fmaxf(s_max, __shfl_xor_sync(0xffffffffu, s_max, off));
+                const float down = __uint_as_float(((254u + 4u) << 23) - (__float_as_uint(s_max) & 0x7F800000u));
+                const float ratio = s_down == 0.0f ? 1.0f : down / s_down;
+                s_down = down;
+                s_limit = 128.0f / down;
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int i = 0; i < 2 * P; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[n][i / 2][i % 2][e] *= ratio;
+            }
+            // (the last tile's factors have been read: its products are issued, and below it the warp met)
+#pragma unroll
+            for (int i = 0; i < KPL; i++) {
+                float fk[2 * G], fv[2 * G];
+#pragma unroll
+                for (int gi = 0; gi < G; gi++) {
+                    const float2 k = unpack16<false>(kraw[i][gi]), v = unpack16<false>(vraw[i][gi]);
+                    fk[gi] = k.x;
+                    fk[G + gi] = fmaf(8.0f, k.x, k.y) * (-1.0f / 72.0f);
+                    fv[gi] = v.x * s_down;
+                    fv[G + gi] = fmaf(8.0f, v.x, v.y);
+                }
+                if (S::Keys >= 32 || lane < S::Keys) {
+                    sts_factors<G>(factors + (i * 32 + lane) * 8 * G, fk);
+                    sts_factors<G>(factors + S::Keys * 8 * G + (i * 32 + lane) * 8 * G, fv);
+                }
+            }
             alive = mbar_wait(full0 + stage * 8, phase, ctl, 1);       // the warp votes
             if (!alive) break;
             in_flight--;
-            __syncwarp();                                      // every lane's copies have landed, and nobody reads the oldest stage any more
-            if (tile + S::Stages - 1 < tile1) {
-                const int p0 = next_p0, p1 = next_p1;
-                if (tile + S::Stages < tile1) { next_p0 = page_of((tile + S::Stages) * kKeys); next_p1 = page_of((tile + S::Stages) * kKeys + 16); }
-                load_tile(tile + S::Stages - 1, p0, p1);
+            __syncwarp();                                      // the factors are written, and nobody reads the oldest stage any more
+            if (tile + S::Stages - 1 < tile1) load_codes(tile + S::Stages - 1, next_pages);
+            if (tile + 1 < tile1) {
+                load_pairs(tile + 1, ahead);
+                ahead = S::Stages - 1 == 2 ? next_pages : tile + 2 < tile1 ? pages_of(tile + 2) : -1;
+                next_pages = tile + S::Stages < tile1 ? pages_of(tile + S::Stages) : -1;
             }
-            cp_async_commit();
-            const uint32_t at = stage * S::StageBytes, kpb = ring + at + 2 * S::CodeBytes + g * 4 * G, vpb = kpb + S::ParamBytes;
+            const uint32_t at = stage * S::StageBytes;
             if (++stage == S::Stages) { stage = 0; phase ^= 1; }
 
             // S^T: keys j * 16 + g and + 8, columns 2t and 2t + 1 of each 8 rows
-            float s[2][NT][4];
+            float s[S::J][NT][4];
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
+            for (int j = 0; j < S::J; j++) {
                 float acc[G][NT][4];
 #pragma unroll
                 for (int gi = 0; gi < G; gi++) {
@@ -484,78 +565,47 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
                 }
 #pragma unroll
                 for (int e2 = 0; e2 < 2; e2++) {
-                    uint32_t pr[G];
-                    lds_pairs<G>(kpb + (j * 16 + e2 * 8) * 4 * G, pr);
-                    float ks[G], kz[G];                        // scale; offset of code 8 over -72, as it meets q_init
-#pragma unroll
-                    for (int gi = 0; gi < G; gi++) {
-                        const float2 f = unpack16<false>(pr[gi]);
-                        ks[gi] = f.x;
-                        kz[gi] = fmaf(8.0f, f.x, f.y) * (-1.0f / 72.0f);
-                    }
+                    float fk[2 * G];
+                    lds_factors<G>(factors + (j * 16 + e2 * 8 + g) * 8 * G, fk);
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
                         for (int c = 0; c < 2; c++) {
-                            float v = kz[0] * q_init[n][0][c];
-                            if constexpr (G == 2) v = fmaf(kz[G - 1], q_init[n][G - 1][c], v);
-                            v = fmaf(ks[0], acc[0][n][e2 * 2 + c], v);
-                            if constexpr (G == 2) v = fmaf(ks[G - 1], acc[G - 1][n][e2 * 2 + c], v);
+                            float v = fk[G] * q_init[n][0][c];
+                            if constexpr (G == 2) v = fmaf(fk[2 * G - 1], q_init[n][G - 1][c], v);
+                            v = fmaf(fk[0], acc[0][n][e2 * 2 + c], v);
+                            if constexpr (G == 2) v = fmaf(fk[G - 1], acc[G - 1][n][e2 * 2 + c], v);
                             s[j][n][e2 * 2 + c] = v;
                         }
                 }
             }
             // masked keys: past what the row's token sees (only the last tiles have any)
-            if ((tile + 1) * kKeys > first_hidden) {
+            if ((tile + 1) * S::Keys > first_hidden) {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
-                        const int limit = it.len - a.n_tok + a.by_group.quot(row0 + n * 8 + 2 * t + c) + 1 - tile * kKeys;
+                        const int limit = it.len - a.n_tok + a.by_group.quot(row0 + n * 8 + 2 * t + c) + 1 - tile * S::Keys;
 #pragma unroll
-                        for (int j = 0; j < 2; j++)
+                        for (int j = 0; j < S::J; j++)
 #pragma unroll
                             for (int e2 = 0; e2 < 2; e2++)
-                                if (j * 16 + e2 * 8 + g >= limit || tile * kKeys + j * 16 + e2 * 8 + g >= it.len) s[j][n][e2 * 2 + c] = -INFINITY;
+                                if (j * 16 + e2 * 8 + g >= limit || tile * S::Keys + j * 16 + e2 * 8 + g >= it.len) s[j][n][e2 * 2 + c] = -INFINITY;
                     }
             }
-            // V's scales and offsets of this thread's keys
-            float vs[2][2][G], vz[2][2][G], s_max = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int e2 = 0; e2 < 2; e2++) {
-                    uint32_t pr[G];
-                    lds_pairs<G>(vpb + (j * 16 + e2 * 8) * 4 * G, pr);
-#pragma unroll
-                    for (int gi = 0; gi < G; gi++) {
-                        const float2 f = unpack16<false>(pr[gi]);
-                        vs[j][e2][gi] = f.x;
-                        vz[j][e2][gi] = fmaf(8.0f, f.x, f.y);
-                        s_max = fmaxf(s_max, f.x);
-                    }
-                }
-            // the running max may be exceeded by 2^8, the scales' reference by 2^3, before the sums are brought to new ones
+            // the running max may be exceeded by 2^8 before the sums are brought to a new one
             float t_max[NT][2];
-            bool raise = s_max > s_limit;
+            bool raise = false;
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    t_max[n][c] = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
+                    t_max[n][c] = fmaxf(s[0][n][c], s[0][n][2 + c]);
+#pragma unroll
+                    for (int j = 1; j < S::J; j++) t_max[n][c] = fmaxf(t_max[n][c], fmaxf(s[j][n][c], s[j][n][2 + c]));
                     raise |= (t_max[n][c] - m[n][c]) * sc[n][c] > kGrow;       // no max yet: inf, unless every key is masked
                 }
             if (__any_sync(0xffffffffu, raise)) {
-                float ratio = 1.0f;
-#pragma unroll
-                for (int off = 16; off > 0; off >>= 1) s_max = fmaxf(s_max, __shfl_xor_sync(0xffffffffu, s_max, off));
-                if (s_max > s_limit) {
-                    // 2^-E such that the largest scale becomes 16 .. 32: with P up to 2^8 and scales up to 2^7 a bracket stays below 2^15
-                    const float down = __uint_as_float(((254u + 4u) << 23) - (__float_as_uint(s_max) & 0x7F800000u));
-                    ratio = s_down == 0.0f ? 1.0f : down / s_down;
-                    s_down = down;
-                    s_limit = 128.0f / down;
-                }
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -571,34 +621,35 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
 #pragma unroll
                         for (int gi = 0; gi < G; gi++) zs[n][gi][c] *= alpha;
 #pragma unroll
-                        for (int i = 0; i < 2 * P; i++) { o[n][i / 2][i % 2][c] *= alpha * ratio; o[n][i / 2][i % 2][2 + c] *= alpha * ratio; }
+                        for (int i = 0; i < 2 * P; i++) { o[n][i / 2][i % 2][c] *= alpha; o[n][i / 2][i % 2][2 + c] *= alpha; }
                     }
             }
             // P, its sums, and the brackets as operand B: columns to rows across the warp
-            uint32_t pf[2][NT][G][2];
+            uint32_t pf[S::J][NT][G][2];
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < S::J; j++)
 #pragma unroll
                 for (int e2 = 0; e2 < 2; e2++) {
-                    float sd[G];
-#pragma unroll
-                    for (int gi = 0; gi < G; gi++) sd[gi] = vs[j][e2][gi] * s_down;
+                    float fv[2 * G];
+                    lds_factors<G>(factors + S::Keys * 8 * G + (j * 16 + e2 * 8 + g) * 8 * G, fv);
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
-                        const float p0 = ex2(fmaf(s[j][n][e2 * 2], sc[n][0], -mc[n][0])), p1 = ex2(fmaf(s[j][n][e2 * 2 + 1], sc[n][1], -mc[n][1]));
-                        l[n][0] += p0;
-                        l[n][1] += p1;
+                        float x[2], p[2];
+                        fma2(x, s[j][n] + e2 * 2, sc[n], mc[n]);
+                        p[0] = ex2(x[0]);
+                        p[1] = ex2(x[1]);
+                        add2(l[n], p);
 #pragma unroll
                         for (int gi = 0; gi < G; gi++) {
-                            zs[n][gi][0] = fmaf(p0, vz[j][e2][gi], zs[n][gi][0]);
-                            zs[n][gi][1] = fmaf(p1, vz[j][e2][gi], zs[n][gi][1]);
-                            pf[j][n][gi][e2] = transpose8x8(pack16<false>(p0 * sd[gi], p1 * sd[gi]));
+                            zs[n][gi][0] = fmaf(p[0], fv[G + gi], zs[n][gi][0]);
+                            zs[n][gi][1] = fmaf(p[1], fv[G + gi], zs[n][gi][1]);
+                            pf[j][n][gi][e2] = transpose8x8(pack16<false>(p[0] * fv[gi], p[1] * fv[gi]));
                         }
                     }
                 }
             // O^T: elements 4g .. 4g + 3 of each piece, two of them per product of 16 rows
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < S::J; j++)
 #pragma unroll
                 for (int gi = 0; gi < G; gi++) {
                     uint32_t y[4];                             // keys 2t, 2t + 1 and 2t + 8, 2t + 9 of piece 2 gi, then of piece 2 gi + 1
@@ -616,7 +667,6 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
                     }
                 }
         }
-        cp_async_wait<0>();
         if (!alive) {
             // a copy did not arrive: the status word says so.  Give those under way as long again, so that none lands in the
             // shared memory of another CTA, and leave the results as they are.
@@ -680,7 +730,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::CtasPerSm) u4_kerne
                     it.h = 0;
                     it.b++;
                     it.len = sequence_length(a.seq_lens, it.b, a.kv_len);
-                    it.tiles = tiles_of(it.len);
+                    it.tiles = tiles_of<S::Keys>(it.len);
                 }
             }
         }
@@ -854,27 +904,60 @@ struct Plan {
 };
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-Plan make_plan(int batch, int hq, int hkv, int n_tok, int kv_len, int d_head, int sm_count) {
+// Clusters of `size` CTAs that the current device holds at once (every instance has one CTA an SM); the GPCs have unequal
+// numbers of SMs, so that these are fewer than sm_count / size.
+int clusters_at_once(DeviceState* st, int size) {
+    if (size == 1) return st ? st->sm_count : 148;
+    if (!st) return 100 / size;
+    static std::atomic<int> known[64][kMaxCluster + 1];
+    std::atomic<int>& k = known[st->device][size];
+    int n = k.load(std::memory_order_relaxed);
+    if (n > 0) return n;
+    constexpr int smem = kWarps * Shape<128, 1>::WarpBytes + 1024;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = size;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(u4_kernel<128, false, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, u4_kernel<128, false, 1>, &cfg) != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        n = 1;
+    }
+    k.store(n, std::memory_order_relaxed);
+    return n;
+}
+
+Plan make_plan(int batch, int hq, int hkv, int n_tok, int kv_len, bool own_lengths, int d_head, DeviceState* st) {
     Plan p;
     const long long rows = (long long)n_tok * (hq / hkv);
     p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
     p.row_blocks = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
-    const long long items = (long long)batch * hkv * p.row_blocks, item_tiles = (kv_len + kKeys - 1) / kKeys;
+    const long long items = (long long)batch * hkv * p.row_blocks, item_tiles = (kv_len + tile_keys(p.nt) - 1) / tile_keys(p.nt);
     p.tiles = items * item_tiles;
-    const long long slots = (long long)sm_count * (p.nt == 1 ? 2 : 1);
-    // A cluster an item, if all are on the GPU at once and its warps get few tiles each beyond an equal share: that many
-    // cost less than the second launch.
+    const long long slots = st ? st->sm_count : 148;
+    // A cluster an item, the largest of which all are on the GPU at once, if its warps get at most one tile beyond an equal share
+    // (us in a graph, line / clusters, D = 128, Hkv = 8: B=16 Skv=1024 13.7 / 10.8, B=16 Skv=4096, a tile more, 26.1 / 22.7; B=1
+    // Skv=8192, a tile more, 12.1 / 12.1; B=1 Skv=16384, two more, 14.5 / 15.9; B=16 Skv=16384, four more, 69 / 72).  Sequences of
+    // their own lengths are taken to be half as long as they may be on average, which the line deals evenly.
     p.cluster = 0;
     if (items <= slots) {
-        const long long most = slots / items < kMaxCluster ? slots / items : kMaxCluster;
-        const long long want = (item_tiles + kWarps - 1) / kWarps, cl = want < most ? want : most;
-        const long long each = (item_tiles + cl * kWarps - 1) / (cl * kWarps), share = (p.tiles + slots * kWarps - 1) / (slots * kWarps);
-        if (each <= share + kClusterTiles) p.cluster = (int)cl;
+        const long long want = (item_tiles + kWarps - 1) / kWarps;
+        int cl = (int)(want < kMaxCluster ? want : kMaxCluster);
+        while (cl > 1 && clusters_at_once(st, cl) < items) cl--;
+        const long long each = (item_tiles + cl * kWarps - 1) / (cl * kWarps), share = (p.tiles / (own_lengths ? 2 : 1) + slots * kWarps - 1) / (slots * kWarps);
+        if (each <= share + kClusterTiles) p.cluster = cl;
     }
     const long long want = (p.tiles + kWarps - 1) / kWarps;
-    p.ctas = p.cluster ? (int)(items * p.cluster) : (int)(want < slots ? want : slots);
+    p.ctas = (int)(want < slots ? want : slots);
     p.record = (size_t)8 * p.nt * (d_head + 2) * sizeof(float);
-    p.bytes = p.cluster ? 256 : align256(p.record * p.ctas * (kWarps + 2)) + align256((size_t)p.ctas * sizeof(int2));
+    p.bytes = align256(p.record * p.ctas * (kWarps + 2)) + align256((size_t)p.ctas * sizeof(int2));      // clusters need none
+    if (p.cluster) p.ctas = (int)(items * p.cluster);
     return p;
 }
 
@@ -909,7 +992,7 @@ FA_EXPORT size_t fa_decode_gqa_u4_workspace_bytes(int batch_size, int num_q_head
         return 0;
     if (d_head != 64 && d_head != 128) return 0;
     DeviceState* st = device_state();
-    return make_plan(batch_size, num_q_heads, num_kv_heads, num_q_tokens > 0 ? num_q_tokens : 1, seq_len_kv, d_head, st ? st->sm_count : 148).bytes;
+    return make_plan(batch_size, num_q_heads, num_kv_heads, num_q_tokens > 0 ? num_q_tokens : 1, seq_len_kv, false, d_head, st).bytes;
 }
 
 FA_EXPORT int fa_decode_gqa_u4(const fa_decode_gqa_u4_args* p) {
@@ -931,14 +1014,16 @@ FA_EXPORT int fa_decode_gqa_u4(const fa_decode_gqa_u4_args* p) {
     DeviceState* st = device_state();
     if (!st) return FA_ERR_CUDA;
     if (st->cc_major != 10) return FA_ERR_NOT_SM100;
-    const Plan plan = make_plan(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->d_head, st->sm_count);
+    const Plan plan = make_plan(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->layout.seq_lens != nullptr, p->d_head, st);
     if (plan.tiles > 0x7FFF0000ll) return FA_ERR_INVALID_ARGUMENT;
     if (!p->workspace || p->workspace_bytes < plan.bytes || !aligned16(p->workspace)) return FA_ERR_WORKSPACE;
     const bool paged = p->layout.block_table != nullptr;
+    const int keys = tile_keys(plan.nt), box_rows = paged && p->layout.page_size < keys ? p->layout.page_size : keys;
+    for (a.box_shift = 0; (1 << a.box_shift) < box_rows;) a.box_shift++;
     const int block_rows = paged ? p->layout.page_size : p->seq_len_kv, blocks = paged ? p->layout.num_pages : p->batch_size;
     for (int i = 0; i < 2; i++) {
         rc = make_tensor_map_u4(i ? &a.tv : &a.tk, i ? p->v_cache : p->k_cache, p->d_head / 2, block_rows, p->num_kv_heads, blocks,
-                                p->layout.row_stride, p->layout.head_stride, p->layout.block_stride, paged && block_rows < kKeys ? block_rows : kKeys);
+                                p->layout.row_stride, p->layout.head_stride, p->layout.block_stride, box_rows);
         if (rc != FA_OK) return rc;
     }
     a.status = st->status;
@@ -948,7 +1033,7 @@ FA_EXPORT int fa_decode_gqa_u4(const fa_decode_gqa_u4_args* p) {
     a.o = static_cast<uint16_t*>(p->o);
     a.lse = p->lse;
     a.scratch = static_cast<float*>(p->workspace);
-    a.meta = reinterpret_cast<int2*>(static_cast<uint8_t*>(p->workspace) + align256(plan.record * plan.ctas * (kWarps + 2)));
+    a.meta = reinterpret_cast<int2*>(static_cast<uint8_t*>(p->workspace) + align256(plan.record * plan.ctas * (kWarps + 2)));     // the line's
     a.p_block_stride = p->layout.param_block_stride;
     a.p_head_stride = p->layout.param_head_stride;
     a.p_row_stride = p->layout.param_row_stride;
