@@ -325,6 +325,8 @@ struct ReadArgs {
     const uint8_t *k, *v;
     const __half2 *kp, *vp;
     uint16_t *k_out, *v_out;
+    long long o_batch, o_row, o_head;                         // elements between the outputs' sequences, rows and heads
+    bool live_only;                                           // rows that a sequence does not have stay as they are, instead of zero
     int hkv, seq_len_kv, n_rows, tiles;
     CacheMap map;
     long long block_stride, head_stride, row_stride;          // bytes
@@ -358,13 +360,15 @@ __global__ void __launch_bounds__(kThreads) read_u4_kernel(const __grid_constant
     const int first = a.first_rows == nullptr ? 0 : a.first_rows[b];
     uint32_t kc[kUnroll], vc[kUnroll];
     __half2 kp[kUnroll], vp[kUnroll];
+    bool live[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) {
         const int n = (tile * kUnroll + u) * SLOTS + slot;
         const long long row = (long long)first + n;
         kc[u] = vc[u] = 0;
         kp[u] = vp[u] = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-        if (n < a.n_rows && row >= 0 && row < len) {
+        live[u] = row >= 0 && row < len;
+        if (n < a.n_rows && live[u]) {
             const CacheRow at = cache_row(a.map, b, (int)row);
             if (at.block >= 0) {
                 const long long o = at.block * a.block_stride + h * a.head_stride + at.in_block * a.row_stride + lane * 4;
@@ -379,8 +383,8 @@ __global__ void __launch_bounds__(kThreads) read_u4_kernel(const __grid_constant
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) {
         const int n = (tile * kUnroll + u) * SLOTS + slot;
-        if (n < a.n_rows) {
-            const long long o = (((long long)b * a.n_rows + n) * a.hkv + h) * D + lane * 8;
+        if (n < a.n_rows && (live[u] || !a.live_only)) {
+            const long long o = b * a.o_batch + n * a.o_row + h * a.o_head + lane * 8;
             *reinterpret_cast<uint4*>(a.k_out + o) = from_u4<BF16>(kc[u], kp[u]);
             *reinterpret_cast<uint4*>(a.v_out + o) = from_u4<BF16>(vc[u], vp[u]);
         }
@@ -619,42 +623,56 @@ FA_EXPORT int fa_cache_append(const fa_cache_append_args* p) {
               : (inter ? run_append_to<128, false, true>(a, p->cache, blocks, stream) : run_append_to<128, false, false>(a, p->cache, blocks, stream));
 }
 
+// Rows of a 4-bit cache in 16 bits at any strides: fa_cache_read_u4, and the caches that attention of many tokens works on.
+int fa::launch_read_u4(const fa_cache_read_args& p, long long o_batch, long long o_row, long long o_head, bool live_only, DeviceState*) {
+    ReadArgs a;
+    const int rc = check_layout(p.layout, FA_CACHE_U4, p.d_head, p.seq_len_kv, 0, &a.map);
+    if (rc != FA_OK) return rc;
+    const int slots = kThreads / (p.d_head / 8);
+    const long long tiles = ((long long)p.num_rows + slots * kUnroll - 1) / (slots * kUnroll);
+    const long long blocks = tiles * p.batch_size * p.num_kv_heads;
+    if (blocks > 0x7FFFFFFFll || (long long)p.num_rows + slots * kUnroll > 0x7FFFFFFFll) return FA_ERR_INVALID_ARGUMENT;
+    a.k = static_cast<const uint8_t*>(p.k_cache);
+    a.v = static_cast<const uint8_t*>(p.v_cache);
+    a.kp = static_cast<const __half2*>(p.k_params);
+    a.vp = static_cast<const __half2*>(p.v_params);
+    a.k_out = static_cast<uint16_t*>(p.k_out);
+    a.v_out = static_cast<uint16_t*>(p.v_out);
+    a.o_batch = o_batch;
+    a.o_row = o_row;
+    a.o_head = o_head;
+    a.live_only = live_only;
+    a.hkv = p.num_kv_heads;
+    a.seq_len_kv = p.seq_len_kv;
+    a.n_rows = p.num_rows;
+    a.tiles = (int)tiles;
+    a.block_stride = p.layout.block_stride;
+    a.head_stride = p.layout.head_stride;
+    a.row_stride = p.layout.row_stride;
+    a.p_block_stride = p.layout.param_block_stride;
+    a.p_head_stride = p.layout.param_head_stride;
+    a.p_row_stride = p.layout.param_row_stride;
+    a.seq_lens = p.layout.seq_lens;
+    a.first_rows = p.first_rows;
+    const bool bf = p.dtype == FA_DTYPE_BF16;
+    auto kernel = p.d_head == 64 ? (bf ? read_u4_kernel<64, true> : read_u4_kernel<64, false>) : (bf ? read_u4_kernel<128, true> : read_u4_kernel<128, false>);
+    return launch_dependent(kernel, (unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(p.stream), 1, a);
+}
+
 FA_EXPORT int fa_cache_read_u4(const fa_cache_read_args* p) {
     if (!p || !p->k_cache || !p->k_params || !p->v_cache || !p->v_params || !p->k_out || !p->v_out) return FA_ERR_INVALID_ARGUMENT;
     if (p->batch_size <= 0 || p->num_kv_heads <= 0 || p->seq_len_kv <= 0 || p->num_rows <= 0) return FA_ERR_INVALID_ARGUMENT;
     if (p->d_head != 64 && p->d_head != 128) return FA_ERR_UNSUPPORTED;
     if (p->dtype != FA_DTYPE_F16 && p->dtype != FA_DTYPE_BF16) return FA_ERR_UNSUPPORTED;
-    ReadArgs a;
-    int rc = check_layout(p->layout, FA_CACHE_U4, p->d_head, p->seq_len_kv, 0, &a.map);
+    if ((long long)p->num_rows + 256 > 0x7FFFFFFFll) return FA_ERR_INVALID_ARGUMENT;
+    CacheMap map;
+    const int rc = check_layout(p->layout, FA_CACHE_U4, p->d_head, p->seq_len_kv, 0, &map);
     if (rc != FA_OK) return rc;
     if (!aligned16(p->k_cache) || !aligned16(p->v_cache) || !aligned16(p->k_params) || !aligned16(p->v_params) || !aligned16(p->k_out) || !aligned16(p->v_out))
         return FA_ERR_MISALIGNED;
-    const int slots = kThreads / (p->d_head / 8);
-    const long long tiles = ((long long)p->num_rows + slots * kUnroll - 1) / (slots * kUnroll);
-    const long long blocks = tiles * p->batch_size * p->num_kv_heads;
-    if (blocks > 0x7FFFFFFFll || (long long)p->num_rows + slots * kUnroll > 0x7FFFFFFFll) return FA_ERR_INVALID_ARGUMENT;
     DeviceState* st = device_state();
     if (!st) return FA_ERR_CUDA;
     if (st->cc_major != 10) return FA_ERR_NOT_SM100;
-    a.k = static_cast<const uint8_t*>(p->k_cache);
-    a.v = static_cast<const uint8_t*>(p->v_cache);
-    a.kp = static_cast<const __half2*>(p->k_params);
-    a.vp = static_cast<const __half2*>(p->v_params);
-    a.k_out = static_cast<uint16_t*>(p->k_out);
-    a.v_out = static_cast<uint16_t*>(p->v_out);
-    a.hkv = p->num_kv_heads;
-    a.seq_len_kv = p->seq_len_kv;
-    a.n_rows = p->num_rows;
-    a.tiles = (int)tiles;
-    a.block_stride = p->layout.block_stride;
-    a.head_stride = p->layout.head_stride;
-    a.row_stride = p->layout.row_stride;
-    a.p_block_stride = p->layout.param_block_stride;
-    a.p_head_stride = p->layout.param_head_stride;
-    a.p_row_stride = p->layout.param_row_stride;
-    a.seq_lens = p->layout.seq_lens;
-    a.first_rows = p->first_rows;
-    const bool bf = p->dtype == FA_DTYPE_BF16;
-    auto kernel = p->d_head == 64 ? (bf ? read_u4_kernel<64, true> : read_u4_kernel<64, false>) : (bf ? read_u4_kernel<128, true> : read_u4_kernel<128, false>);
-    return launch_dependent(kernel, (unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(p->stream), 1, a);
+    const long long row = (long long)p->num_kv_heads * p->d_head;
+    return launch_read_u4(*p, row * p->num_rows, row, p->d_head, false, st);
 }

@@ -43,6 +43,8 @@ constexpr int kMaxCluster = 8;                 // portable cluster size
 constexpr int tile_keys(int nt) { return nt == 1 ? 64 : 32; }
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kClusterTiles = 1;               // see make_plan
+constexpr int kManyRows = 64, kManyKeys = 1024;   // see many_rows
+constexpr size_t kCopyBytes = 256u << 20;      // of K and V in fp16 at a time
 constexpr float kGrow = 8.0f;                  // a running max may be exceeded by this much (in powers of two) before it is raised
 
 struct U4Args {
@@ -892,6 +894,57 @@ __global__ void __launch_bounds__(1024) u4_merge_kernel(const __grid_constant__ 
     }
 }
 
+// ------------------------------------------------------------------------------------------ many tokens
+// bf16 q as fp16 for the 16-bit kernel: a power of two for each (sequence, KV head) puts its largest element at 2^14 .. 2^15 and
+// goes back into the scores' scale, as in u4_kernel.  `top`: the largest element's bits (a maximum, so in any order the same).
+__global__ void __launch_bounds__(256) q_top_kernel(const uint4* q, int* top, int per_head, int hkv, FastDiv by_hkv, FastDiv by_tokens) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    // block (sequence and token, KV head): `per_head` 16-byte pieces
+    const int bt = by_hkv.quot(blockIdx.x), h = blockIdx.x - bt * hkv, b = by_tokens.quot(bt);
+    uint32_t m = 0;
+    for (int i = threadIdx.x; i < per_head; i += blockDim.x) {
+        const uint4 u = q[(long long)blockIdx.x * per_head + i];
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) m = max(m, max(w[j] & 0x7FFFu, (w[j] >> 16) & 0x7FFFu));
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((threadIdx.x & 31) == 0) atomicMax(top + b * hkv + h, (int)m);
+}
+__global__ void __launch_bounds__(256) q_f16_kernel(const uint4* q, uint4* out, const int* top, float* factor, int per_head, int hkv, FastDiv by_hkv, FastDiv by_tokens) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int bt = by_hkv.quot(blockIdx.x), h = blockIdx.x - bt * hkv, b = by_tokens.quot(bt);
+    const uint32_t e = max((uint32_t)top[b * hkv + h] >> 7, 15u);
+    const float up = __uint_as_float((268u - e) << 23);
+    if (threadIdx.x == 0) factor[b * hkv + h] = __uint_as_float((e - 14u) << 23);          // every token writes the same
+    for (int i = threadIdx.x; i < per_head; i += blockDim.x) {
+        const uint4 u = q[(long long)blockIdx.x * per_head + i];
+        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 f = unpack16<true>(w[j]);
+            w[j] = pack16<false>(f.x * up, f.y * up);
+        }
+        out[(long long)blockIdx.x * per_head + i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+__global__ void __launch_bounds__(256) f16_to_bf16_kernel(uint4* o, long long n) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const uint4 u = o[i];
+        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 f = unpack16<false>(w[j]);
+            w[j] = pack16<true>(f.x, f.y);
+        }
+        o[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
 // ------------------------------------------------------------------------------------------ host
 struct Plan {
     int nt;                 // 8-row columns of a block
@@ -981,6 +1034,105 @@ int run_u4_rows(const U4Args& a, const Plan& p, DeviceState* st, cudaStream_t st
     return run_u4<D, BF16, 4>(a, p.ctas, st, stream);
 }
 
+// Many query rows: the 16-bit kernel (tcgen05) over a copy of the cache in fp16.  mma.sync runs at a quarter of tcgen05's rate,
+// and a row block reads and unpacks the whole cache again; the copy costs 4.5 bytes an element once.
+struct ManyPlan {
+    int batch;                                // sequences of a copy
+    int splits;                               // KV splits of the 16-bit kernel
+    size_t cache, partial, q, factor;         // bytes: K's copy (V's as much), partial results, q in fp16, factors and tops
+    size_t bytes() const { return 2 * cache + partial + q + 2 * factor; }
+};
+bool many_rows(int hq, int hkv, int n_tok, int kv_len) {
+    const long long rows = (long long)n_tok * (hq / hkv);
+    return rows >= kManyRows && kv_len >= kManyKeys && hq / hkv <= 128;
+}
+ManyPlan make_many_plan(int batch, int hq, int hkv, int n_tok, int kv_len, int d_head) {
+    ManyPlan p;
+    const size_t one = (size_t)hkv * kv_len * d_head * 2;
+    const size_t fit = kCopyBytes / (2 * one);
+    p.batch = fit < 1 ? 1 : fit < (size_t)batch ? (int)fit : batch;
+    p.cache = align256(one * p.batch);
+    const int group = hq / hkv, per_tile = 128 / group < n_tok ? 128 / group : n_tok, n_qt = (n_tok + per_tile - 1) / per_tile;
+    p.splits = fa_decode_gqa_default_splits(p.batch * n_qt, hkv, kv_len);
+    p.partial = align256(fa_decode_workspace_bytes(p.batch, n_tok * hq, d_head, p.splits));
+    p.q = align256((size_t)batch * n_tok * hq * d_head * 2);
+    p.factor = align256((size_t)batch * hkv * sizeof(float));
+    return p;
+}
+
+int run_many(const fa_decode_gqa_u4_args* p, int n_tok, DeviceState* st) {
+    const ManyPlan m = make_many_plan(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->d_head);
+    cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
+    uint8_t* at = static_cast<uint8_t*>(p->workspace);
+    uint8_t *k16 = at, *v16 = k16 + m.cache, *partial = v16 + m.cache, *q16 = partial + m.partial;
+    float* factor = reinterpret_cast<float*>(q16 + m.q);
+    int* top = reinterpret_cast<int*>(q16 + m.q + m.factor);
+    const bool bf = p->dtype == FA_DTYPE_BF16;
+    const size_t row = (size_t)p->num_q_heads * p->d_head;                       // elements of a token
+    const long long blocks = (long long)p->batch_size * n_tok * p->num_kv_heads, pieces = (long long)p->batch_size * n_tok * row / 8;
+    const int per_head = (int)(row / 8 / p->num_kv_heads), hkv = p->num_kv_heads;
+    const FastDiv by_hkv(hkv), by_tokens(n_tok);
+    int rc;
+    if (bf) {
+        FA_CUDA_TRY(cudaMemsetAsync(top, 0, (size_t)p->batch_size * hkv * sizeof(int), stream));
+        const uint4* q = static_cast<const uint4*>(p->q);
+        const int threads = per_head >= 256 ? 256 : (per_head + 31) / 32 * 32;
+        if ((rc = launch_dependent(q_top_kernel, (unsigned)blocks, threads, 0, stream, 1, q, top, per_head, hkv, by_hkv, by_tokens)) != FA_OK) return rc;
+        if ((rc = launch_dependent(q_f16_kernel, (unsigned)blocks, threads, 0, stream, 1, q, reinterpret_cast<uint4*>(q16), top, factor, per_head, hkv, by_hkv, by_tokens)) != FA_OK)
+            return rc;
+    }
+    for (int b0 = 0; b0 < p->batch_size; b0 += m.batch) {
+        const int nb = p->batch_size - b0 < m.batch ? p->batch_size - b0 : m.batch;
+        fa_cache_read_args r = {};
+        r.layout = p->layout;
+        if (r.layout.seq_lens) r.layout.seq_lens += b0;
+        const bool paged = r.layout.block_table != nullptr;
+        if (paged) r.layout.block_table += (size_t)b0 * r.layout.block_table_stride;
+        const size_t skip = paged ? 0 : (size_t)b0 * r.layout.block_stride, pskip = paged ? 0 : (size_t)b0 * r.layout.param_block_stride * 4;
+        r.k_cache = static_cast<const uint8_t*>(p->k_cache) + skip;
+        r.v_cache = static_cast<const uint8_t*>(p->v_cache) + skip;
+        r.k_params = static_cast<const uint8_t*>(p->k_params) + pskip;
+        r.v_params = static_cast<const uint8_t*>(p->v_params) + pskip;
+        r.k_out = k16;
+        r.v_out = v16;
+        r.batch_size = nb;
+        r.num_kv_heads = hkv;
+        r.seq_len_kv = r.num_rows = p->seq_len_kv;
+        r.d_head = p->d_head;
+        r.dtype = FA_DTYPE_F16;
+        r.stream = p->stream;
+        const long long head = (long long)p->seq_len_kv * p->d_head;
+        if ((rc = launch_read_u4(r, head * hkv, p->d_head, head, true, st)) != FA_OK) return rc;
+        fa_decode_gqa_args g = {};
+        const size_t q0 = (size_t)b0 * n_tok * row;
+        g.q = bf ? static_cast<const void*>(q16 + 2 * q0) : static_cast<const uint16_t*>(p->q) + q0;
+        g.k = k16;
+        g.v = v16;
+        g.o = static_cast<uint16_t*>(p->o) + q0;
+        g.lse = p->lse ? p->lse + (size_t)b0 * n_tok * p->num_q_heads : nullptr;
+        g.batch_size = nb;
+        g.num_q_heads = p->num_q_heads;
+        g.num_kv_heads = hkv;
+        g.seq_len_kv = p->seq_len_kv;
+        g.d_head = p->d_head;
+        g.scale = p->scale;
+        g.dtype = FA_DTYPE_F16;
+        g.num_splits = m.splits;
+        g.kv_batch_stride = head * hkv;
+        g.kv_head_stride = head;
+        g.kv_row_stride = p->d_head;
+        g.seq_lens = r.layout.seq_lens;
+        g.num_q_tokens = n_tok;
+        g.workspace = partial;
+        g.workspace_bytes = m.partial;
+        g.stream = p->stream;
+        if ((rc = decode_gqa(&g, bf ? factor + (size_t)b0 * hkv : nullptr)) != FA_OK) return rc;
+    }
+    if (!bf) return FA_OK;
+    const long long want = (pieces + 255) / 256, most = 16ll * st->sm_count;
+    return launch_dependent(f16_to_bf16_kernel, (unsigned)(want < most ? want : most), 256, 0, stream, 1, static_cast<uint4*>(p->o), pieces);
+}
+
 }  // namespace
 }  // namespace fa
 
@@ -992,6 +1144,8 @@ FA_EXPORT size_t fa_decode_gqa_u4_workspace_bytes(int batch_size, int num_q_head
         return 0;
     if (d_head != 64 && d_head != 128) return 0;
     DeviceState* st = device_state();
+    if (many_rows(num_q_heads, num_kv_heads, num_q_tokens > 0 ? num_q_tokens : 1, seq_len_kv))
+        return make_many_plan(batch_size, num_q_heads, num_kv_heads, num_q_tokens, seq_len_kv, d_head).bytes();
     return make_plan(batch_size, num_q_heads, num_kv_heads, num_q_tokens > 0 ? num_q_tokens : 1, seq_len_kv, false, d_head, st).bytes;
 }
 
@@ -1014,6 +1168,11 @@ FA_EXPORT int fa_decode_gqa_u4(const fa_decode_gqa_u4_args* p) {
     DeviceState* st = device_state();
     if (!st) return FA_ERR_CUDA;
     if (st->cc_major != 10) return FA_ERR_NOT_SM100;
+    if (many_rows(p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv)) {
+        const size_t need = make_many_plan(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->d_head).bytes();
+        if (!p->workspace || p->workspace_bytes < need || !aligned16(p->workspace)) return FA_ERR_WORKSPACE;
+        return run_many(p, n_tok, st);
+    }
     const Plan plan = make_plan(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->layout.seq_lens != nullptr, p->d_head, st);
     if (plan.tiles > 0x7FFF0000ll) return FA_ERR_INVALID_ARGUMENT;
     if (!p->workspace || p->workspace_bytes < plan.bytes || !aligned16(p->workspace)) return FA_ERR_WORKSPACE;

@@ -144,5 +144,10 @@ int launch_decode_gqa(const GqaLaunch& g, DeviceState* st);
 // a 16-bit or e4m3 cache.
 struct CacheMap;
 int check_layout(const fa_cache_layout& l, int cache, int d_head, int seq_len_kv, int elem, CacheMap* map);
+// The kernel of fa_cache_read_u4 with any strides of the outputs (elements).  `live_only`: rows that a sequence does not have
+// are not written.
+int launch_read_u4(const fa_cache_read_args& p, long long o_batch, long long o_row, long long o_head, bool live_only, DeviceState* st);
+// fa_decode_gqa with a factor on the scores of each (sequence, KV head) (16-bit types; device, may be null).
+int decode_gqa(const fa_decode_gqa_args* a, const float* score_factor);
 
 }  // namespace fa

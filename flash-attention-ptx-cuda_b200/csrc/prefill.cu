@@ -909,6 +909,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 const int limit0 = min(it.kv_len, lim0 + row0 / gq.group), limit1 = min(it.kv_len, lim0 + (row0 + 8) / gq.group);
                 float scale_log2 = scale_log2_in;
                 if constexpr (FP8) scale_log2 *= q_scale[it.bh] * k_scale[it.bh];
+                else if (GQA && q_scale != nullptr) scale_log2 *= q_scale[it.bh];
                 const uint64_t scale2 = pack2(scale_log2, scale_log2);
                 float m0 = -1e30f, m1 = -1e30f;           // reference max of this thread's partial sums
                 uint64_t sum0 = pack2(0.0f, 0.0f), sum1 = sum0;
@@ -1072,6 +1073,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                                        : GQA  ? max(0, min(it.kv_len, it.kv_len - gq.n_tok + 1 + it.tok0)) : it.kv_len;
             float scale_log2 = scale_log2_in;
             if constexpr (FP8) scale_log2 *= q_scale[it.bh] * k_scale[it.bh];
+            else if (GQA && q_scale != nullptr) scale_log2 *= q_scale[it.bh];
             const uint64_t scale2 = pack2(scale_log2, scale_log2);
             // Running state of THIS thread: the reference max its partial row sum is expressed in.
             // The row's two threads alternate tiles; the max in use travels from tile to tile

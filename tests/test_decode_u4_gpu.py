@@ -332,3 +332,95 @@ def test_refused_by_the_operator(op, dev):
                       ((q, kc, kp, vc, vp, 0.1, torch.zeros(3, device=dev, dtype=torch.int32)), ValueError)):
         with pytest.raises(err):
             op.decode_gqa_u4(*args)
+
+
+def check_many(q, cache, o, lse, scale):
+    """Many query rows go through a copy of the cache in fp16: beside O's rounding, V^ (2^-12 of it), P (2^-12) and K^
+    (2^-12 of its elements) are rounded.  Scores are off by at most d = scale * 2^-12 * sum |q k| (and 32-bit parts, taken as
+    2^-20 of the same sum), so P by the factors exp(+-2d), and O by at most sum p |V^| (2^-12 + 2^-12 + exp(2d) - 1 ...)."""
+    want, want_l, _, _ = reference(q, cache, scale)
+    b, t, hq, d = q.shape
+    hkv = cache.tensors[0].shape[2]
+    for i in range(b):
+        (kc, kp), (vc, vp) = cache.packed[0][i], cache.packed[1][i]
+        if kc.shape[0] == 0:
+            assert not o[i].any() and torch.isinf(lse[i]).all()
+            continue
+        k, v = u4_unpack(kc, kp), u4_unpack(vc, vp)
+        x = q[i].double().abs().view(t, hkv, hq // hkv, d)
+        dev = scale * float(torch.einsum("thgd,hd->thg", x, k.abs().amax(0)).max()) * (2.0 ** -12 + 2.0 ** -20)
+        top = v.abs().amax(0).repeat_interleave(hq // hkv, 0)[None]             # sum p |V^| <= max |V^|
+        tol = top * (2.0 ** -11 + 2.0 ** -18 + np.expm1(2 * dev)) + want[i].abs() * (torch.finfo(q.dtype).eps / 2 + 2.0 ** -12) + 2.0 ** -24
+        assert ((o[i].double() - want[i]).abs() <= tol).all()
+        fin = torch.isfinite(want_l[i])
+        assert torch.equal(torch.isfinite(lse[i]), fin)
+        assert ((lse[i].double() - want_l[i])[fin].abs() <= dev + 2.0 ** -18).all()
+        # and on average the roundings are as small as theirs are: sqrt of the sum of their squares, 4 of 2^-12 / sqrt(3), doubled
+        rel = float((o[i].double() - want[i]).norm() / want[i].norm())
+        assert rel < 2 * (2 * 2.0 ** -12 + torch.finfo(q.dtype).eps / 2), rel
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,t,hq,hkv,skv,page,lens", [
+    (1, 64, 1, 1, 1024, 0, None),                      # the smallest that counts as many rows
+    (2, 33, 8, 2, 1100, 16, [1100, 700]),
+    (3, 100, 6, 3, 1500, 0, [1500, 40, 0]),            # fewer keys than tokens, and none
+    (2, 300, 5, 1, 1027, 64, [1027, 1026]),
+])
+def test_many_tokens(op, dev, dtype, d, b, t, hq, hkv, skv, page, lens):
+    q, cache = make(dev, dtype, b, t, hq, hkv, skv, d, lens, page, seed=t)
+    o, lse = run(op, q, cache, d ** -0.5, lens=lens is not None or page != 0)
+    check_many(q, cache, o, lse, d ** -0.5)
+
+
+def test_many_tokens_of_any_magnitude(op, dev):
+    """bf16 queries far outside fp16's range, another for each sequence and KV head."""
+    b, t, hq, hkv, skv, d = 2, 40, 8, 2, 1024, 64
+    q, cache = make(dev, "bf16", b, t, hq, hkv, skv, d, seed=11)
+    size = torch.tensor([[1e-9, 1e9], [3e5, 1.0]], device=dev).repeat_interleave(hq // hkv, 1)[:, None, :, None]
+    for i in range(2):
+        for h in range(2):                             # one magnitude at a time decides the scale
+            s = float(size[i, 0, h * 4, 0])
+            qs = (q.float() * size).bfloat16()
+            o, lse = run(op, qs, cache, 0.125 / s)
+            small = qs[i:i + 1, :, h * 4:h * 4 + 4]
+            class View:
+                tensors = [cache.tensors[0][:, :, h:h + 1]]
+                packed = [[(c[:, h:h + 1], p[:, h:h + 1])] for c, p in (cache.packed[0][i], cache.packed[1][i])]
+            check_many(small, View, o[i:i + 1, :, h * 4:h * 4 + 4], lse[i:i + 1, :, h * 4:h * 4 + 4], 0.125 / s)
+
+
+def test_many_tokens_copy_in_parts(op, dev):
+    """More sequences than one copy holds (256 MB of K and V): the same bits as sequence by sequence with the same splits."""
+    b, t, hq, hkv, skv, d = 3, 16, 32, 8, 24000, 128
+    lens = [24000, 17, 20001]
+    q, cache = make(dev, "f16", b, t, hq, hkv, skv, d, lens, seed=12)
+    o, lse = run(op, q, cache, 0.0884)
+    kc, kp, vc, vp = cache.tensors
+    for i in range(b):
+        oi, li = op.decode_gqa_u4(q[i:i + 1], kc[i:i + 1], kp[i:i + 1], vc[i:i + 1], vp[i:i + 1], 0.0884,
+                                  torch.tensor(lens[i:i + 1], device=dev, dtype=torch.int32))
+        assert torch.equal(torch.isinf(li), torch.isinf(lse[i:i + 1]))
+        fin = torch.isfinite(li)
+        assert (li - lse[i:i + 1])[fin].abs().max() < 1e-4 and (oi.float() - o[i:i + 1].float()).abs().max() < 4 * 2.0 ** -11
+
+
+def test_many_tokens_captured_and_replayed(op, dev):
+    q, cache = make(dev, "bf16", 2, 40, 8, 2, 1100, 128, [1100, 900], page=16, seed=13)
+    lens = torch.tensor(cache.lens, device=dev, dtype=torch.int32)
+    kc, kp, vc, vp = cache.tensors
+    side = torch.cuda.Stream(device=dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        op.decode_gqa_u4(q, kc, kp, vc, vp, 0.0884, lens, cache.table)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = op.decode_gqa_u4(q, kc, kp, vc, vp, 0.0884, lens, cache.table)
+    torch.cuda.synchronize()
+    q.copy_(q.flip(0) * 100)
+    lens.copy_(torch.tensor([500, 60], device=dev))
+    graph.replay()
+    torch.cuda.synchronize()
+    want = op.decode_gqa_u4(q, kc, kp, vc, vp, 0.0884, lens, cache.table)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
