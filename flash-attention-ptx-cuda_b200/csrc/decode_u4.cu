@@ -39,11 +39,12 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kMaxCluster = 8;                 // portable cluster size
 // Keys of a tile.  The longer one has a third fewer instructions a key besides the products and twice the independent ones
-// to fill a product's latency with; with more than one column of 8 rows there are enough of those, and no registers.
+// to fill a product's latency with (B=32 Hkv=8 Skv=16384: 151 us with 32, 126 with 64); with two columns of 8 rows there are
+// enough of those, and no registers.
 constexpr int tile_keys(int nt) { return nt == 1 ? 64 : 32; }
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kClusterTiles = 1;               // see make_plan
-constexpr int kManyRows = 64, kManyKeys = 1024;   // see many_rows
+constexpr int kManyRows = 96, kManyKeys = 256;    // see many_rows
 constexpr size_t kCopyBytes = 256u << 20;      // of K and V in fp16 at a time
 constexpr float kGrow = 8.0f;                  // a running max may be exceeded by this much (in powers of two) before it is raised
 
@@ -78,7 +79,7 @@ struct Shape {
     static constexpr int G = D / kU4Group;                     // groups of a row
     static constexpr int Keys = tile_keys(NT), J = Keys / 16;  // of a tile, and its 16-key steps
     static constexpr int RowBytes = D / 2;
-    static constexpr int Stages = NT == 4 ? 4 : 3;
+    static constexpr int Stages = 3;
     static constexpr int CodeBytes = Keys * RowBytes;
     static constexpr int StageBytes = 2 * CodeBytes;
     static constexpr int FactorBytes = Keys * G * 16;         // of a tile: for each key K's (scale, offset) and V's, unpacked
@@ -989,7 +990,7 @@ int clusters_at_once(DeviceState* st, int size) {
 Plan make_plan(int batch, int hq, int hkv, int n_tok, int kv_len, bool own_lengths, int d_head, DeviceState* st) {
     Plan p;
     const long long rows = (long long)n_tok * (hq / hkv);
-    p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    p.nt = rows <= 8 ? 1 : 2;
     p.row_blocks = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
     const long long items = (long long)batch * hkv * p.row_blocks, item_tiles = (kv_len + tile_keys(p.nt) - 1) / tile_keys(p.nt);
     p.tiles = items * item_tiles;
@@ -1030,12 +1031,15 @@ int run_u4(const U4Args& a, int ctas, DeviceState* st, cudaStream_t stream) {
 template <int D, bool BF16>
 int run_u4_rows(const U4Args& a, const Plan& p, DeviceState* st, cudaStream_t stream) {
     if (p.nt == 1) return run_u4<D, BF16, 1>(a, p.ctas, st, stream);
-    if (p.nt == 2) return run_u4<D, BF16, 2>(a, p.ctas, st, stream);
-    return run_u4<D, BF16, 4>(a, p.ctas, st, stream);
+    return run_u4<D, BF16, 2>(a, p.ctas, st, stream);
 }
 
 // Many query rows: the 16-bit kernel (tcgen05) over a copy of the cache in fp16.  mma.sync runs at a quarter of tcgen05's rate,
-// and a row block reads and unpacks the whole cache again; the copy costs 4.5 bytes an element once.
+// and a block of 16 rows reads and unpacks the whole cache again; the copy costs 4.5 bytes an element once.  (us in a graph, row
+// blocks / copy, f16 D=128 Hkv=8: B=8 Skv=4096 64 rows 61 / 66, 128 rows 109 / 71, 256 rows 203 / 73; B=1 Skv=4096 64 rows 17 / 19,
+// 128 rows 23 / 22, 256 rows 38 / 22; B=1 Skv=512 256 rows 12.3 / 11.7.  Blocks of 32 rows need more registers than
+// there are: 97 and 163 where those of 16 take 61 and 109.)  The copy rounds K^ and V^ to fp16, what a 16-bit cache of the
+// same values would hold: O is off by 4e-4 of its norm where the row blocks' is by 3e-4 and fp16 itself by 2e-4.
 struct ManyPlan {
     int batch;                                // sequences of a copy
     int splits;                               // KV splits of the 16-bit kernel
