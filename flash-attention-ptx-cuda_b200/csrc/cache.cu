@@ -10,6 +10,7 @@
 #include <cmath>
 #include <cuda_fp8.h>
 
+#include "fast_div.h"
 #include "host_common.h"
 #include "ptx.cuh"
 #include "u4.cuh"
@@ -176,6 +177,7 @@ struct AppendArgs {
     long long p_block_stride, p_head_stride, p_row_stride;    // pairs
     const int *seq_lens, *num_new, *positions;
     const float *q_scale, *k_scale, *v_scale;
+    FastDiv by_tokens, by_pairs, by_splits, by_group;
 };
 
 struct Token {
@@ -184,7 +186,7 @@ struct Token {
 };
 __device__ __forceinline__ Token token(const AppendArgs& a, int n) {
     Token r;
-    r.b = n / a.n_tokens;
+    r.b = a.by_tokens.quot(n);
     const int t = n - r.b * a.n_tokens;
     r.row = sequence_length(a.seq_lens, r.b, a.seq_len_kv) - a.n_tokens + t;
     r.live = r.row >= 0 && (a.num_new == nullptr || t >= a.n_tokens - a.num_new[r.b]);
@@ -204,45 +206,75 @@ __device__ __forceinline__ uint2 to_e4m3(const uint4& x, float inv) {
     return make_uint2(e4m3x4(make_float2(a.x * inv, a.y * inv), make_float2(b.x * inv, b.y * inv)),
                       e4m3x4(make_float2(c.x * inv, c.y * inv), make_float2(d.x * inv, d.y * inv)));
 }
+template <bool BF16>
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (BF16) asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 // 8 elements as 4-bit codes; the 8 lanes of a group of 64 call this together.  Returns the codes, and scale and
-// offset in every lane.
+// offset in every lane.  An element past +-65504 gets the code of the border: its difference from the offset is clamped.
 template <bool BF16>
 __device__ __forceinline__ uint32_t to_u4(const uint4& x, __half2* param) {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    float f[8];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 a = unpack16<BF16>(w[i]);
-        f[2 * i] = max_nan(min_nan(a.x, kU4Max), -kU4Max);
-        f[2 * i + 1] = max_nan(min_nan(a.y, kU4Max), -kU4Max);
-    }
-    float lo = f[0], hi = f[0];
-#pragma unroll
-    for (int i = 1; i < 8; i++) { lo = min_nan(lo, f[i]); hi = max_nan(hi, f[i]); }
+    uint32_t lo2 = min2_nan<BF16>(min2_nan<BF16>(w[0], w[1]), min2_nan<BF16>(w[2], w[3]));
+    uint32_t hi2 = max2_nan<BF16>(max2_nan<BF16>(w[0], w[1]), max2_nan<BF16>(w[2], w[3]));
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {
-        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        lo2 = min2_nan<BF16>(lo2, __shfl_xor_sync(0xffffffffu, lo2, o));
+        hi2 = max2_nan<BF16>(hi2, __shfl_xor_sync(0xffffffffu, hi2, o));
     }
+    const float2 l = unpack16<BF16>(lo2), h = unpack16<BF16>(hi2);
+    const float lo = max_nan(min_nan(min_nan(l.x, l.y), kU4Max), -kU4Max), hi = max_nan(min_nan(max_nan(h.x, h.y), kU4Max), -kU4Max);
     const __half z16 = __float2half_rn(lo);
     const float z = __half2float(z16);
     const __half s16 = __float2half_rn(__fmul_rn(__fsub_rn(hi, z), 1.0f / 15.0f));
     const float s = __half2float(s16), inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
+    // round to a whole number, ties to even, by adding 1.5 * 2^23: the code is in the last bits; 16 a + b of the bits then
+    // strings the codes together, with the constant's share taken off at the end
+    constexpr float kRound = 12582912.0f;
+    constexpr uint32_t kBits = 0x4B400000u;
     uint32_t codes = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(f[i], z), inv), 0.0f), 15.0f);
-        codes |= (uint32_t)__float2int_rn(c) << (4 * i);
+    for (int i = 7; i >= 0; i--) {
+        const float2 f = unpack16<BF16>(w[i / 2]);
+        const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(i & 1 ? f.y : f.x, z), inv), 0.0f), 15.0f);
+        codes = codes * 16u + __float_as_uint(__fadd_rn(c, kRound));
     }
+    constexpr uint32_t kShare = kBits * 0x11111111u;
     *param = __halves2half2(s16, z16);
-    return codes;
+    return codes - kShare;
+}
+
+// kUnroll heads of a token and every `step`-th after, from `src` (the lane's part of head 0): loads all before it uses one.
+// `use(h, x)` is called by whole warps, with zeros where there is no head.
+template <int D, class Use>
+__device__ __forceinline__ void walk_heads(const uint16_t* src, int first, int end, int step, bool live, Use use) {
+    for (int h0 = first; __any_sync(0xffffffffu, h0 < end); h0 += step * kUnroll) {
+        uint4 x[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; u++) {
+            x[u] = make_uint4(0, 0, 0, 0);
+            if (live && h0 + u * step < end) x[u] = ld_row_16(src + (h0 + u * step) * D);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; u++) use(h0 + u * step, x[u]);
+    }
 }
 
 template <int D, bool BF16, bool INTER, int CACHE>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) append_kernel(const __grid_constant__ AppendArgs a) {
     constexpr int LPR = D / 8, SLOTS = kThreads / LPR;
     extern __shared__ float2 table[];                       // [tokens][dim / 2]
-    const int split = blockIdx.x % a.splits, n0 = blockIdx.x / a.splits * a.tokens;
+    const int split = (int)blockIdx.x - a.by_splits.quot(blockIdx.x) * a.splits, n0 = a.by_splits.quot(blockIdx.x) * a.tokens;
     const int pairs = a.rot.dim / 2;
     grid_dependency_wait();
     grid_launch_dependents();
@@ -250,73 +282,64 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     const int h_begin = split * per, h_end = min(heads, h_begin + per);
     if (h_begin < a.hq + a.hkv)                             // not v alone
         for (int i = threadIdx.x; i < a.tokens * pairs; i += kThreads) {
-            const int t = i / pairs;
+            const int t = a.by_pairs.quot(i);
             float2 cs;
             cos_sin(a.rot, token(a, min(n0 + t, a.n_all - 1)).position, i - t * pairs, false, &cs.x, &cs.y);
             table[i] = cs;
         }
     __syncthreads();
     const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR;
-    const int t = slot & (a.tokens - 1), step = SLOTS / a.tokens;
+    const int t = slot & (a.tokens - 1), step = SLOTS / a.tokens, mine = slot / a.tokens;
     const int n = n0 + t;
     const bool in = n < a.n_all;
     const Token tk = token(a, min(n, a.n_all - 1));
+    const bool live = in && tk.live;
     CacheRow at = {-1, 0};
-    if (in && tk.live) at = cache_row(a.map, tk.b, tk.row);
+    if (live) at = cache_row(a.map, tk.b, tk.row);
     Turn<BF16, INTER> turn;
     turn.template load<LPR>(table + t * pairs, lane, a.rot.dim);
-    const int group = a.hq / a.hkv;
-    for (int h0 = h_begin; h0 < h_end; h0 += step * kUnroll) {
-        uint4 x[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; u++) {
-            const int h = h0 + u * step + slot / a.tokens;
-            x[u] = make_uint4(0, 0, 0, 0);
-            if (h < h_end && in && tk.live) {
-                const uint16_t* p = h < a.hq ? a.q + n * a.q_stride + h * D
-                                  : h < a.hq + a.hkv ? a.k + n * a.k_stride + (h - a.hq) * D
-                                                     : a.v + n * a.v_stride + (h - a.hq - a.hkv) * D;
-                x[u] = ld_row_16(p + lane * 8);
+
+    // q
+    if (h_begin < a.hq) {
+        const long long o = (long long)n * a.hq * D + lane * 8;
+        const int end = min(h_end, a.hq);
+        walk_heads<D>(a.q + n * a.q_stride + lane * 8, h_begin + mine, end, step, live, [&](int h, const uint4& x) {
+            const uint4 y = turn.template apply<LPR>(x);
+            if (h >= end || !in) return;
+            if constexpr (CACHE == FA_CACHE_E4M3) {
+                const float inv = live ? __frcp_rn(a.q_scale[tk.b * a.hkv + a.by_group.quot(h)]) : 0.0f;
+                *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.q_out) + o + h * D) = live ? to_e4m3<BF16>(y, inv) : make_uint2(0, 0);
+            } else {
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.q_out) + o + h * D) = live ? y : make_uint4(0, 0, 0, 0);    // turned zeros may be -0
             }
+        });
+    }
+    // k and v into the cache: `in_cache` for this thread's rows, `pairs` for their scale and offset
+    const bool store = live && at.block >= 0;
+    const long long row = at.block * a.block_stride + at.in_block * a.row_stride + lane * (CACHE == FA_CACHE_U4 ? 4 : CACHE == FA_CACHE_E4M3 ? 8 : 16);
+    const long long prow = CACHE == FA_CACHE_U4 ? at.block * a.p_block_stride + at.in_block * a.p_row_stride + lane / 8 : 0;
+    auto put = [&](uint8_t* cache, __half2* params, const float* scale, int end, int h, const uint4& y) {
+        uint8_t* p = cache + row + h * a.head_stride;
+        if constexpr (CACHE == FA_CACHE_U4) {
+            __half2 param;
+            const uint32_t codes = to_u4<BF16>(y, &param);
+            if (!store || h >= end) return;
+            *reinterpret_cast<uint32_t*>(p) = codes;
+            if ((lane & 7) == 0) params[prow + h * a.p_head_stride] = param;
+        } else if (store && h < end) {
+            if constexpr (CACHE == FA_CACHE_E4M3) *reinterpret_cast<uint2*>(p) = to_e4m3<BF16>(y, __frcp_rn(scale[tk.b * a.hkv + h]));
+            else *reinterpret_cast<uint4*>(p) = y;
         }
-#pragma unroll
-        for (int u = 0; u < kUnroll; u++) {
-            const int h = h0 + u * step + slot / a.tokens;
-            const bool mine = h < h_end && in;
-            const uint4 turned = turn.template apply<LPR>(x[u]);
-            const uint4 y = h < a.hq + a.hkv ? turned : x[u];
-            const bool is_v = h >= a.hq + a.hkv;
-            const int kv_head = is_v ? h - a.hq - a.hkv : h - a.hq;
-            if (h < a.hq) {
-                if (mine) {
-                    const long long o = ((long long)n * a.hq + h) * D + lane * 8;
-                    if constexpr (CACHE == FA_CACHE_E4M3) {
-                        const float inv = tk.live ? __frcp_rn(a.q_scale[tk.b * a.hkv + h / group]) : 0.0f;
-                        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.q_out) + o) = tk.live ? to_e4m3<BF16>(y, inv) : make_uint2(0, 0);
-                    } else {
-                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.q_out) + o) = tk.live ? y : make_uint4(0, 0, 0, 0);
-                    }
-                }
-            }
-            const bool store = mine && h >= a.hq && at.block >= 0;
-            uint8_t* row = (is_v ? a.v_cache : a.k_cache) + at.block * a.block_stride + (long long)kv_head * a.head_stride + at.in_block * a.row_stride;
-            if constexpr (CACHE == FA_CACHE_U4) {
-                __half2 param;
-                const uint32_t codes = to_u4<BF16>(y, &param);       // lanes of a row agree on `store`; all take part
-                if (store) {
-                    *reinterpret_cast<uint32_t*>(row + lane * 4) = codes;
-                    if ((lane & 7) == 0)
-                        (is_v ? a.v_params : a.k_params)[at.block * a.p_block_stride + (long long)kv_head * a.p_head_stride + at.in_block * a.p_row_stride + lane / 8] = param;
-                }
-            } else if (store) {
-                if constexpr (CACHE == FA_CACHE_E4M3) {
-                    const float inv = __frcp_rn((is_v ? a.v_scale : a.k_scale)[tk.b * a.hkv + kv_head]);
-                    *reinterpret_cast<uint2*>(row + lane * 8) = to_e4m3<BF16>(y, inv);
-                } else {
-                    *reinterpret_cast<uint4*>(row + lane * 16) = y;
-                }
-            }
-        }
+    };
+    if (h_begin < a.hq + a.hkv && h_end > a.hq) {
+        const int first = max(h_begin - a.hq, 0), end = min(h_end - a.hq, a.hkv);
+        walk_heads<D>(a.k + n * a.k_stride + lane * 8, first + mine, end, step, live,
+                      [&](int h, const uint4& x) { put(a.k_cache, a.k_params, a.k_scale, end, h, turn.template apply<LPR>(x)); });
+    }
+    if (h_end > a.hq + a.hkv) {
+        const int first = max(h_begin - a.hq - a.hkv, 0), end = h_end - a.hq - a.hkv;
+        walk_heads<D>(a.v + n * a.v_stride + lane * 8, first + mine, end, step, live,
+                      [&](int h, const uint4& x) { put(a.v_cache, a.v_params, a.v_scale, end, h, x); });
     }
 }
 
@@ -398,11 +421,11 @@ int make_rotary(const fa_rotary& r, int d_head, bool optional, Rotary* out) {
     if (r.rotary_dim == 0) return optional ? FA_OK : FA_ERR_INVALID_ARGUMENT;
     if (r.rotary_dim > d_head || r.rotary_dim % 16 != 0) return FA_ERR_UNSUPPORTED;
     if (r.inv_freq == nullptr || !std::isfinite(r.amplitude) || (r.interleaved != 0 && r.interleaved != 1)) return FA_ERR_INVALID_ARGUMENT;
-    const long double two_pi = 6.283185307179586476925286766559L;
+    const long double turns = 1.0L / 6.283185307179586476925286766559L;
     for (int i = 0; i < r.rotary_dim / 2; i++) {
         if (!std::isfinite(r.inv_freq[i])) return FA_ERR_INVALID_ARGUMENT;
-        long double f = r.inv_freq[i] / two_pi;
-        f -= std::floor(f);                                  // whole turns are none
+        long double f = r.inv_freq[i] * turns;
+        if (f < 0.0L || f >= 1.0L) f -= std::floor(f);       // whole turns are none
         out->turns[i] = f >= 1.0L ? 0ull : (unsigned long long)(f * 18446744073709551616.0L);
     }
     out->amplitude = r.amplitude;
@@ -613,6 +636,10 @@ FA_EXPORT int fa_cache_append(const fa_cache_append_args* p) {
     a.q_scale = p->q_scale;
     a.k_scale = p->k_scale;
     a.v_scale = p->v_scale;
+    a.by_tokens = FastDiv(a.n_tokens);
+    a.by_pairs = FastDiv(a.rot.dim > 0 ? a.rot.dim / 2 : 1);
+    a.by_splits = FastDiv(a.splits);
+    a.by_group = FastDiv(a.hq > 0 ? a.hq / a.hkv : 1);
     const unsigned blocks = (unsigned)(tiles * a.splits);
     cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
     const bool bf = p->dtype == FA_DTYPE_BF16, inter = p->rotary.interleaved != 0;
