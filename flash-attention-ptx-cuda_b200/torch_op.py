@@ -19,6 +19,7 @@ GPU the operators raise.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -29,6 +30,7 @@ from fa_b200 import FaError
 
 _DTYPES = {torch.float16: "f16", torch.bfloat16: "bf16"}
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
+_HERE = contextlib.nullcontext()
 
 
 def _check(q, k, v):
@@ -187,6 +189,10 @@ def _(q, k_cache, v_cache, scale, seq_lens=None, block_table=None):
 def _rows(t: torch.Tensor, what: str, elem_per_16: int = 8, copy: bool = False) -> tuple[torch.Tensor, tuple[int, int, int]]:
     """A 4-D tensor with the strides of its first three dimensions, as the library wants them: contiguous last dimension,
     16-byte multiples.  Another one is copied if ``copy``, else refused."""
+    if t.is_contiguous() and t.shape[3] % elem_per_16 == 0 and t.data_ptr() % 16 == 0:
+        _, n1, n2, n3 = t.shape
+        return t, (n1 * n2 * n3, n2 * n3, n3)
+
     def strides(x):
         return tuple(x.shape[3] if n == 1 else s for n, s in zip(x.shape[:3], x.stride()[:3]))
 
@@ -212,28 +218,37 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "pla
     return torch.tensor(list(out), dtype=torch.float64), amp
 
 
+def _stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _on(device: torch.device):
+    """torch.cuda.device(device), at no cost where it is the current one."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse):
     if q.dtype not in _DTYPES or k.dtype != q.dtype:
         raise TypeError("fa_b200: q and k must share dtype float16 or bfloat16")
     if not (q.is_cuda and k.is_cuda):
         raise RuntimeError("fa_b200: tensors must be on a CUDA device (there is no CPU path)")
-    if q.dim() != 4 or k.dim() != 4 or (q.shape[0], *q.shape[2:]) != (k.shape[0], *k.shape[2:]):
-        raise ValueError("fa_b200::rope: expected q [B,Hq,S,D] and k [B,Hkv,S,D]")
+    device = q.device
+    if q.dim() != 4 or k.dim() != 4 or (q.shape[0], *q.shape[2:]) != (k.shape[0], *k.shape[2:]) or k.device != device:
+        raise ValueError("fa_b200::rope: expected q [B,Hq,S,D] and k [B,Hkv,S,D] on one device")
     b, hq, s, d = q.shape
     hkv = k.shape[1]
     inv_freq = _inv_freq(inv_freq)
     (q, qs), (k, ks) = _rows(q, "q", copy=True), _rows(k, "k", copy=True)
-    q_out, k_out = torch.empty((b, hq, s, d), device=q.device, dtype=q.dtype), torch.empty((b, hkv, s, d), device=q.device, dtype=q.dtype)
-    kw = {}
+    q_out, k_out = q.new_empty((b, hq, s, d)), k.new_empty((b, hkv, s, d))
+    pos_stride = 0
     if positions is not None:
-        if positions.is_floating_point() or tuple(positions.shape) not in ((s,), (b, s)) or positions.device != q.device:
+        if positions.is_floating_point() or tuple(positions.shape) not in ((s,), (b, s)) or positions.device != device:
             raise ValueError("fa_b200::rope: positions are integers [S] or [B, S] on q's device")
         positions = positions.to(torch.int32).contiguous()
-        kw = dict(positions=positions, positions_stride=s if positions.dim() == 2 else 0)
-    with torch.cuda.device(q.device):
+        pos_stride = s if positions.dim() == 2 else 0
+    with _on(device):
         _fa.rope(q, k if hkv else None, q_out, k_out if hkv else None, b, hq, hkv, s, d, inv_freq, 2 * inv_freq.numel(),
-                 interleaved, float(amplitude), dtype=_DTYPES[q.dtype], inverse=inverse, q_strides=qs, k_strides=ks,
-                 stream=torch.cuda.current_stream(q.device), **kw)
+                 interleaved, amplitude, _DTYPES[q.dtype], positions, pos_stride, 0, inverse, qs, ks, stream=_stream(device))
     return q_out, k_out
 
 
@@ -265,9 +280,14 @@ torch.library.register_autograd("fa_b200::rope", _rope_backward, setup_context=_
 
 
 class _Rope(torch.autograd.Function):
-    forward = staticmethod(_run_rope)
-    setup_context = staticmethod(_rope_setup_context)
-    backward = staticmethod(_rope_backward)
+    @staticmethod
+    def forward(ctx, q, k, inv_freq, positions, interleaved, amplitude, inverse):
+        ctx.args = inv_freq, positions, interleaved, amplitude, not inverse
+        return _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse)
+
+    @staticmethod
+    def backward(ctx, d_q, d_k):
+        return *rope(d_q, d_k, *ctx.args), None, None, None, None, None
 
 
 def rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,
@@ -278,8 +298,9 @@ def rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, positions: to
     default 0 .. S-1; ``inverse`` turns back.  Returns the rotated (q, k), contiguous.
 
     ``torch.ops.fa_b200.rope`` is the same; plain tensors in eager mode go to the kernel without the dispatcher, whose
-    20 us a call a short prompt would feel."""
-    if type(q) in _PLAIN and type(k) in _PLAIN and not torch.compiler.is_compiling() and not is_in_torch_dispatch_mode():
+    20 us a call (50 with a gradient) a short prompt would feel."""
+    if (type(q) in _PLAIN and type(k) in _PLAIN and not torch.compiler.is_compiling() and not is_in_torch_dispatch_mode()
+            and not torch._C._are_functorch_transforms_active()):
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
             return _Rope.apply(q, k, inv_freq, positions, interleaved, amplitude, inverse)
         return _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse)
@@ -396,11 +417,11 @@ def cache_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: tor
         inv_freq = _inv_freq(inv_freq)
         kw.update(inv_freq=inv_freq, rotary_dim=2 * inv_freq.numel(), interleaved=interleaved, amplitude=float(amplitude))
     q_out = torch.empty((b, t, hq, d), device=q.device, dtype=k_cache.dtype if e4m3 else q.dtype)
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         _fa.cache_append(tokens[1], tokens[2], k_cache, v_cache, b, t, hkv, skv, d, dtype=_DTYPES[q.dtype],
                          cache_dtype="u4" if k_params is not None else "e4m3" if e4m3 else _DTYPES[q.dtype], q=tokens[0],
                          q_out=q_out, num_q_heads=hq, token_strides=tuple(strides), k_params=k_params, v_params=v_params,
-                         stream=torch.cuda.current_stream(q.device), **kw)
+                         stream=_stream(q.device), **kw)
     return q_out
 
 
@@ -426,9 +447,9 @@ def cache_read_u4(k_cache: torch.Tensor, k_params: torch.Tensor, v_cache: torch.
     if first_rows is not None:
         kw["first_rows"] = _per_sequence(first_rows, batch, k_cache.device, "first_rows")
     k, v = (torch.empty((batch, num_rows, hkv, d), device=k_cache.device, dtype=dtype) for _ in range(2))
-    with torch.cuda.device(k_cache.device):
+    with _on(k_cache.device):
         _fa.cache_read_u4(k_cache, k_params, v_cache, v_params, k, v, batch, hkv, skv, d, num_rows, dtype=_DTYPES[dtype],
-                          stream=torch.cuda.current_stream(k_cache.device), **kw)
+                          stream=_stream(k_cache.device), **kw)
     return k, v
 
 
@@ -458,12 +479,12 @@ def decode_gqa_u4(q: torch.Tensor, k_cache: torch.Tensor, k_params: torch.Tensor
     q, _ = _rows(q.contiguous(), "q", copy=True)
     o = torch.empty_like(q)
     lse = torch.empty((b, t, hq), device=q.device, dtype=torch.float32)
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         ws_bytes = _fa.decode_gqa_u4_workspace_bytes(b, hq, hkv, t, skv, d)
         ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8)
         _fa.decode_gqa_u4(q, k_cache, k_params, v_cache, v_params, o, lse, b, hq, hkv, skv, d, float(scale),
                           dtype=_DTYPES[q.dtype], num_q_tokens=t, workspace=ws, workspace_bytes=ws_bytes,
-                          stream=torch.cuda.current_stream(q.device), **kw)
+                          stream=_stream(q.device), **kw)
     return o, lse
 
 
