@@ -39,11 +39,34 @@ __device__ __forceinline__ void cos_sin(const Rotary& r, int position, int pair,
     *s = (float)((inverse ? -sd : sd) * r.amplitude);
 }
 
+// Two 32-bit operations at a time, each rounded by itself.
+struct F2 {
+    unsigned long long v;
+    __device__ __forceinline__ F2() {}
+    __device__ __forceinline__ F2(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+    __device__ __forceinline__ explicit F2(const float2& f) : F2(f.x, f.y) {}
+    __device__ __forceinline__ float2 get() const {
+        float2 f;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+        return f;
+    }
+};
+__device__ __forceinline__ F2 operator*(const F2& a, const F2& b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 operator+(const F2& a, const F2& b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+
 // A thread's part of a row: 8 elements from `lane * 8` on, turned.  With the half layout its partners lie in the lane
-// `partner`; `sin` comes with the sign of its half.
+// `partner`; `s` comes with the sign of its half.  Neighbouring pairs: c is (cos, cos), s is (-sin, sin).
 template <bool BF16, bool INTER>
 struct Turn {
-    float c[INTER ? 4 : 8], s[INTER ? 4 : 8];
+    F2 c[4], s[4];
     int partner;
     bool on;
     // `table`: cos and sin of the thread's token, pair by pair
@@ -54,14 +77,22 @@ struct Turn {
         if (!on) return;
         if constexpr (INTER) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) { c[e] = table[lane * 4 + e].x; s[e] = table[lane * 4 + e].y; }
+            for (int e = 0; e < 4; e++) {
+                const float2 cs = table[lane * 4 + e];
+                c[e] = F2(cs.x, cs.x);
+                s[e] = F2(-cs.y, cs.y);
+            }
         } else {
             const int half = dim / 16;                     // lanes of the first halves
             const bool second = lane >= half;
             partner = second ? lane - half : lane + half;
             const int p = (second ? lane - half : lane) * 8;
 #pragma unroll
-            for (int e = 0; e < 8; e++) { c[e] = table[p + e].x; s[e] = second ? table[p + e].y : -table[p + e].y; }
+            for (int e = 0; e < 4; e++) {
+                const float2 a = table[p + 2 * e], b = table[p + 2 * e + 1];
+                c[e] = F2(a.x, b.x);
+                s[e] = second ? F2(a.y, b.y) : F2(-a.y, -b.y);
+            }
         }
     }
     // All lanes of the warp call this.  Products and sums are rounded one by one, so that a value is the same
@@ -70,21 +101,13 @@ struct Turn {
     __device__ __forceinline__ uint4 apply(const uint4& x) const {
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
         uint32_t y[4];
-        if constexpr (INTER) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 a = unpack16<BF16>(w[i]);
-                y[i] = pack16<BF16>(__fsub_rn(__fmul_rn(a.x, c[i]), __fmul_rn(a.y, s[i])),
-                                    __fadd_rn(__fmul_rn(a.y, c[i]), __fmul_rn(a.x, s[i])));
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t pw = __shfl_sync(0xffffffffu, w[i], partner, LPR);
-                const float2 a = unpack16<BF16>(w[i]), p = unpack16<BF16>(pw);
-                y[i] = pack16<BF16>(__fadd_rn(__fmul_rn(a.x, c[2 * i]), __fmul_rn(p.x, s[2 * i])),
-                                    __fadd_rn(__fmul_rn(a.y, c[2 * i + 1]), __fmul_rn(p.y, s[2 * i + 1])));
-            }
+        for (int i = 0; i < 4; i++) {
+            const float2 f = unpack16<BF16>(w[i]);
+            float2 r;
+            if constexpr (INTER) r = (F2(f) * c[i] + F2(f.y, f.x) * s[i]).get();
+            else r = (F2(f) * c[i] + F2(unpack16<BF16>(__shfl_sync(0xffffffffu, w[i], partner, LPR))) * s[i]).get();
+            y[i] = pack16<BF16>(r.x, r.y);
         }
         return on ? make_uint4(y[0], y[1], y[2], y[3]) : x;
     }
@@ -202,9 +225,9 @@ __device__ __forceinline__ uint32_t e4m3x4(float2 a, float2 b) {
 // 8 elements as e4m3 codes of value * inv.
 template <bool BF16>
 __device__ __forceinline__ uint2 to_e4m3(const uint4& x, float inv) {
-    const float2 a = unpack16<BF16>(x.x), b = unpack16<BF16>(x.y), c = unpack16<BF16>(x.z), d = unpack16<BF16>(x.w);
-    return make_uint2(e4m3x4(make_float2(a.x * inv, a.y * inv), make_float2(b.x * inv, b.y * inv)),
-                      e4m3x4(make_float2(c.x * inv, c.y * inv), make_float2(d.x * inv, d.y * inv)));
+    const F2 i(inv, inv);
+    return make_uint2(e4m3x4((F2(unpack16<BF16>(x.x)) * i).get(), (F2(unpack16<BF16>(x.y)) * i).get()),
+                      e4m3x4((F2(unpack16<BF16>(x.z)) * i).get(), (F2(unpack16<BF16>(x.w)) * i).get()));
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
@@ -242,104 +265,130 @@ __device__ __forceinline__ uint32_t to_u4(const uint4& x, __half2* param) {
     // strings the codes together, with the constant's share taken off at the end
     constexpr float kRound = 12582912.0f;
     constexpr uint32_t kBits = 0x4B400000u;
+    const F2 minus_z(-z, -z), inv2(inv, inv), round2(kRound, kRound);
     uint32_t codes = 0;
 #pragma unroll
-    for (int i = 7; i >= 0; i--) {
-        const float2 f = unpack16<BF16>(w[i / 2]);
-        const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(i & 1 ? f.y : f.x, z), inv), 0.0f), 15.0f);
-        codes = codes * 16u + __float_as_uint(__fadd_rn(c, kRound));
+    for (int i = 3; i >= 0; i--) {
+        const float2 c = ((F2(unpack16<BF16>(w[i])) + minus_z) * inv2).get();
+        const float2 r = (F2(fminf(fmaxf(c.x, 0.0f), 15.0f), fminf(fmaxf(c.y, 0.0f), 15.0f)) + round2).get();
+        codes = (codes * 16u + __float_as_uint(r.y)) * 16u + __float_as_uint(r.x);
     }
     constexpr uint32_t kShare = kBits * 0x11111111u;
     *param = __halves2half2(s16, z16);
     return codes - kShare;
 }
 
-// kUnroll heads of a token and every `step`-th after, from `src` (the lane's part of head 0): loads all before it uses one.
-// `use(h, x)` is called by whole warps, with zeros where there is no head.
-template <int D, class Use>
-__device__ __forceinline__ void walk_heads(const uint16_t* src, int first, int end, int step, bool live, Use use) {
-    for (int h0 = first; __any_sync(0xffffffffu, h0 < end); h0 += step * kUnroll) {
-        uint4 x[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; u++) {
-            x[u] = make_uint4(0, 0, 0, 0);
-            if (live && h0 + u * step < end) x[u] = ld_row_16(src + (h0 + u * step) * D);
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; u++) use(h0 + u * step, x[u]);
-    }
-}
-
+// A thread keeps to one token and walks its heads, those of q, then k, then v, kAppendUnroll at a time; the next ones are
+// loaded before these are used, the first ones before the block computes its cos and sin.  What bounds it is the chain
+// of loads that a block waits for, one after the other (lengths, page, rows), and then the 150 instructions that 16 bytes of a
+// row cost: small blocks of few tokens, 8 of them an SM (512 tokens to 8 sequences, Hq=32 Hkv=8 D=128, e4m3 / 4-bit with its read
+// back, us in a graph: 256 threads and 8 tokens 22.7 / 29.9, 128 and 2 20.0 / 26.6; one token to 16 sequences 3.3, 2.8).
+constexpr int kAppendThreads = 128, kAppendTokens = 2, kAppendUnroll = 2;
 template <int D, bool BF16, bool INTER, int CACHE>
-__global__ void __launch_bounds__(kThreads, 4) append_kernel(const __grid_constant__ AppendArgs a) {
-    constexpr int LPR = D / 8, SLOTS = kThreads / LPR;
+__global__ void __launch_bounds__(kAppendThreads, 8) append_kernel(const __grid_constant__ AppendArgs a) {
+    constexpr int LPR = D / 8, SLOTS = kAppendThreads / LPR, U = kAppendUnroll;
     extern __shared__ float2 table[];                       // [tokens][dim / 2]
-    const int split = (int)blockIdx.x - a.by_splits.quot(blockIdx.x) * a.splits, n0 = a.by_splits.quot(blockIdx.x) * a.tokens;
-    const int pairs = a.rot.dim / 2;
+    const int tile = a.by_splits.quot(blockIdx.x), split = (int)blockIdx.x - tile * a.splits, n0 = tile * a.tokens;
+    const int pairs = a.rot.dim / 2, hqk = a.hq + a.hkv, heads = hqk + a.hkv;
+    const int per = (heads + a.splits - 1) / a.splits, h_begin = split * per, h_end = min(heads, h_begin + per);
+    const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR;
+    const int t = slot & (a.tokens - 1), step = SLOTS / a.tokens, mine = slot / a.tokens, n = n0 + t;
     grid_dependency_wait();
     grid_launch_dependents();
-    const int heads = a.hq + 2 * a.hkv, per = (heads + a.splits - 1) / a.splits;
-    const int h_begin = split * per, h_end = min(heads, h_begin + per);
-    if (h_begin < a.hq + a.hkv)                             // not v alone
-        for (int i = threadIdx.x; i < a.tokens * pairs; i += kThreads) {
-            const int t = a.by_pairs.quot(i);
-            float2 cs;
-            cos_sin(a.rot, token(a, min(n0 + t, a.n_all - 1)).position, i - t * pairs, false, &cs.x, &cs.y);
-            table[i] = cs;
-        }
-    __syncthreads();
-    const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR;
-    const int t = slot & (a.tokens - 1), step = SLOTS / a.tokens, mine = slot / a.tokens;
-    const int n = n0 + t;
     const bool in = n < a.n_all;
     const Token tk = token(a, min(n, a.n_all - 1));
     const bool live = in && tk.live;
+
+    // groups of heads of one kind: 0 q, 1 k, 2 v, [h0, end) of that kind left
+    struct Group {
+        int kind, h0, end;
+    };
+    auto begin_kind = [&](int kind) {
+        Group g;
+        do {
+            const int base = kind == 0 ? 0 : kind == 1 ? a.hq : hqk;
+            g.kind = kind;
+            g.h0 = max(h_begin - base, 0);
+            g.end = min(h_end - base, kind == 0 ? a.hq : a.hkv);
+        } while (g.h0 >= g.end && ++kind < 3);
+        g.kind = kind;
+        return g;
+    };
+    auto load = [&](const Group& g, uint4 (&x)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; u++) x[u] = make_uint4(0, 0, 0, 0);
+        if (g.kind > 2 || !live) return;
+        const uint16_t* p = (g.kind == 0 ? a.q + n * a.q_stride : g.kind == 1 ? a.k + n * a.k_stride : a.v + n * a.v_stride) + (g.h0 + mine) * D + lane * 8;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (g.h0 + mine + u * step < g.end) x[u] = ld_row_16(p + u * step * D);
+    };
+    Group g = begin_kind(0);
+    uint4 x[U];
+    load(g, x);
+    if (h_begin < hqk)                                      // not v alone
+        for (int i = threadIdx.x; i < a.tokens * pairs; i += kAppendThreads) {
+            const int ti = a.by_pairs.quot(i);
+            float2 cs;
+            cos_sin(a.rot, token(a, min(n0 + ti, a.n_all - 1)).position, i - ti * pairs, false, &cs.x, &cs.y);
+            table[i] = cs;
+        }
     CacheRow at = {-1, 0};
     if (live) at = cache_row(a.map, tk.b, tk.row);
+    __syncthreads();
     Turn<BF16, INTER> turn;
     turn.template load<LPR>(table + t * pairs, lane, a.rot.dim);
-
-    // q
-    if (h_begin < a.hq) {
-        const long long o = (long long)n * a.hq * D + lane * 8;
-        const int end = min(h_end, a.hq);
-        walk_heads<D>(a.q + n * a.q_stride + lane * 8, h_begin + mine, end, step, live, [&](int h, const uint4& x) {
-            const uint4 y = turn.template apply<LPR>(x);
-            if (h >= end || !in) return;
-            if constexpr (CACHE == FA_CACHE_E4M3) {
-                const float inv = live ? __frcp_rn(a.q_scale[tk.b * a.hkv + a.by_group.quot(h)]) : 0.0f;
-                *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.q_out) + o + h * D) = live ? to_e4m3<BF16>(y, inv) : make_uint2(0, 0);
-            } else {
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.q_out) + o + h * D) = live ? y : make_uint4(0, 0, 0, 0);    // turned zeros may be -0
-            }
-        });
-    }
-    // k and v into the cache: `in_cache` for this thread's rows, `pairs` for their scale and offset
     const bool store = live && at.block >= 0;
-    const long long row = at.block * a.block_stride + at.in_block * a.row_stride + lane * (CACHE == FA_CACHE_U4 ? 4 : CACHE == FA_CACHE_E4M3 ? 8 : 16);
+    constexpr int kLaneBytes = CACHE == FA_CACHE_U4 ? 4 : CACHE == FA_CACHE_E4M3 ? 8 : 16;
+    const long long row = at.block * a.block_stride + at.in_block * a.row_stride + lane * kLaneBytes;
     const long long prow = CACHE == FA_CACHE_U4 ? at.block * a.p_block_stride + at.in_block * a.p_row_stride + lane / 8 : 0;
-    auto put = [&](uint8_t* cache, __half2* params, const float* scale, int end, int h, const uint4& y) {
-        uint8_t* p = cache + row + h * a.head_stride;
-        if constexpr (CACHE == FA_CACHE_U4) {
-            __half2 param;
-            const uint32_t codes = to_u4<BF16>(y, &param);
-            if (!store || h >= end) return;
-            *reinterpret_cast<uint32_t*>(p) = codes;
-            if ((lane & 7) == 0) params[prow + h * a.p_head_stride] = param;
-        } else if (store && h < end) {
-            if constexpr (CACHE == FA_CACHE_E4M3) *reinterpret_cast<uint2*>(p) = to_e4m3<BF16>(y, __frcp_rn(scale[tk.b * a.hkv + h]));
-            else *reinterpret_cast<uint4*>(p) = y;
+
+    while (g.kind <= 2) {
+        Group next = g;
+        next.h0 += step * U;
+        if (next.h0 >= next.end) next = begin_kind(g.kind + 1);
+        uint4 x_next[U];
+        load(next, x_next);
+        if (g.kind == 0) {
+            uint8_t* p = static_cast<uint8_t*>(a.q_out) + (((long long)n * a.hq + g.h0 + mine) * D + lane * 8) * (CACHE == FA_CACHE_E4M3 ? 1 : 2);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const uint4 y = turn.template apply<LPR>(x[u]);
+                const int h = g.h0 + mine + u * step;
+                if (h < g.end && in) {
+                    if constexpr (CACHE == FA_CACHE_E4M3) {
+                        *reinterpret_cast<uint2*>(p + u * step * D) = live ? to_e4m3<BF16>(y, __frcp_rn(a.q_scale[tk.b * a.hkv + a.by_group.quot(h)])) : make_uint2(0, 0);
+                    } else {
+                        *reinterpret_cast<uint4*>(p + u * step * D * 2) = live ? y : make_uint4(0, 0, 0, 0);    // turned zeros may be -0
+                    }
+                }
+            }
+        } else {
+            uint8_t* cache = (g.kind == 2 ? a.v_cache : a.k_cache) + row;
+            [[maybe_unused]] __half2* params = (g.kind == 2 ? a.v_params : a.k_params) + prow;
+            [[maybe_unused]] const float* scale = (g.kind == 2 ? a.v_scale : a.k_scale) + tk.b * a.hkv;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                uint4 y = x[u];
+                if (g.kind == 1) y = turn.template apply<LPR>(y);
+                const int h = g.h0 + mine + u * step;
+                const bool put = store && h < g.end;
+                if constexpr (CACHE == FA_CACHE_U4) {
+                    __half2 param;
+                    const uint32_t codes = to_u4<BF16>(y, &param);           // lanes of a row agree on `put`; all take part
+                    if (put) {
+                        *reinterpret_cast<uint32_t*>(cache + h * a.head_stride) = codes;
+                        if ((lane & 7) == 0) params[h * a.p_head_stride] = param;
+                    }
+                } else if (put) {
+                    if constexpr (CACHE == FA_CACHE_E4M3) *reinterpret_cast<uint2*>(cache + h * a.head_stride) = to_e4m3<BF16>(y, __frcp_rn(scale[h]));
+                    else *reinterpret_cast<uint4*>(cache + h * a.head_stride) = y;
+                }
+            }
         }
-    };
-    if (h_begin < a.hq + a.hkv && h_end > a.hq) {
-        const int first = max(h_begin - a.hq, 0), end = min(h_end - a.hq, a.hkv);
-        walk_heads<D>(a.k + n * a.k_stride + lane * 8, first + mine, end, step, live,
-                      [&](int h, const uint4& x) { put(a.k_cache, a.k_params, a.k_scale, end, h, turn.template apply<LPR>(x)); });
-    }
-    if (h_end > a.hq + a.hkv) {
-        const int first = max(h_begin - a.hq - a.hkv, 0), end = h_end - a.hq - a.hkv;
-        walk_heads<D>(a.v + n * a.v_stride + lane * 8, first + mine, end, step, live,
-                      [&](int h, const uint4& x) { put(a.v_cache, a.v_params, a.v_scale, end, h, x); });
+        g = next;
+#pragma unroll
+        for (int u = 0; u < U; u++) x[u] = x_next[u];
     }
 }
 
@@ -459,7 +508,7 @@ int run_rope(const RopeArgs& a, unsigned blocks, cudaStream_t stream) {
 }
 template <int D, bool BF16, bool INTER, int CACHE>
 int run_append(const AppendArgs& a, unsigned blocks, cudaStream_t stream) {
-    return launch_dependent(append_kernel<D, BF16, INTER, CACHE>, blocks, kThreads, (size_t)a.tokens * (a.rot.dim / 2) * sizeof(float2), stream, 1, a);
+    return launch_dependent(append_kernel<D, BF16, INTER, CACHE>, blocks, kAppendThreads, (size_t)a.tokens * (a.rot.dim / 2) * sizeof(float2), stream, 1, a);
 }
 template <int D, bool BF16, bool INTER>
 int run_append_to(const AppendArgs& a, int cache, unsigned blocks, cudaStream_t stream) {
@@ -621,9 +670,9 @@ FA_EXPORT int fa_cache_append(const fa_cache_append_args* p) {
     a.n_tokens = p->num_tokens;
     a.n_all = (int)n_all;
     a.seq_len_kv = p->seq_len_kv;
-    a.tokens = pow2_at_least((int)((n_all + 2 * st->sm_count - 1) / (2 * st->sm_count)), 8);
+    a.tokens = pow2_at_least((int)((n_all + 2 * st->sm_count - 1) / (2 * st->sm_count)), kAppendTokens);
     const long long tiles = (n_all + a.tokens - 1) / a.tokens;
-    a.splits = head_splits(tiles, heads, kThreads / (p->d_head / 8) / a.tokens, st->sm_count);
+    a.splits = head_splits(tiles, heads, kAppendThreads / (p->d_head / 8) / a.tokens, st->sm_count);
     a.block_stride = p->layout.block_stride * unit;
     a.head_stride = p->layout.head_stride * unit;
     a.row_stride = p->layout.row_stride * unit;
