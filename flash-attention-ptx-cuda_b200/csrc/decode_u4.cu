@@ -85,6 +85,8 @@ struct Shape {
     static constexpr int FactorBytes = Keys * G * 16;         // of a tile: for each key K's (scale, offset) and V's, unpacked
     static constexpr int WarpBytes = Stages * StageBytes + FactorBytes;
     static constexpr int Rows = 8 * NT;
+    // the rings, aligned, and a cluster's rows: from each of its CTAs up to Rows / size of them (rounded up), O [D], max, sum
+    static constexpr int SmemBytes = 1024 + kWarps * WarpBytes + (Rows + kMaxCluster - 1) * (D + 4) * 4;
     static constexpr int Record = Rows * (D + 2);              // floats: O [row][D], then m [row], l [row]
     static_assert(Record * 4 <= WarpBytes, "a record fits the ring it replaces");
 };
@@ -176,29 +178,25 @@ __device__ __forceinline__ uint32_t code16(uint32_t x) {
 template <int D>
 __device__ __forceinline__ int piece(int r, int c) { return D == 128 ? c ^ ((r >> 1) & 3) : c ^ ((r >> 2) & 1); }
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// What CTA `rank` of the cluster has at this CTA's shared address `p`.
-__device__ __forceinline__ uint32_t cluster_address(const float* p, int rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ float ld_cluster(const float* p, int rank) {
-    float x;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(cluster_address(p, rank)) : "memory");
-    return x;
-}
-__device__ __forceinline__ float4 ld_cluster4(const float* p, int rank) {
-    float4 x;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(cluster_address(p, rank)) : "memory");
-    return x;
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Four floats to where CTA `rank` of the cluster has this CTA's shared address `p`.
+__device__ __forceinline__ void st_cluster4(const float* p, int rank, const float4& x) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w) : "memory");
 }
 
 // Weight of a record (its max in powers of two, its sum) in a merge with maximum `mx`: none if it is empty; a NaN sum without a
 // max is kept.
 __device__ __forceinline__ float record_weight(float m, float l, float mx) { return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : ex2(m - mx); }
+
+__device__ __forceinline__ void add_record(float4& f, float& sum, float m, float l, float mx, const float* o) {
+    const float w = record_weight(m, l, mx);
+    const float4 z = *reinterpret_cast<const float4*>(o);
+    sum = fmaf(w, l, sum);
+    f.x = fmaf(w, z.x, f.x); f.y = fmaf(w, z.y, f.y); f.z = fmaf(w, z.z, f.z); f.w = fmaf(w, z.w, f.w);
+}
 
 // Four elements of an output row from its sums, and the row's LSE with the first of them.
 template <int D, bool BF16>
@@ -225,7 +223,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
     __shared__ int s_abort, s_never;
     __shared__ int s_prefix[kWarps * 32], s_warp[kWarps];      // tiles (of one head and row block) before a thread's sequences
     __shared__ int s_item[kRecords], s_before[kWarps], s_after[kWarps];
-    __shared__ float s_m[kRecords][S::Rows], s_l[kRecords][S::Rows], s_w[kRecords][S::Rows];
+    __shared__ float s_m[kRecords][S::Rows], s_l[kRecords][S::Rows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     if (tid == 0) {
         prefetch_tensormap(&a.tk);
@@ -235,6 +233,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
         fence_mbar_init();
     }
     const WaitCtl ctl{&s_abort, a.status};
+    if (a.cluster > 1) cluster_arrive();                       // waited for before the first access to another CTA
     grid_dependency_wait();
     grid_launch_dependents();
 
@@ -345,73 +344,73 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
 #pragma unroll
     for (int c = 0; c < P / 2; c++) m_at[c] = ring + m_row * S::RowBytes + piece<D>(m_row, 2 * c + (lane >> 4)) * 16;
 
+    // ---- loads: of the item `ld`, which the warp works on or is about to begin
+    Item ld = it;
+    auto page_of = [&](int key) -> int {                       // -1: names none, or past the end
+        if (key >= ld.len) return -1;
+        if (a.map.page_shift < 0) return ld.b;
+        const int p = a.map.block_table[(long long)ld.b * a.map.table_stride + (key >> a.map.page_shift)];
+        return (unsigned)p < (unsigned)a.map.n_pages ? p : -1;
+    };
+    // pages of a tile's boxes, one a lane
+    auto pages_of = [&](int tile) { return lane < boxes ? page_of(tile * S::Keys + (lane << box_shift)) : -1; };
+    auto load_codes = [&](int tile, int pages) {
+        const int k0 = tile * S::Keys;
+        const uint32_t dst = ring + load_stage * S::StageBytes, bar = full0 + load_stage * 8;
+        load_stage = load_stage + 1 == S::Stages ? 0 : load_stage + 1;
+        in_flight++;
+        if (boxes == 1) {
+            const int p = __shfl_sync(0xffffffffu, pages, 0);
+            if (elect_one()) {
+                // rows past the block and pages that name none read as zero; rows past the sequence's end hold any codes, and are masked
+                mbar_arrive_expect_tx(bar, 2 * S::CodeBytes);
+                tma_load_4d(dst, &a.tk, bar, 0, k0 & in_page, ld.h, p);
+                tma_load_4d(dst + S::CodeBytes, &a.tv, bar, 0, k0 & in_page, ld.h, p);
+            }
+        } else {
+            if (elect_one()) mbar_arrive_expect_tx(bar, 2 * S::CodeBytes);
+            __syncwarp();
+            if (lane < boxes) {
+                const uint32_t at = dst + (lane << box_shift) * S::RowBytes;
+                const int row = (k0 + (lane << box_shift)) & in_page;
+                tma_load_4d(at, &a.tk, bar, 0, row, ld.h, pages);
+                tma_load_4d(at + S::CodeBytes, &a.tv, bar, 0, row, ld.h, pages);
+            }
+            __syncwarp();
+        }
+    };
+    constexpr int KPL = S::Keys / 32;                          // keys of a lane
+    uint32_t kraw[KPL][G], vraw[KPL][G];
+    auto load_pairs = [&](int tile, int pages) {
+#pragma unroll
+        for (int i = 0; i < KPL; i++) {
+            const int key = tile * S::Keys + i * 32 + lane, p = __shfl_sync(0xffffffffu, pages, (i * 32 + lane) >> box_shift);
+#pragma unroll
+            for (int gi = 0; gi < G; gi++) kraw[i][gi] = vraw[i][gi] = 0;
+            if (key < ld.len && p >= 0) {
+                const long long off = p * a.p_block_stride + (long long)ld.h * a.p_head_stride + (long long)(key & in_page) * a.p_row_stride;
+                ldg_pairs<G>(a.kp + off, kraw[i]);
+                ldg_pairs<G>(a.vp + off, vraw[i]);
+            }
+        }
+    };
+    int ahead = -1, next_pages = -1;                           // pages of the tile whose pairs are loaded next, and of the one whose codes are
+    static_assert(S::Stages == 3, "two tiles of codes are under way, and one of pairs");
+    auto start = [&](int tile0, int tile1) {                   // the look-ups first, so that they wait together
+        const int pages = pages_of(tile0);
+        ahead = tile0 + 1 < tile1 ? pages_of(tile0 + 1) : -1;
+        next_pages = tile0 + 2 < tile1 ? pages_of(tile0 + 2) : -1;
+        load_pairs(tile0, pages);
+        load_codes(tile0, pages);
+        if (tile0 + 1 < tile1) load_codes(tile0 + 1, ahead);
+    };
+    if (w_begin < w_end) start(w_begin - item_start, min(it.tiles, w_end - item_start));
+
     // ---- item by item
     for (int x = w_begin; x < w_end && alive;) {
         const int tile0 = x - item_start, tile1 = min(it.tiles, tile0 + w_end - x);
         const int row0 = it.rb * S::Rows;
 
-        // ---- loads of a tile
-        const long long hp_off = (long long)it.h * a.p_head_stride;
-        auto page_of = [&](int key) -> int {                   // -1: names none, or past the end
-            if (key >= it.len) return -1;
-            if (a.map.page_shift < 0) return it.b;
-            const int p = a.map.block_table[(long long)it.b * a.map.table_stride + (key >> a.map.page_shift)];
-            return (unsigned)p < (unsigned)a.map.n_pages ? p : -1;
-        };
-        // pages of a tile's boxes, one a lane
-        auto pages_of = [&](int tile) { return lane < boxes ? page_of(tile * S::Keys + (lane << box_shift)) : -1; };
-        auto load_codes = [&](int tile, int pages) {
-            const int k0 = tile * S::Keys;
-            const uint32_t dst = ring + load_stage * S::StageBytes, bar = full0 + load_stage * 8;
-            load_stage = load_stage + 1 == S::Stages ? 0 : load_stage + 1;
-            in_flight++;
-            if (boxes == 1) {
-                const int p = __shfl_sync(0xffffffffu, pages, 0);
-                if (elect_one()) {
-                    // rows past the block and pages that name none read as zero; rows past the sequence's end hold any codes, and are masked
-                    mbar_arrive_expect_tx(bar, 2 * S::CodeBytes);
-                    tma_load_4d(dst, &a.tk, bar, 0, k0 & in_page, it.h, p);
-                    tma_load_4d(dst + S::CodeBytes, &a.tv, bar, 0, k0 & in_page, it.h, p);
-                }
-            } else {
-                if (elect_one()) mbar_arrive_expect_tx(bar, 2 * S::CodeBytes);
-                __syncwarp();
-                if (lane < boxes) {
-                    const uint32_t at = dst + (lane << box_shift) * S::RowBytes;
-                    const int row = (k0 + (lane << box_shift)) & in_page;
-                    tma_load_4d(at, &a.tk, bar, 0, row, it.h, pages);
-                    tma_load_4d(at + S::CodeBytes, &a.tv, bar, 0, row, it.h, pages);
-                }
-                __syncwarp();
-            }
-        };
-        constexpr int KPL = (S::Keys + 31) / 32;                 // keys of a lane
-        uint32_t kraw[KPL][G], vraw[KPL][G];
-        auto load_pairs = [&](int tile, int pages) {
-#pragma unroll
-            for (int i = 0; i < KPL; i++) {
-                const int key = tile * S::Keys + i * 32 + lane, p = __shfl_sync(0xffffffffu, pages, (i * 32 + lane) >> box_shift);
-#pragma unroll
-                for (int gi = 0; gi < G; gi++) kraw[i][gi] = vraw[i][gi] = 0;
-                if (key < it.len && p >= 0 && (S::Keys >= 32 || lane < S::Keys)) {
-                    const long long off = p * a.p_block_stride + hp_off + (long long)(key & in_page) * a.p_row_stride;
-                    ldg_pairs<G>(a.kp + off, kraw[i]);
-                    ldg_pairs<G>(a.vp + off, vraw[i]);
-                }
-            }
-        };
-
-        int pages = pages_of(tile0), next_pages = -1;          // of the tile whose pairs are loaded next, and of the one whose codes are
-        load_pairs(tile0, pages);
-#pragma unroll
-        for (int i = 0; i < S::Stages - 1; i++) {
-            if (tile0 + i < tile1) {
-                next_pages = i == 0 ? pages : pages_of(tile0 + i);
-                load_codes(tile0 + i, next_pages);
-            }
-        }
-        int ahead = S::Stages - 1 == 2 ? next_pages : tile0 + 1 < tile1 ? pages_of(tile0 + 1) : -1;
-        next_pages = tile0 + S::Stages - 1 < tile1 ? pages_of(tile0 + S::Stages - 1) : -1;
         // q as operand B: column g of the n-th 8 rows; 8 elements of a 16-byte piece of codes are two steps of k, in pairs
         // (i, i + 4) as the codes lie in a word.  bf16 rows are brought to fp16 by a power of two that puts their
         // largest element at 2^14: exact for elements down to 2^-28 of that one, and the rest is below its 32-bit rounding.
@@ -535,11 +534,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
             if (!alive) break;
             in_flight--;
             __syncwarp();                                      // the factors are written, and nobody reads the oldest stage any more
-            if (tile + S::Stages - 1 < tile1) load_codes(tile + S::Stages - 1, next_pages);
+            if (tile + 2 < tile1) load_codes(tile + 2, next_pages);
             if (tile + 1 < tile1) {
                 load_pairs(tile + 1, ahead);
-                ahead = S::Stages - 1 == 2 ? next_pages : tile + 2 < tile1 ? pages_of(tile + 2) : -1;
-                next_pages = tile + S::Stages < tile1 ? pages_of(tile + S::Stages) : -1;
+                ahead = next_pages;
+                next_pages = tile + 3 < tile1 ? pages_of(tile + 3) : -1;
             }
             const uint32_t at = stage * S::StageBytes;
             if (++stage == S::Stages) { stage = 0; phase ^= 1; }
@@ -681,10 +680,25 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
         }
         __syncwarp();
 
+        // ---- the next item's first loads, before this one's sums are written
+        const int x_next = x + tile1 - tile0, start_next = item_start + it.tiles;
+        const bool last = x_next >= w_end;
+        if (!last && alive) {
+            if (++ld.rb == a.row_blocks) {
+                ld.rb = 0;
+                if (++ld.h == a.hkv) {
+                    ld.h = 0;
+                    ld.b++;
+                    ld.len = sequence_length(a.seq_lens, ld.b, a.kv_len);
+                    ld.tiles = tiles_of<S::Keys>(ld.len);
+                }
+            }
+            start(0, min(ld.tiles, w_end - x_next));
+        }
+
         // ---- the item's sums, or this warp's part of them
         const float up = s_down == 0.0f ? 0.0f : 1.0f / s_down;
         const bool whole = tile0 == 0 && tile1 == it.tiles && a.cluster <= 1;     // a cluster's result is its last step's
-        const bool last = x + tile1 - tile0 >= w_end;
         const int item = (it.b * a.hkv + it.h) * a.row_blocks + it.rb;
         float* record = last ? tail_record : head_record;
         if (!whole) {
@@ -723,20 +737,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
                     s_l[2 * warp + last][r] = l[n][c];
                 }
             }
-        // ---- the next item
-        x += tile1 - tile0;
-        item_start += it.tiles;
-        if (x < w_end) {
-            if (++it.rb == a.row_blocks) {
-                it.rb = 0;
-                if (++it.h == a.hkv) {
-                    it.h = 0;
-                    it.b++;
-                    it.len = sequence_length(a.seq_lens, it.b, a.kv_len);
-                    it.tiles = tiles_of<S::Keys>(it.len);
-                }
-            }
-        }
+        x = x_next;
+        item_start = start_next;
+        it = ld;
     }
 
     // ---- the CTA's records
@@ -748,104 +751,90 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
     }
     __threadfence_block();
     __syncthreads();
-    for (int i = tid; i < kRecords * S::Rows; i += kWarps * 32) {          // each one's weight in its item
-        const int y = i / S::Rows, r = i % S::Rows, item = s_item[y];
-        if (item >= 0) {
-            float mx = -INFINITY;
+    constexpr int kQuads = S::Rows * (D / 4);                  // four elements of a row
+    if (a.cluster > 0) {
+        // all of one item, a warp's (it has none if it had no tile, or wrote the whole item)
+        const int cl = a.cluster, per_rank = a.by_cluster.quot(S::Rows + cl - 1);       // rows of a CTA
+        if (cl > 1) cluster_wait();                            // the others run: their shared memory may be written
+        for (int i = tid; i < kQuads; i += kWarps * 32) {
+            const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+            float mx = -INFINITY, sum = 0.0f;
+            bool any = false;
 #pragma unroll
-            for (int z = 0; z < kRecords; z++)
-                if (s_item[z] == item) mx = fmaxf(mx, s_m[z][r]);
-            s_w[y][r] = record_weight(s_m[y][r], s_l[y][r], mx);
+            for (int w = 0; w < kWarps; w++)
+                if (s_item[2 * w + 1] >= 0) { mx = fmaxf(mx, s_m[2 * w + 1][r]); any = true; }
+            float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kWarps; w++)
+                if (s_item[2 * w + 1] >= 0)
+                    add_record(f, sum, s_m[2 * w + 1][r], s_l[2 * w + 1][r], mx, reinterpret_cast<const float*>(smem + w * S::WarpBytes) + r * D + d);
+            if (cl > 1) {
+                // row r is CTA (r % cl)'s: into its shared memory, where it waits for those of the others
+                const int owner = r - a.by_cluster.quot(r) * cl;
+                const float* to = reinterpret_cast<const float*>(smem + kWarps * S::WarpBytes) + (rank * per_rank + a.by_cluster.quot(r)) * (D + 4);
+                st_cluster4(to + d, owner, f);
+                if (d == 0) st_cluster4(to + D, owner, make_float4(mx, sum, 0.0f, 0.0f));
+            } else if (any && it.rb * S::Rows + r < a.rows) {
+                store_quad<D, BF16>(a, out_row(a, it.b, it.h, it.rb * S::Rows + r), d, f, mx, sum);
+            }
         }
+        if (cl > 1) {
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();
+            const float* from = reinterpret_cast<const float*>(smem + kWarps * S::WarpBytes);
+            for (int i = tid; i < kQuads; i += kWarps * 32) {
+                const int y = i / (D / 4), d = (i % (D / 4)) * 4, r = y * cl + rank;
+                if (r >= S::Rows || it.rb * S::Rows + r >= a.rows) break;
+                float mx = -INFINITY, sum = 0.0f;
+                float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int c = 0; c < cl; c++) mx = fmaxf(mx, from[(c * per_rank + y) * (D + 4) + D]);
+                for (int c = 0; c < cl; c++) {
+                    const float* rec = from + (c * per_rank + y) * (D + 4);
+                    add_record(f, sum, rec[D], rec[D + 1], mx, rec + d);
+                }
+                store_quad<D, BF16>(a, out_row(a, it.b, it.h, it.rb * S::Rows + r), d, f, mx, sum);
+            }
+        }
+        return;
     }
-    __syncthreads();
+    // items of the line: the records of each are members of a mask, and their loads wait together
+    const int my_item = lane < kRecords ? s_item[lane] : -1;
     int2 carried = make_int2(-1, 0);
-    constexpr int kQuads = S::Rows * (D / 4), kEach = (kQuads + kWarps * 32 - 1) / (kWarps * 32);
-    float4 mine[kEach];                                        // cluster: the CTA's sums
-    float mine_m[kEach], mine_l[kEach];
-#pragma unroll
-    for (int j = 0; j < kEach; j++) { mine[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f); mine_m[j] = -INFINITY; mine_l[j] = 0.0f; }
-    for (int k = 0; k < kRecords;) {
-        const int item = s_item[k];
-        if (item < 0) { k++; continue; }
-        int end = k + 1;                                       // records of this item: k .. end - 1, with gaps
-        for (int i = k + 1; i < kRecords; i++) {
-            const int y = s_item[i];
-            if (y == item) end = i + 1;
-            else if (y >= 0) break;
-        }
+    for (unsigned left = __ballot_sync(0xffffffffu, my_item >= 0); left != 0;) {
+        const int k = __ffs(left) - 1, item = __shfl_sync(0xffffffffu, my_item, k);
+        const unsigned members = __ballot_sync(0xffffffffu, my_item == item);
+        left &= ~members;
         // it begins before this CTA's part if its first warp says so and this is that warp's first record, and ends after it likewise
-        const int w0 = k >> 1, w1 = (end - 1) >> 1;
+        const int w0 = k >> 1, w1 = (31 - __clz(members)) >> 1;
         const bool starts_before = s_before[w0] != 0 && item == (s_item[2 * w0] >= 0 ? s_item[2 * w0] : s_item[2 * w0 + 1]);
         const bool ends_after = s_after[w1] != 0 && item == (s_item[2 * w1 + 1] >= 0 ? s_item[2 * w1 + 1] : s_item[2 * w1]);
         float* slot = a.scratch + ((size_t)gridDim.x * kWarps + 2 * blockIdx.x + (starts_before ? 0 : 1)) * S::Record;
         const int bh = a.by_row_blocks.quot(item), rb = item - bh * a.row_blocks, b = a.by_hkv.quot(bh), h = bh - b * a.hkv;
-        if (ends_after && !starts_before && a.cluster == 0) carried = make_int2(item, (s_after[w1] - 1) / chunk + 1);
-#pragma unroll
-        for (int j = 0; j < kEach; j++) {
-            const int i = tid + j * kWarps * 32;
-            if (i >= kQuads) break;
+        if (ends_after && !starts_before) carried = make_int2(item, (s_after[w1] - 1) / chunk + 1);
+        for (int i = tid; i < kQuads; i += kWarps * 32) {
             const int r = i / (D / 4), d = (i % (D / 4)) * 4;
             float mx = -INFINITY, sum = 0.0f;
             float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int y = k; y < end; y++)
-                if (s_item[y] == item) {
-                    const float* rec = y & 1 ? reinterpret_cast<const float*>(smem + (y >> 1) * S::WarpBytes) : a.scratch + (size_t)(blockIdx.x * kWarps + (y >> 1)) * S::Record;
-                    const float w = s_w[y][r];
-                    const float4 z = *reinterpret_cast<const float4*>(rec + r * D + d);
-                    mx = fmaxf(mx, s_m[y][r]);
-                    sum = fmaf(w, s_l[y][r], sum);
-                    f.x = fmaf(w, z.x, f.x); f.y = fmaf(w, z.y, f.y); f.z = fmaf(w, z.z, f.z); f.w = fmaf(w, z.w, f.w);
-                }
-            if (a.cluster > 1) {
-                mine[j] = f; mine_m[j] = mx; mine_l[j] = sum;
-            } else if (starts_before || ends_after) {
+#pragma unroll
+            for (int y = 0; y < kRecords; y++)
+                if (members >> y & 1) mx = fmaxf(mx, s_m[y][r]);
+#pragma unroll
+            for (int y = 1; y < kRecords; y += 2)              // a warp's last item: in its ring
+                if (members >> y & 1) add_record(f, sum, s_m[y][r], s_l[y][r], mx, reinterpret_cast<const float*>(smem + (y >> 1) * S::WarpBytes) + r * D + d);
+            if (members & 0x55555555u)
+#pragma unroll
+                for (int y = 0; y < kRecords; y += 2)          // its first: in the workspace
+                    if (members >> y & 1) add_record(f, sum, s_m[y][r], s_l[y][r], mx, a.scratch + (size_t)(blockIdx.x * kWarps + (y >> 1)) * S::Record + r * D + d);
+            if (starts_before || ends_after) {
                 *reinterpret_cast<float4*>(slot + r * D + d) = f;
                 if (d == 0) { slot[S::Rows * D + r] = mx; slot[S::Rows * (D + 1) + r] = sum; }
             } else if (rb * S::Rows + r < a.rows) {
                 store_quad<D, BF16>(a, out_row(a, b, h, rb * S::Rows + r), d, f, mx, sum);
             }
         }
-        k = end;
     }
-    if (a.cluster == 0) {
-        if (tid == 0) a.meta[blockIdx.x] = carried;
-    } else if (a.cluster > 1) {
-        // ---- the item's CTAs: each leaves its sums in its shared memory, the first ones read them all
-        __syncthreads();                                       // the records have been read
-        float* rec = reinterpret_cast<float*>(smem);
-#pragma unroll
-        for (int j = 0; j < kEach; j++) {
-            const int i = tid + j * kWarps * 32;
-            if (i >= kQuads) break;
-            *reinterpret_cast<float4*>(rec + i * 4) = mine[j];
-            if (i % (D / 4) == 0) { rec[S::Rows * D + i / (D / 4)] = mine_m[j]; rec[S::Rows * (D + 1) + i / (D / 4)] = mine_l[j]; }
-        }
-        cluster_sync();
-        for (int i = rank * kWarps * 32 + tid; i < kQuads; i += a.cluster * kWarps * 32) {
-            const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-            if (it.rb * S::Rows + r >= a.rows) break;
-            float cm[kMaxCluster], cl[kMaxCluster], mx = -INFINITY, sum = 0.0f;
-            float4 cz[kMaxCluster], f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int c = 0; c < kMaxCluster; c++)
-                if (c < a.cluster) {
-                    cm[c] = ld_cluster(rec + S::Rows * D + r, c);
-                    cl[c] = ld_cluster(rec + S::Rows * (D + 1) + r, c);
-                    cz[c] = ld_cluster4(rec + i * 4, c);
-                    mx = fmaxf(mx, cm[c]);
-                }
-#pragma unroll
-            for (int c = 0; c < kMaxCluster; c++)
-                if (c < a.cluster) {
-                    const float w = record_weight(cm[c], cl[c], mx);
-                    sum = fmaf(w, cl[c], sum);
-                    f.x = fmaf(w, cz[c].x, f.x); f.y = fmaf(w, cz[c].y, f.y); f.z = fmaf(w, cz[c].z, f.z); f.w = fmaf(w, cz[c].w, f.w);
-                }
-            store_quad<D, BF16>(a, out_row(a, it.b, it.h, it.rb * S::Rows + r), d, f, mx, sum);
-        }
-        cluster_sync();                                        // nobody leaves while its shared memory may be read
-    }
+    if (tid == 0) a.meta[blockIdx.x] = carried;
 }
 
 // Items that lie in several CTAs: a block takes 8 rows of the item that begins in CTA c and goes on, four warps a row, and
@@ -967,7 +956,7 @@ int clusters_at_once(DeviceState* st, int size) {
     std::atomic<int>& k = known[st->device][size];
     int n = k.load(std::memory_order_relaxed);
     if (n > 0) return n;
-    constexpr int smem = kWarps * Shape<128, 1>::WarpBytes + 1024;
+    constexpr int smem = Shape<128, 1>::SmemBytes;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(size);
     cfg.blockDim = dim3(kWarps * 32);
@@ -1019,7 +1008,7 @@ template <int D, bool BF16, int NT>
 int run_u4(const U4Args& a, int ctas, DeviceState* st, cudaStream_t stream) {
     using S = Shape<D, NT>;
     static bool configured[64] = {};
-    const int smem = kWarps * S::WarpBytes + 1024;
+    const int smem = S::SmemBytes;
     if (!configured[st->device]) {
         FA_CUDA_TRY(cudaFuncSetAttribute(u4_kernel<D, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         configured[st->device] = true;
