@@ -470,15 +470,17 @@ def rope(*args, **kw) -> None:
 
 
 def cache_append_raw(k, v, k_cache, v_cache, batch_size, num_tokens, num_kv_heads, seq_len_kv, d_head, dtype="f16",
-                     cache_dtype="f16", kv_strides=(0, 0, 0), q=None, q_out=None, num_q_heads=0,
+                     cache_dtype=None, kv_strides=(0, 0, 0), q=None, q_out=None, num_q_heads=0,
                      token_strides=(0, 0, 0), k_params=None, v_params=None, param_strides=(0, 0, 0), block_table=None,
                      block_table_stride=0, page_size=0, num_pages=0, seq_lens=None, num_new=None, positions=None,
                      inv_freq=None, rotary_dim=0, interleaved=False, amplitude=1.0, q_scale=None, k_scale=None,
                      v_scale=None, stream=None) -> int:
-    """fa_cache_append; ``cache_dtype`` is that of q, k and v, "e4m3" or "u4"; ``kv_strides`` and ``param_strides`` are
+    """fa_cache_append; ``cache_dtype`` is that of q, k and v (also if None), "e4m3" or "u4"; ``kv_strides`` and ``param_strides`` are
     (block, head, row) strides of the cache, a block being a page or a whole sequence; ``token_strides`` those between
     the tokens of q, k, v.  Returns the status code."""
-    if cache_dtype in ("f16", "bf16") and cache_dtype != dtype:
+    if cache_dtype is None:
+        cache_dtype = FA_CACHE_16BIT
+    elif cache_dtype in ("f16", "bf16") and DTYPES[cache_dtype] != DTYPES.get(dtype, dtype):
         return FA_ERR_UNSUPPORTED
     return (_lib or lib()).fa_cache_append(_pack_append(
         _adr(q), _adr(k), _adr(v), _adr(q_out), _adr(k_cache), _adr(v_cache), _adr(k_params), _adr(v_params),

@@ -28,6 +28,7 @@ constexpr int kMaxPairs = 64;
 struct Rotary {
     unsigned long long turns[kMaxPairs];
     double amplitude;
+    float minus_zero[2];                 // both -0, known to the host alone (see F2)
     int dim;                             // elements that turn; 0: none
 };
 
@@ -39,7 +40,9 @@ __device__ __forceinline__ void cos_sin(const Rotary& r, int position, int pair,
     *s = (float)((inverse ? -sd : sd) * r.amplitude);
 }
 
-// Two 32-bit operations at a time, each rounded by itself.
+// Two 32-bit operations at a time, each rounded by itself.  A product that is added to something is written as a b + (-0)
+// with the -0 from the kernel's arguments: mul.rn.f32x2 and add.rn.f32x2 came out as one multiply-add with one rounding
+// (1e-4 of fp16 results another, and with them levels of a 4-bit cache), unlike their forms for one value.
 struct F2 {
     unsigned long long v;
     __device__ __forceinline__ F2() {}
@@ -54,6 +57,11 @@ struct F2 {
 __device__ __forceinline__ F2 operator*(const F2& a, const F2& b) {
     F2 r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 product(const F2& a, const F2& b, const F2& minus_zero) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(minus_zero.v));
     return r;
 }
 __device__ __forceinline__ F2 operator+(const F2& a, const F2& b) {
@@ -98,15 +106,16 @@ struct Turn {
     // All lanes of the warp call this.  Products and sums are rounded one by one, so that a value is the same
     // wherever it is computed: a cache in 4 bits takes its levels from it.
     template <int LPR>
-    __device__ __forceinline__ uint4 apply(const uint4& x) const {
+    __device__ __forceinline__ uint4 apply(const uint4& x, const Rotary& rot) const {
+        const F2 mz(rot.minus_zero[0], rot.minus_zero[1]);
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
         uint32_t y[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float2 f = unpack16<BF16>(w[i]);
             float2 r;
-            if constexpr (INTER) r = (F2(f) * c[i] + F2(f.y, f.x) * s[i]).get();
-            else r = (F2(f) * c[i] + F2(unpack16<BF16>(__shfl_sync(0xffffffffu, w[i], partner, LPR))) * s[i]).get();
+            if constexpr (INTER) r = (product(F2(f), c[i], mz) + product(F2(f.y, f.x), s[i], mz)).get();
+            else r = (product(F2(f), c[i], mz) + product(F2(unpack16<BF16>(__shfl_sync(0xffffffffu, w[i], partner, LPR))), s[i], mz)).get();
             y[i] = pack16<BF16>(r.x, r.y);
         }
         return on ? make_uint4(y[0], y[1], y[2], y[3]) : x;
@@ -176,7 +185,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
 #pragma unroll
         for (int u = 0; u < kUnroll; u++) {
             const int h = h0 + u * step + slot / a.tokens;
-            const uint4 y = turn.template apply<LPR>(x[u]);
+            const uint4 y = turn.template apply<LPR>(x[u], a.rot);
             if (live[u]) {
                 const RopeTensor& r = h < a.hq ? a.q : a.k;
                 *reinterpret_cast<uint4*>(r.out + b * r.os.batch + (h < a.hq ? h : h - a.hq) * r.os.head + s * r.os.row + lane * 8) = y;
@@ -353,7 +362,7 @@ __global__ void __launch_bounds__(kAppendThreads, 8) append_kernel(const __grid_
             uint8_t* p = static_cast<uint8_t*>(a.q_out) + (((long long)n * a.hq + g.h0 + mine) * D + lane * 8) * (CACHE == FA_CACHE_E4M3 ? 1 : 2);
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const uint4 y = turn.template apply<LPR>(x[u]);
+                const uint4 y = turn.template apply<LPR>(x[u], a.rot);
                 const int h = g.h0 + mine + u * step;
                 if (h < g.end && in) {
                     if constexpr (CACHE == FA_CACHE_E4M3) {
@@ -370,7 +379,7 @@ __global__ void __launch_bounds__(kAppendThreads, 8) append_kernel(const __grid_
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 uint4 y = x[u];
-                if (g.kind == 1) y = turn.template apply<LPR>(y);
+                if (g.kind == 1) y = turn.template apply<LPR>(y, a.rot);
                 const int h = g.h0 + mine + u * step;
                 const bool put = store && h < g.end;
                 if constexpr (CACHE == FA_CACHE_U4) {
@@ -466,6 +475,7 @@ __global__ void __launch_bounds__(kThreads) read_u4_kernel(const __grid_constant
 // ------------------------------------------------------------------------------------------ host
 int make_rotary(const fa_rotary& r, int d_head, bool optional, Rotary* out) {
     *out = Rotary{};
+    out->minus_zero[0] = out->minus_zero[1] = -0.0f;
     if (r.rotary_dim < 0) return FA_ERR_INVALID_ARGUMENT;
     if (r.rotary_dim == 0) return optional ? FA_OK : FA_ERR_INVALID_ARGUMENT;
     if (r.rotary_dim > d_head || r.rotary_dim % 16 != 0) return FA_ERR_UNSUPPORTED;

@@ -490,8 +490,14 @@ int fa_cache_read_u4(const fa_cache_read_args* args);
  * fa_decode_gqa_u4: fa_decode_gqa over a 4-bit cache.  q, o [B, T, Hq, D] in `dtype`, lse [B, T, Hq]
  * (optional); T = num_q_tokens newest tokens per sequence (0 = 1), token t sees keys
  * [0, len - T + t]; a token that sees no key yields O = 0, LSE = -inf.  workspace: at least
- * fa_decode_gqa_u4_workspace_bytes(...) of the same sizes; two calls that may run at the same
- * time need one each.
+ * fa_decode_gqa_u4_workspace_bytes(...) of the same sizes on the same device; two calls that may
+ * run at the same time need one each.
+ *
+ * Few query rows (T * Hq / Hkv < 96): one pass over the codes, which are exact on the tensor core; about
+ * 12 MB of workspace.  Many: fa_decode_gqa's kernel over a copy of K and V in fp16 (so they are
+ * rounded once more, as a 16-bit cache of the same values would hold them), up to 256 MB of them or one
+ * sequence's at a time, in the workspace; bf16 queries reach it as fp16 times a power of two for each
+ * (sequence, KV head).
  */
 typedef struct fa_decode_gqa_u4_args {
     const void*     q;
@@ -504,7 +510,7 @@ typedef struct fa_decode_gqa_u4_args {
     int             batch_size;
     int             num_q_heads;
     int             num_kv_heads;  /* divides num_q_heads */
-    int             num_q_tokens;
+    int             num_q_tokens;  /* at most seq_len_kv */
     int             seq_len_kv;
     int             d_head;        /* 64 or 128 */
     float           scale;

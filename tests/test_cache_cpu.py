@@ -55,6 +55,14 @@ def _append(fa, **kw):
     return fa.cache_append_raw(*[base.pop(n) for n in names], **base)
 
 
+def test_append_types_by_name_and_number(fa):
+    """Past the types, the next check is the alignment."""
+    for dtype, cache in (("f16", None), ("f16", "f16"), (0, "f16"), (1, "bf16"), (1, None), ("bf16", "bf16"), ("bf16", 0)):
+        assert _append(fa, dtype=dtype, cache_dtype=cache, k_cache=8) == fa.FA_ERR_MISALIGNED
+    for dtype, cache in (("f16", "bf16"), (0, "bf16"), (1, "f16")):
+        assert _append(fa, dtype=dtype, cache_dtype=cache, k_cache=8) == fa.FA_ERR_UNSUPPORTED
+
+
 U4 = dict(cache_dtype="u4", kv_strides=(64 * 128, 64 * 64, 64), param_strides=(256, 128, 2), k_params=16, v_params=16)
 E4M3 = dict(cache_dtype="e4m3", q_scale=16, k_scale=16, v_scale=16)
 PAGED = dict(block_table=16, block_table_stride=4, page_size=16, num_pages=9)

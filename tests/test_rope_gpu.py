@@ -170,3 +170,49 @@ def test_captured_and_replayed_with_training_step(op, dev):
     torch.cuda.synchronize()
     for a, c in zip(outs, step()):
         assert torch.equal(a, c)
+
+
+def test_registered_operator_is_the_same_with_its_gradient(op, dev):
+    """torch.ops.fa_b200.rope (what compiled code reaches) and the eager call: the same bits, forward and backward."""
+    q, k = _x(dev, "bf16", 18, 2, 4, 21, 64).requires_grad_(), _x(dev, "bf16", 19, 2, 1, 21, 64).requires_grad_()
+    g, h = _x(dev, "bf16", 20, 2, 4, 21, 64), _x(dev, "bf16", 21, 2, 1, 21, 64)
+    f, _ = op.rope_frequencies(64)
+    pos = torch.arange(21, device=dev) * 1000
+    results = []
+    for fn in (op.rope, torch.ops.fa_b200.rope):
+        a, b = fn(q, k, f, pos, True, 1.25)
+        results.append((a, b, *torch.autograd.grad((a, b), (q, k), (g, h))))
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
+
+
+def test_side_stream(op, dev):
+    """Work on another stream than the tensors' own, ordered by the caller."""
+    x = _x(dev, "f16", 22, 1, 8, 300, 128)
+    f, _ = op.rope_frequencies(128)
+    want = op.rope(x, x, f)
+    s = torch.cuda.Stream(device=dev)
+    s.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(s):
+        got = op.rope(x, x, f)
+    s.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("inter", [False, True])
+def test_every_operation_is_rounded_by_itself(op, dev, dtype, inter):
+    """Products and their sum rounded to 32 bits one by one, then once to 16: the same bits as separate 32-bit operations,
+    which a cache in 4 bits depends on.  (One multiply-add instead gives 1e-4 of fp16 results another value.)"""
+    s, d = 2000, 128
+    x = _x(dev, dtype, 23, 1, 8, s, d)
+    f, _ = op.rope_frequencies(d)
+    y, _ = op.rope(x, x, f, None, inter)
+    ang = torch.arange(s, device=dev).double()[:, None] * f.to(dev)
+    c, sn = ang.cos().float(), ang.sin().float()
+    v = x.float()
+    a, b = (v[..., 0::2], v[..., 1::2]) if inter else (v[..., :d // 2], v[..., d // 2:])
+    want = torch.stack((a * c - b * sn, b * c + a * sn), -1 if inter else -2).flatten(-2).to(x.dtype)
+    # cos and sin come from angles in 64 bits by two ways: a value next to a border of 32 bits may round either way (2^-29
+    # relative a rounding of 2^-24, a few of 10^6), and then a 16-bit one in 2^13 or less of these
+    assert int((y != want).sum()) <= 2
