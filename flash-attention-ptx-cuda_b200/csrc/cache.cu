@@ -3,10 +3,10 @@
 //
 // The reference has none of them: its programs start from Q, K and V (src/demo.cu:28-70).
 //
-// All three read every element once and write it once, so HBM bounds them.  A row of D elements is covered by D / 8
-// lanes with one 16-byte access each; a block of 256 threads has 16 (D = 128) or 32 (D = 64) rows in flight at a time,
-// kUnroll such groups before it uses the first.  A thread keeps to one token and walks heads, so cos and sin of its 8
-// elements are read once, from a table in shared memory that the block computes for its tokens.
+// All three read every element once and write it once.  A row of D elements is covered by D / 8 lanes with one 16-byte
+// access each, so that a warp's access is two (D = 128) or four whole rows.  A thread keeps to one token and walks heads, so
+// cos and sin of its 8 elements are read once, from a table in shared memory that the block computes for its tokens: in 64
+// bits, which costs 30 operations of the 64-bit pipe a pair and token, 2 for each 16 bytes moved.
 #include <cmath>
 #include <cuda_fp8.h>
 
@@ -145,6 +145,8 @@ struct RopeArgs {
     bool inverse;
 };
 
+// Blocks of 8 tokens of a sequence and, while SMs are idle, parts of the heads; kUnroll rows a thread under way.  HBM bounds
+// it: bf16 B=2 Hq=32 Hkv=8 S=4096 D=128, half of the head turned, 168 MB in 31 us, 5.4 TB/s.
 template <int D, bool BF16, bool INTER>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
     constexpr int LPR = D / 8, SLOTS = kThreads / LPR;
@@ -428,7 +430,9 @@ __device__ __forceinline__ uint4 from_u4(uint32_t codes, __half2 param) {
     return make_uint4(y[0], y[1], y[2], y[3]);
 }
 
-// A block takes kUnroll groups of consecutive rows of one head.
+// A block takes kUnroll groups of consecutive rows of one head: the codes and pairs of consecutive rows lie together where the cache
+// is laid out for attention, and what it writes are whole rows either way.  HBM bounds it, by its writes: 4 sequences of 16384 rows,
+// Hkv=8 D=128, 344 MB in 57 us, 6.0 TB/s.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads) read_u4_kernel(const __grid_constant__ ReadArgs a) {
     constexpr int LPR = D / 8, SLOTS = kThreads / LPR;

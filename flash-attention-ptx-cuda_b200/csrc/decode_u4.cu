@@ -23,6 +23,10 @@
 // only once, at the end, where the CTA merges what its warps have of the same item.  Items that lie in several CTAs go
 // through the workspace and a second small kernel.  Short jobs are done in one launch instead: a cluster of up to 8 CTAs an
 // item, which merges through distributed shared memory (plan.cluster says when).
+//
+// Measured (f16, 4 query heads a KV head, D = 128, a call in a graph): B=32 Hkv=8 Skv=16384 126 us, 4.8 TB/s (loads alone 104; unpacking K and V
+// takes the rest: instructions that wait for one another with two warps a scheduler, slots 50 % used); B=16 Skv=4096 21.5; B=1 Skv=2048
+// 7.4; 16 query rows B=32 Skv=16384 198.
 #include <atomic>
 #include <cmath>
 #include <cuda_bf16.h>
