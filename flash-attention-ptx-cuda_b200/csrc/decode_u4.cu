@@ -17,8 +17,8 @@
 // came in, written and read back.  So the products are mma.sync m16n8k16 with the unpacked codes as the register operand A:
 // keys are the rows of S^T = K Q^T, head elements the rows of O^T = V^T P^T, and a query row takes one of 8 columns.
 //
-// Work split.  All (sequence, KV head, row block) items are laid out one after the other in tiles of 32 keys, and the
-// resulting line is cut into equal parts, one for each warp of the GPU, whatever the lengths of the sequences: a warp may
+// Work split.  All (sequence, KV head, row block) items are laid out one after the other in tiles of 64 or 32 keys, and
+// the resulting line is cut into equal parts, one for each warp of the GPU, whatever the lengths of the sequences: a warp may
 // finish one item, do several and begin the next.  A warp streams its tiles through a ring of its own and meets the others
 // only once, at the end, where the CTA merges what its warps have of the same item.  Items that lie in several CTAs go
 // through the workspace and a second small kernel.  Short jobs are done in one launch instead: a cluster of up to 8 CTAs an
@@ -48,7 +48,7 @@ constexpr int kMaxCluster = 8;                 // portable cluster size
 constexpr int tile_keys(int nt) { return nt == 1 ? 64 : 32; }
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kClusterTiles = 1;               // see make_plan
-constexpr int kManyRows = 96, kManyKeys = 256;    // see many_rows
+constexpr int kManyRows = 96, kManyKeys = 512;    // see many_rows
 constexpr size_t kCopyBytes = 256u << 20;      // of K and V in fp16 at a time
 constexpr float kGrow = 8.0f;                  // a running max may be exceeded by this much (in powers of two) before it is raised
 
@@ -1032,7 +1032,8 @@ int run_u4_rows(const U4Args& a, const Plan& p, DeviceState* st, cudaStream_t st
 // blocks / copy, f16 D=128 Hkv=8: B=8 Skv=4096 64 rows 61 / 66, 128 rows 109 / 71, 256 rows 203 / 73; B=1 Skv=4096 64 rows 17 / 19,
 // 128 rows 23 / 22, 256 rows 38 / 22; B=1 Skv=512 256 rows 12.3 / 11.7.  Blocks of 32 rows need more registers than
 // there are: 97 and 163 where those of 16 take 61 and 109.)  The copy rounds K^ and V^ to fp16, what a 16-bit cache of the
-// same values would hold: O is off by 4e-4 of its norm where the row blocks' is by 3e-4 and fp16 itself by 2e-4.
+// same values would hold: O is off by 4e-4 of its norm where the row blocks' is by 3e-4 and fp16 itself by 2e-4, and the LSE of a row
+// that sees few keys by up to 1e-4, which is why short caches stay with the row blocks.
 struct ManyPlan {
     int batch;                                // sequences of a copy
     int splits;                               // KV splits of the 16-bit kernel

@@ -493,7 +493,7 @@ int fa_cache_read_u4(const fa_cache_read_args* args);
  * fa_decode_gqa_u4_workspace_bytes(...) of the same sizes on the same device; two calls that may
  * run at the same time need one each.
  *
- * Few query rows (T * Hq / Hkv < 96): one pass over the codes, which are exact on the tensor core; about
+ * Few query rows (T * Hq / Hkv < 96, or fewer than 512 keys): one pass over the codes, which are exact on the tensor core; about
  * 12 MB of workspace.  Many: fa_decode_gqa's kernel over a copy of K and V in fp16 (so they are
  * rounded once more, as a 16-bit cache of the same values would hold them), up to 256 MB of them or one
  * sequence's at a time, in the workspace; bf16 queries reach it as fp16 times a power of two for each

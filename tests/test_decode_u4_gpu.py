@@ -363,7 +363,7 @@ def check_many(q, cache, o, lse, scale):
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("b,t,hq,hkv,skv,page,lens", [
-    (1, 96, 1, 1, 256, 0, None),                       # the smallest that counts as many rows
+    (1, 96, 1, 1, 512, 0, None),                       # the smallest that counts as many rows
     (2, 33, 8, 2, 1100, 16, [1100, 700]),
     (3, 100, 6, 3, 1500, 0, [1500, 40, 0]),            # fewer keys than tokens, and none
     (2, 300, 5, 1, 1027, 64, [1027, 1026]),
