@@ -78,7 +78,7 @@ PAGED = dict(block_table=16, block_table_stride=4, page_size=16, num_pages=9)
     (dict(kv_strides=(64 * 256, 132, 256)), "MISALIGNED"), (dict(token_strides=(512, 260, 256)), "MISALIGNED"),
     (dict(token_strides=(512, 128, 256)), "INVALID_ARGUMENT"), (dict(k_cache=8), "MISALIGNED"),
     (dict(E4M3, k_scale=None), "INVALID_ARGUMENT"), (dict(E4M3, q_scale=None), "INVALID_ARGUMENT"),
-    (dict(E4M3, d_head=64, rotary_dim=64), "UNSUPPORTED"), (dict(E4M3, kv_strides=(64 * 256, 136, 256)), "MISALIGNED"),
+    (dict(E4M3, d_head=64, rotary_dim=64), "UNSUPPORTED"), (dict(E4M3, num_kv_heads=1025, num_q_heads=1025), "UNSUPPORTED"), (dict(E4M3, kv_strides=(64 * 256, 136, 256)), "MISALIGNED"),
     (dict(U4, k_params=None), "INVALID_ARGUMENT"), (dict(U4, param_strides=(0, 0, 0)), "INVALID_ARGUMENT"),
     (dict(U4, param_strides=(256, 129, 2)), "MISALIGNED"), (dict(U4, kv_strides=(64 * 128, 64 * 64, 56)), "INVALID_ARGUMENT"),
     (dict(U4, kv_strides=(64 * 128, 64 * 64, 72)), "MISALIGNED"),

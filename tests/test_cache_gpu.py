@@ -103,6 +103,7 @@ SHAPES = [
     ("bf16", 4, 7, 5, 1, 128, 33, 0, True, [33, 0, -4, 99], [7, 3, 2, 0]),    # no rows; lengths out of range; padding
     ("f16", 2, 40, 4, 4, 128, 64, 32, False, [64, 41], [0, 40]),
     ("bf16", 1, 300, 3, 1, 64, 300, 0, False, None, [123]),
+    ("f16", 2, 3, 300, 300, 128, 5, 0, False, [5, 2], None),              # many KV heads
 ]
 
 
