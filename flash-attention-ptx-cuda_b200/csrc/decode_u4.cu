@@ -1142,9 +1142,10 @@ FA_EXPORT size_t fa_decode_gqa_u4_workspace_bytes(int batch_size, int num_q_head
         return 0;
     if (d_head != 64 && d_head != 128) return 0;
     DeviceState* st = device_state();
-    if (many_rows(num_q_heads, num_kv_heads, num_q_tokens > 0 ? num_q_tokens : 1, seq_len_kv))
-        return make_many_plan(batch_size, num_q_heads, num_kv_heads, num_q_tokens, seq_len_kv, d_head).bytes();
-    return make_plan(batch_size, num_q_heads, num_kv_heads, num_q_tokens > 0 ? num_q_tokens : 1, seq_len_kv, false, d_head, st).bytes;
+    const int n_tok = num_q_tokens > 0 ? num_q_tokens : 1;
+    if (many_rows(num_q_heads, num_kv_heads, n_tok, seq_len_kv))
+        return make_many_plan(batch_size, num_q_heads, num_kv_heads, n_tok, seq_len_kv, d_head).bytes();
+    return make_plan(batch_size, num_q_heads, num_kv_heads, n_tok, seq_len_kv, false, d_head, st).bytes;
 }
 
 FA_EXPORT int fa_decode_gqa_u4(const fa_decode_gqa_u4_args* p) {

@@ -474,6 +474,8 @@ def decode_gqa_u4(q: torch.Tensor, k_cache: torch.Tensor, k_params: torch.Tensor
     if q.dim() != 4:
         raise ValueError("fa_b200::decode_gqa_u4: expected q [B,T,Hq,D]")
     b, t, hq, d = q.shape
+    if t == 0:                                                 # to the library 0 is the default, one token
+        raise ValueError("fa_b200::decode_gqa_u4: q has no tokens")
     skv, kw = _cache_kw(k_cache, v_cache, d, b, seq_lens, block_table, k_params, v_params)
     hkv = k_cache.shape[2]
     q, _ = _rows(q.contiguous(), "q", copy=True)

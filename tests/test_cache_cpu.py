@@ -127,6 +127,7 @@ def test_attention_workspace(fa):
     size = fa.decode_gqa_u4_workspace_bytes
     assert size(0, 4, 2, 1, 64, 128) == size(1, 3, 2, 1, 64, 128) == size(1, 4, 2, 1, 64, 96) == 0
     assert 0 < size(1, 4, 2, 1, 64, 128) <= size(8, 4, 2, 1, 4096, 128) == size(8, 4, 2, 0, 4096, 128)
+    assert size(2, 128, 1, 0, 4096, 128) == size(2, 128, 1, 1, 4096, 128) > 0     # no number of tokens: one, of many rows here
     assert size(64, 32, 8, 1, 4096, 128) > 148 * 10 * 8 * 130 * 4 - 1      # parts of the line: 10 records an SM
 
 

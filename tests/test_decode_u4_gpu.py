@@ -328,7 +328,7 @@ def test_refused_by_the_operator(op, dev):
     kc, kp, vc, vp = cache.tensors
     for args, err in (((q.float(), kc, kp, vc, vp, 0.1), TypeError), ((q, kc, kp, vc[:, :32], vp, 0.1), ValueError),
                       ((q, kc, kp.float(), vc, vp, 0.1), ValueError), ((q[:1], kc, kp, vc, vp, 0.1), ValueError),
-                      ((q[0], kc, kp, vc, vp, 0.1), ValueError), ((q, kc.float(), kp, vc.float(), vp, 0.1), TypeError),
+                      ((q[0], kc, kp, vc, vp, 0.1), ValueError), ((q[:, :0], kc, kp, vc, vp, 0.1), ValueError), ((q, kc.float(), kp, vc.float(), vp, 0.1), TypeError),
                       ((q, kc, kp, vc, vp, 0.1, torch.zeros(3, device=dev, dtype=torch.int32)), ValueError)):
         with pytest.raises(err):
             op.decode_gqa_u4(*args)
