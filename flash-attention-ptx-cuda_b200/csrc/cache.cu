@@ -520,6 +520,10 @@ int pow2_at_least(int n, int most) {
 }
 
 bool strides_ok(const fa_strides& s) { return s.batch >= 0 && s.head >= 0 && s.row >= 0; }
+// A tensor that is its own result: every row is read before it is written if both lie in the same places.
+bool in_place_ok(const void* in, const void* out, const fa_strides& is, const fa_strides& os, int batch, int heads, int seq_len) {
+    return in != out || ((batch == 1 || is.batch == os.batch) && (heads == 1 || is.head == os.head) && (seq_len == 1 || is.row == os.row));
+}
 bool strides_aligned(const fa_strides& s) { return s.batch % 8 == 0 && s.head % 8 == 0 && s.row % 8 == 0; }
 fa_strides or_dense(const fa_strides& s, int heads, int seq_len, int d_head) {
     if (s.batch || s.head || s.row) return s;
@@ -574,6 +578,7 @@ using namespace fa;
 FA_EXPORT int fa_rope(const fa_rope_args* p) {
     if (!p || !p->q || !p->q_out) return FA_ERR_INVALID_ARGUMENT;
     if (p->batch_size <= 0 || p->num_q_heads <= 0 || p->num_kv_heads < 0 || p->seq_len <= 0) return FA_ERR_INVALID_ARGUMENT;
+    if ((long long)p->num_q_heads + p->num_kv_heads > 1 << 24) return FA_ERR_INVALID_ARGUMENT;
     if ((p->num_kv_heads > 0) != (p->k != nullptr) || (p->k != nullptr) != (p->k_out != nullptr)) return FA_ERR_INVALID_ARGUMENT;
     if (p->inverse != 0 && p->inverse != 1) return FA_ERR_INVALID_ARGUMENT;
     if (p->positions_stride < 0 || (long long)p->position_offset + p->seq_len - 1 > 0x7FFFFFFFll) return FA_ERR_INVALID_ARGUMENT;
@@ -587,13 +592,16 @@ FA_EXPORT int fa_rope(const fa_rope_args* p) {
     if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->q_out) || !aligned16(p->k_out)) return FA_ERR_MISALIGNED;
     if (!strides_aligned(p->q_strides) || !strides_aligned(p->k_strides) || !strides_aligned(p->q_out_strides) || !strides_aligned(p->k_out_strides))
         return FA_ERR_MISALIGNED;
-    DeviceState* st = device_state();
-    if (!st) return FA_ERR_CUDA;
-    if (st->cc_major != 10) return FA_ERR_NOT_SM100;
     a.q = {static_cast<const uint16_t*>(p->q), static_cast<uint16_t*>(p->q_out), or_dense(p->q_strides, p->num_q_heads, p->seq_len, p->d_head),
            or_dense(p->q_out_strides, p->num_q_heads, p->seq_len, p->d_head)};
     a.k = {static_cast<const uint16_t*>(p->k), static_cast<uint16_t*>(p->k_out), or_dense(p->k_strides, p->num_kv_heads, p->seq_len, p->d_head),
            or_dense(p->k_out_strides, p->num_kv_heads, p->seq_len, p->d_head)};
+    if (!in_place_ok(p->q, p->q_out, a.q.is, a.q.os, p->batch_size, p->num_q_heads, p->seq_len) ||
+        (p->k && !in_place_ok(p->k, p->k_out, a.k.is, a.k.os, p->batch_size, p->num_kv_heads, p->seq_len)))
+        return FA_ERR_INVALID_ARGUMENT;
+    DeviceState* st = device_state();
+    if (!st) return FA_ERR_CUDA;
+    if (st->cc_major != 10) return FA_ERR_NOT_SM100;
     a.hq = p->num_q_heads;
     a.heads = p->num_q_heads + p->num_kv_heads;
     a.seq_len = p->seq_len;
@@ -662,8 +670,8 @@ FA_EXPORT int fa_cache_append(const fa_cache_append_args* p) {
     }
     if (p->cache == FA_CACHE_U4 && (!p->k_params || !p->v_params)) return FA_ERR_INVALID_ARGUMENT;
     const long long n_all = (long long)p->batch_size * p->num_tokens;
+    if (n_all > 0x7FFFFFFFll || n_all * (p->num_q_heads + 2ll * p->num_kv_heads) > 0x7FFFFFFFll) return FA_ERR_INVALID_ARGUMENT;
     const int heads = p->num_q_heads + 2 * p->num_kv_heads;
-    if (n_all * heads > 0x7FFFFFFFll) return FA_ERR_INVALID_ARGUMENT;
     AppendArgs a;
     int rc = make_rotary(p->rotary, p->d_head, true, &a.rot);
     if (rc != FA_OK) return rc;
@@ -679,6 +687,7 @@ FA_EXPORT int fa_cache_append(const fa_cache_append_args* p) {
     a.k_stride = p->k_token_stride ? p->k_token_stride : dense_kv;
     a.v_stride = p->v_token_stride ? p->v_token_stride : dense_kv;
     if (a.q_stride < dense_q || a.k_stride < dense_kv || a.v_stride < dense_kv) return FA_ERR_INVALID_ARGUMENT;
+    if (p->q && p->q == p->q_out && (p->cache == FA_CACHE_E4M3 || (n_all > 1 && a.q_stride != dense_q))) return FA_ERR_INVALID_ARGUMENT;
     DeviceState* st = device_state();
     if (!st) return FA_ERR_CUDA;
     if (st->cc_major != 10) return FA_ERR_NOT_SM100;

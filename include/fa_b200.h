@@ -425,7 +425,7 @@ typedef struct fa_cache_layout {
  *       can be parts of one projection's output.
  *   q_out [B, T, Hq, D] dense: rotated q, in `dtype`; for an e4m3 cache its codes, rounded from the
  *       rotated 16-bit value times 1 / q_scale[b * Hkv + kv head].  Zero for tokens that are not
- *       stored.  May be q itself if q is dense and the cache is not e4m3.
+ *       stored.  May be q itself if q is dense and the cache is not e4m3 (refused otherwise).
  *   k rotated and v go into the caches: FA_CACHE_16BIT in `dtype`; FA_CACHE_E4M3 (d_head 128, up to 1024 KV heads) as codes of
  *       the 16-bit value times 1 / {k,v}_scale[b * Hkv + kv head], saturating; FA_CACHE_U4 as above.
  * Everything else in the caches stays as it is.

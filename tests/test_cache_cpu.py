@@ -42,6 +42,8 @@ def _rope(fa, **kw):
     (dict(inv_freq=(ctypes.c_double * 32)(*[float("inf")] * 32)), "INVALID_ARGUMENT"),
     (dict(position_offset=2 ** 31 - 8 + 1), "INVALID_ARGUMENT"), (dict(positions=16, positions_stride=-1), "INVALID_ARGUMENT"),
     (dict(q=24), "MISALIGNED"), (dict(q_strides=(4096, 512, 68)), "MISALIGNED"), (dict(k_out_strides=(0, -64, 64)), "INVALID_ARGUMENT"),
+    (dict(q_strides=(4096, 64, 256)), "INVALID_ARGUMENT"), (dict(k_out_strides=(4096, 64, 128)), "INVALID_ARGUMENT"),   # in place, elsewhere
+    (dict(num_q_heads=2 ** 30, num_kv_heads=2 ** 30), "INVALID_ARGUMENT"),
 ])
 def test_rope_refusals(fa, change, code):
     assert _rope(fa, **change) == getattr(fa, "FA_ERR_" + code)
@@ -79,6 +81,8 @@ PAGED = dict(block_table=16, block_table_stride=4, page_size=16, num_pages=9)
     (dict(token_strides=(512, 128, 256)), "INVALID_ARGUMENT"), (dict(k_cache=8), "MISALIGNED"),
     (dict(E4M3, k_scale=None), "INVALID_ARGUMENT"), (dict(E4M3, q_scale=None), "INVALID_ARGUMENT"),
     (dict(E4M3, d_head=64, rotary_dim=64), "UNSUPPORTED"), (dict(E4M3, num_kv_heads=1025, num_q_heads=1025), "UNSUPPORTED"), (dict(E4M3, kv_strides=(64 * 256, 136, 256)), "MISALIGNED"),
+    (dict(E4M3), "INVALID_ARGUMENT"), (dict(token_strides=(1024, 0, 0)), "INVALID_ARGUMENT"),       # q_out is q, of other places
+    (dict(num_kv_heads=2 ** 30, num_q_heads=2 ** 30), "INVALID_ARGUMENT"), (dict(batch_size=2 ** 30, num_tokens=64), "INVALID_ARGUMENT"),
     (dict(U4, k_params=None), "INVALID_ARGUMENT"), (dict(U4, param_strides=(0, 0, 0)), "INVALID_ARGUMENT"),
     (dict(U4, param_strides=(256, 129, 2)), "MISALIGNED"), (dict(U4, kv_strides=(64 * 128, 64 * 64, 56)), "INVALID_ARGUMENT"),
     (dict(U4, kv_strides=(64 * 128, 64 * 64, 72)), "MISALIGNED"),
