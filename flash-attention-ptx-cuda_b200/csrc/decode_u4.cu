@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
 #pragma unroll
             for (int i = 0; i < KPL; i++)
 #pragma unroll
-                for (int gi = 0; gi < G; gi++) s_max = fmaxf(s_max, unpack16<false>(vraw[i][gi]).x);
+                for (int gi = 0; gi < G; gi++) s_max = fmaxf(s_max, fabsf(unpack16<false>(vraw[i][gi]).x));
             if (__any_sync(0xffffffffu, s_max > s_limit)) {
 #pragma unroll
                 for (int off = 16; off > 0; off >>= 1) s_max = fmaxf(s_max, __shfl_xor_sync(0xffffffffu, s_max, off));

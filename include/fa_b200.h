@@ -394,7 +394,7 @@ int fa_rope_inv_freq(const fa_rope_scaling* scaling, int rotary_dim, double* inv
  *
  * FA_CACHE_U4, a cache in 4 bits: two codes to a byte, the even element of the row in the low
  * half; every 64 elements have a pair (scale, offset) of fp16, value = offset + scale * code, code
- * 0..15.  4.5 bits an element.  The pairs of a row are contiguous (d_head / 64 of them); the
+ * 0..15 (a cache of other origin may have scales of either sign).  4.5 bits an element.  The pairs of a row are contiguous (d_head / 64 of them); the
  * param strides count pairs and are multiples of d_head / 64.  What fa_cache_append stores, with
  * x the 16-bit element (clamped to +-65504, a NaN makes its 64 elements NaN):
  *     offset = fp16(min x), scale = fp16((max x - offset) / 15),

@@ -189,6 +189,30 @@ def test_large_scores_and_uneven_scales(op, dev):
         check(q, cache, o, lse, scale, skv)
 
 
+@pytest.mark.parametrize("t", [1, 3])
+def test_scales_of_either_sign(op, dev, t):
+    """The same values written from the other end: offset + 15 scale as offset, -scale, 15 - code."""
+    b, hq, hkv, skv, d = 2, 8, 2, 700, 128
+    q, cache = make(dev, "f16", b, t, hq, hkv, skv, d, seed=14)
+    for x in (0, 1):
+        for i in range(b):
+            codes, params = cache.packed[x][i]
+            turn = torch.rand(params.shape[:2], device=dev) < 0.5 if t == 3 else torch.ones(params.shape[:2], device=dev, dtype=torch.bool)
+            z, s = params[..., 1].float(), params[..., 0].float()
+            new = torch.stack([-s, z + 15 * s], -1).half()
+            params.copy_(torch.where(turn[..., None, None], new, params))
+            codes.copy_(torch.where(turn[..., None], 255 - codes, codes))          # both codes of a byte
+            cache.tensors[2 * x][i, :skv], cache.tensors[2 * x + 1][i, :skv] = codes, params
+    o, lse = run(op, q, cache, 0.0884)
+    want, want_l, amount, worst = reference(q, cache, 0.0884)
+    largest = max(float(p[..., 0].abs().max()) for p in (cache.packed[0][0][1], cache.packed[0][1][1]))
+    d0 = 16 * 2.0 ** -23 * 79 * float(q.double().abs().sum(-1).max()) * largest * 0.0884 + 2.0 ** -22     # as in check(), of |scale|
+    steps = (skv // 16 + 16) * 2.0 ** -23
+    tol = amount * (2.0 ** -12 + 2 * d0 + steps) + want.abs() * 2.0 ** -11 + 2.0 ** -25
+    assert ((o.double() - want).abs() <= tol).all()
+    assert ((lse.double() - want_l).abs() <= 2 * d0 + steps + 2.0 ** -23 * want_l.abs()).all()
+
+
 def test_nan_in_a_key_reaches_its_head_alone(op, dev):
     q, cache = make(dev, "f16", 2, 1, 4, 2, 100, 64, seed=4)
     kc, kp, vc, vp = cache.tensors
@@ -424,3 +448,23 @@ def test_many_tokens_captured_and_replayed(op, dev):
     torch.cuda.synchronize()
     want = op.decode_gqa_u4(q, kc, kp, vc, vp, 0.0884, lens, cache.table)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_many_tokens_whatever_the_workspace_holds(fa, op, dev, dtype):
+    """Rows past a sequence's end are not copied: what lies there, here NaN, reaches nothing."""
+    b, t, hq, hkv, skv, d = 3, 50, 8, 2, 1100, 128
+    lens = [1100, 513, 7]
+    q, cache = make(dev, dtype, b, t, hq, hkv, skv, d, lens, seed=15)
+    want, want_l = run(op, q, cache, 0.0884)
+    check_many(q, cache, want, want_l, 0.0884)
+    kc, kp, vc, vp = cache.tensors
+    need = fa.decode_gqa_u4_workspace_bytes(b, hq, hkv, t, skv, d)
+    o, lse = torch.full_like(want, float("nan")), torch.full_like(want_l, float("nan"))
+    fa.decode_gqa_u4(q, kc, kp, vc, vp, o, lse, b, hq, hkv, skv, d, 0.0884, dtype=dtype, num_q_tokens=t,
+                     kv_strides=(kc.stride(0), kc.stride(2), kc.stride(1)),
+                     param_strides=(kp.stride(0) // 2, kp.stride(2) // 2, kp.stride(1) // 2),
+                     seq_lens=torch.tensor(lens, device=dev, dtype=torch.int32),
+                     workspace=torch.full((need,), 255, device=dev, dtype=torch.uint8), workspace_bytes=need,
+                     stream=torch.cuda.current_stream())
+    assert torch.equal(o, want) and torch.equal(lse, want_l)
