@@ -265,14 +265,13 @@ def _(q, k, inv_freq, positions=None, interleaved=False, amplitude=1.0, inverse=
 
 def _rope_setup_context(ctx, inputs, output):
     _, _, inv_freq, positions, interleaved, amplitude, inverse = inputs
-    ctx.save_for_backward(*(() if positions is None else (positions,)))
-    ctx.inv_freq, ctx.how = inv_freq, (interleaved, amplitude, not inverse)
+    ctx.save_for_backward(inv_freq, positions)                 # so that autograd sees if one is overwritten in between
+    ctx.how = interleaved, amplitude, not inverse
 
 
 def _rope_backward(ctx, d_q, d_k):
     """The map is linear: its gradient is the transposed one, the rotation back (with the same amplitude)."""
-    positions = ctx.saved_tensors[0] if ctx.saved_tensors else None
-    d_q, d_k = rope(d_q, d_k, ctx.inv_freq, positions, *ctx.how)
+    d_q, d_k = rope(d_q, d_k, *ctx.saved_tensors, *ctx.how)
     return d_q, d_k, None, None, None, None, None
 
 
@@ -282,12 +281,12 @@ torch.library.register_autograd("fa_b200::rope", _rope_backward, setup_context=_
 class _Rope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, inv_freq, positions, interleaved, amplitude, inverse):
-        ctx.args = inv_freq, positions, interleaved, amplitude, not inverse
+        _rope_setup_context(ctx, (q, k, inv_freq, positions, interleaved, amplitude, inverse), None)
         return _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse)
 
     @staticmethod
     def backward(ctx, d_q, d_k):
-        return *rope(d_q, d_k, *ctx.args), None, None, None, None, None
+        return _rope_backward(ctx, d_q, d_k)
 
 
 def rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,

@@ -124,6 +124,18 @@ def test_gradient(op, dev, dtype, inter, rot):
     _check(ones, torch.ones_like(gq), p, f, inter, amp, inverse=True)
 
 
+@pytest.mark.parametrize("which", ["positions", "inv_freq"])
+@pytest.mark.parametrize("registered", [False, True])
+def test_overwritten_before_the_backward_pass(op, dev, which, registered):
+    q = torch.randn((1, 2, 8, 64), device=dev).half().requires_grad_()
+    k = torch.randn((1, 1, 8, 64), device=dev).half()
+    f, pos = op.rope_frequencies(64)[0], torch.arange(8, device=dev, dtype=torch.int32)
+    qo, _ = (torch.ops.fa_b200.rope if registered else op.rope)(q, k, f, pos)
+    (pos if which == "positions" else f).mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        qo.float().sum().backward()
+
+
 def test_nan_and_inf_stay_in_their_pair(op, dev):
     s, d, rot = 4, 64, 32
     x = _x(dev, "f16", 13, 1, 1, s, d)
