@@ -228,18 +228,19 @@ def _on(device: torch.device):
 
 
 def _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse):
-    if q.dtype not in _DTYPES or k.dtype != q.dtype:
+    dtype, device, q_shape, k_shape = q.dtype, q.device, q.shape, k.shape
+    if dtype not in _DTYPES or k.dtype != dtype:
         raise TypeError("fa_b200: q and k must share dtype float16 or bfloat16")
     if not (q.is_cuda and k.is_cuda):
         raise RuntimeError("fa_b200: tensors must be on a CUDA device (there is no CPU path)")
-    device = q.device
-    if q.dim() != 4 or k.dim() != 4 or (q.shape[0], *q.shape[2:]) != (k.shape[0], *k.shape[2:]) or k.device != device:
+    if len(q_shape) != 4 or len(k_shape) != 4 or q_shape[0] != k_shape[0] or q_shape[2:] != k_shape[2:] or k.device != device:
         raise ValueError("fa_b200::rope: expected q [B,Hq,S,D] and k [B,Hkv,S,D] on one device")
-    b, hq, s, d = q.shape
-    hkv = k.shape[1]
+    b, hq, s, d = q_shape
+    hkv = k_shape[1]
     inv_freq = _inv_freq(inv_freq)
     (q, qs), (k, ks) = _rows(q, "q", copy=True), _rows(k, "k", copy=True)
-    q_out, k_out = q.new_empty((b, hq, s, d)), k.new_empty((b, hkv, s, d))
+    q_out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q_shape)      # the first costs half
+    k_out = torch.empty_like(k) if k.is_contiguous() else k.new_empty(k_shape)
     pos_stride = 0
     if positions is not None:
         if positions.is_floating_point() or tuple(positions.shape) not in ((s,), (b, s)) or positions.device != device:
@@ -248,7 +249,7 @@ def _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse):
         pos_stride = s if positions.dim() == 2 else 0
     with _on(device):
         _fa.rope(q, k if hkv else None, q_out, k_out if hkv else None, b, hq, hkv, s, d, inv_freq, 2 * inv_freq.numel(),
-                 interleaved, amplitude, _DTYPES[q.dtype], positions, pos_stride, 0, inverse, qs, ks, stream=_stream(device))
+                 interleaved, amplitude, _DTYPES[dtype], positions, pos_stride, 0, inverse, qs, ks, stream=_stream(device))
     return q_out, k_out
 
 
