@@ -436,7 +436,10 @@ def _adr(x) -> int:
         return 0
     if x.__class__ is int:
         return x
-    return ctypes.addressof(x) if isinstance(x, ctypes.Array) else x.data_ptr()
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return ctypes.addressof(x)
 
 
 def rope_inv_freq(rotary_dim, base=10000.0, scaling="plain", factor=1.0, original_length=0.0, slow=0.0, fast=0.0):
