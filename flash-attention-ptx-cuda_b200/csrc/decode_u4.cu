@@ -226,6 +226,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
     __shared__ __align__(8) uint64_t s_full[kWarps][S::Stages];
     __shared__ int s_abort, s_never;
     __shared__ int s_prefix[kWarps * 32], s_warp[kWarps];      // tiles (of one head and row block) before a thread's sequences
+    __shared__ int s_len[kWarps * 32];                         // keys of the last of them
     __shared__ int s_item[kRecords], s_before[kWarps], s_after[kWarps];
     __shared__ float s_m[kRecords][S::Rows], s_l[kRecords][S::Rows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -261,11 +262,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
         const int per_thread = (a.batch + kWarps * 32 - 1) / (kWarps * 32);   // sequences of a thread
         int total = a.batch * tiles_of<S::Keys>(a.kv_len);
         if (a.seq_lens != nullptr) {
-            int sum = 0;
+            int sum = 0, len = 0;
             for (int i = 0; i < per_thread; i++) {
                 const int b = tid * per_thread + i;
-                if (b < a.batch) sum += tiles_of<S::Keys>(sequence_length(a.seq_lens, b, a.kv_len));
+                if (b >= a.batch) break;
+                len = sequence_length(a.seq_lens, b, a.kv_len);
+                sum += tiles_of<S::Keys>(len);
             }
+            s_len[tid] = len;
             int inc = sum;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -304,16 +308,16 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
             b_start = it.b * it.tiles * per_b;
         } else {
             const int per_thread = (a.batch + kWarps * 32 - 1) / (kWarps * 32);
-            int lo = 0, hi = kWarps * 32 - 1;                  // last thread whose sequences begin at or before w_begin
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (s_prefix[mid] * per_b <= w_begin && mid * per_thread < a.batch) lo = mid;
-                else hi = mid - 1;
+            int lo = -1;                                       // last thread whose sequences begin at or before w_begin
+#pragma unroll
+            for (int i = 0; i < kWarps; i++) {
+                const int y = i * 32 + lane;
+                lo += __popc(__ballot_sync(0xffffffffu, s_prefix[y] * per_b <= w_begin && y * per_thread < a.batch));
             }
             it.b = lo * per_thread;
             b_start = s_prefix[lo] * per_b;
             for (;;) {
-                it.len = sequence_length(a.seq_lens, it.b, a.kv_len);
+                it.len = per_thread == 1 ? s_len[lo] : sequence_length(a.seq_lens, it.b, a.kv_len);
                 it.tiles = tiles_of<S::Keys>(it.len);
                 const int end = b_start + it.tiles * per_b;
                 if (w_begin < end || it.b + 1 >= a.batch) break;
