@@ -490,7 +490,7 @@ int fa_cache_read_u4(const fa_cache_read_args* args);
  * fa_decode_gqa_u4: fa_decode_gqa over a 4-bit cache.  q, o [B, T, Hq, D] in `dtype`, lse [B, T, Hq]
  * (optional); T = num_q_tokens newest tokens per sequence (0 = 1), token t sees keys
  * [0, len - T + t]; a token that sees no key yields O = 0, LSE = -inf.  Rows past a sequence's end may hold anything; a NaN
- * in a row of V reaches the T tokens of its head, those before it too (0 * NaN).  workspace: at least
+ * in a row of V may reach all T tokens of its head, those before it too (0 * NaN).  workspace: at least
  * fa_decode_gqa_u4_workspace_bytes(...) of the same sizes on the same device; two calls that may
  * run at the same time need one each.
  *
