@@ -145,7 +145,7 @@ struct RopeArgs {
     bool inverse;
 };
 
-// Blocks of 8 tokens of a sequence and, while SMs are idle, parts of the heads; kUnroll rows a thread under way.  HBM bounds
+// Blocks of 8 or 16 tokens of a sequence and, while SMs are idle, parts of the heads; kUnroll rows a thread under way.  HBM bounds
 // it: bf16 B=2 Hq=32 Hkv=8 S=4096 D=128, half of the head turned, 168 MB in 31 us, 5.4 TB/s.
 template <int D, bool BF16, bool INTER>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
@@ -605,10 +605,14 @@ FA_EXPORT int fa_rope(const fa_rope_args* p) {
     a.hq = p->num_q_heads;
     a.heads = p->num_q_heads + p->num_kv_heads;
     a.seq_len = p->seq_len;
-    a.tokens = pow2_at_least(p->seq_len, 8);
+    // 8 tokens a block, and with d_head 64 16 where that leaves blocks enough: then either has two heads of a token at a time, 8 a turn
+    // of the loop, of which a last turn wastes fewer than of 16 (us in a graph, 8 / 16: B=4 Hq=32 Hkv=8 S=4096 37.6 / 35.4, B=8 H=12
+    // 50.2 / 44.9; with too few blocks, B=1 Hq=32 Hkv=8 S=4096, 11.3 / 12.2)
+    const int slots = kThreads / (p->d_head / 8);
+    const bool many = (long long)p->batch_size * ((p->seq_len + slots / 2 - 1) / (slots / 2)) >= 2ll * st->sm_count;
+    a.tokens = pow2_at_least(p->seq_len, many ? slots / 2 : 8);
     a.tiles = (p->seq_len + a.tokens - 1) / a.tokens;
     const long long tiles = (long long)a.tiles * p->batch_size;
-    const int slots = kThreads / (p->d_head / 8);
     a.splits = head_splits(tiles, a.heads, slots / a.tokens, st->sm_count);
     a.positions = p->positions;
     a.positions_stride = p->positions_stride;

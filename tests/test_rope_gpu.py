@@ -41,6 +41,18 @@ def test_rope(op, dev, dtype, inter, d, rot, b, hq, hkv, s):
         assert torch.equal(y[..., rot:], x[..., rot:])
 
 
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("b,hq,hkv,s", [(5, 3, 2, 1001), (2, 13, 1, 3000), (300, 5, 0, 15)])
+def test_rope_many_tokens_of_small_heads(op, dev, inter, b, hq, hkv, s):
+    """d_head 64 with enough tokens for the larger blocks, which the last ones do not fill."""
+    q, k = _x(dev, "f16", 5, b, hq, s, 64), _x(dev, "f16", 6, b, hkv, s, 64)
+    f, _ = op.rope_frequencies(64)
+    qo, ko = op.rope(q, k, f, None, inter)
+    _check(qo, q, np.arange(s), f, inter)
+    if hkv:
+        _check(ko, k, np.arange(s), f, inter)
+
+
 @pytest.mark.parametrize("b,hq,hkv,s", [(1, 40, 8, 3), (3, 5, 1, 9), (1, 71, 0, 130), (2, 32, 8, 1000), (5, 3, 3, 8)])
 def test_rope_sizes(op, dev, b, hq, hkv, s):
     q, k = _x(dev, "bf16", 3, b, hq, s, 128), _x(dev, "bf16", 4, b, hkv, s, 128)
