@@ -295,7 +295,7 @@ __device__ __forceinline__ uint32_t to_u4(const uint4& x, __half2* param) {
 // row cost: small blocks of few tokens, 8 of them an SM (512 tokens to 8 sequences, Hq=32 Hkv=8 D=128, e4m3 / 4-bit with its read
 // back, us in a graph: 256 threads and 8 tokens 22.7 / 29.9, 128 and 2 20.0 / 26.6; one token to 16 sequences 3.3, 2.8; the scales
 // of e4m3 inverted once a block instead of once a row 20.3 -> 19.6).
-constexpr int kAppendThreads = 128, kAppendTokens = 2, kAppendUnroll = 2;
+constexpr int kAppendThreads = 128, kAppendUnroll = 2;
 template <int D, bool BF16, bool INTER, int CACHE>
 __global__ void __launch_bounds__(kAppendThreads, 8) append_kernel(const __grid_constant__ AppendArgs a) {
     constexpr int LPR = D / 8, SLOTS = kAppendThreads / LPR, U = kAppendUnroll;
@@ -708,9 +708,15 @@ FA_EXPORT int fa_cache_append(const fa_cache_append_args* p) {
     a.n_tokens = p->num_tokens;
     a.n_all = (int)n_all;
     a.seq_len_kv = p->seq_len_kv;
-    a.tokens = pow2_at_least((int)((n_all + 2 * st->sm_count - 1) / (2 * st->sm_count)), kAppendTokens);
+    // Tokens of a block: a power of two, 2 to 8, such that the KV heads fill a turn of a token's threads (8 heads of 2 tokens with d_head
+    // 128, of 4 with 64); fewer while that leaves SMs idle.  (us in a graph, 2 tokens / this, 8 x 512 tokens: D=64 Hq=32 Hkv=8
+    // 4-bit 15.2 / 12.7, Hq=12 Hkv=4 12.9 / 8.2; D=128 Hq=16 Hkv=1 15.1 / 12.6; 8 also with Hq=32 Hkv=8 D=64 13.9, 16 with Hq=8 Hkv=1
+    // D=64 7.2 where 8 take 6.1.)
+    const int slots = kAppendThreads / (p->d_head / 8);
+    const int fill = pow2_at_least((slots * kAppendUnroll + p->num_kv_heads - 1) / p->num_kv_heads, 8);
+    a.tokens = pow2_at_least((int)((n_all + 2 * st->sm_count - 1) / (2 * st->sm_count)), fill > 2 ? fill : 2);
     const long long tiles = (n_all + a.tokens - 1) / a.tokens;
-    a.splits = head_splits(tiles, heads, kAppendThreads / (p->d_head / 8) / a.tokens, st->sm_count);
+    a.splits = head_splits(tiles, heads, slots / a.tokens, st->sm_count);
     a.block_stride = p->layout.block_stride * unit;
     a.head_stride = p->layout.head_stride * unit;
     a.row_stride = p->layout.row_stride * unit;

@@ -104,6 +104,8 @@ SHAPES = [
     ("f16", 2, 40, 4, 4, 128, 64, 32, False, [64, 41], [0, 40]),
     ("bf16", 1, 300, 3, 1, 64, 300, 0, False, None, [123]),
     ("f16", 2, 3, 300, 300, 128, 5, 0, False, [5, 2], None),              # many KV heads
+    ("bf16", 3, 801, 3, 1, 64, 900, 0, True, [900, 850, 3], None),        # the largest blocks, across sequences
+    ("f16", 2, 1201, 4, 2, 128, 1300, 16, False, [1300, 1250], [1201, 700]),
 ]
 
 
