@@ -578,7 +578,7 @@ using namespace fa;
 FA_EXPORT int fa_rope(const fa_rope_args* p) {
     if (!p || !p->q || !p->q_out) return FA_ERR_INVALID_ARGUMENT;
     if (p->batch_size <= 0 || p->num_q_heads <= 0 || p->num_kv_heads < 0 || p->seq_len <= 0) return FA_ERR_INVALID_ARGUMENT;
-    if ((long long)p->num_q_heads + p->num_kv_heads > 1 << 24) return FA_ERR_INVALID_ARGUMENT;
+    if ((long long)p->num_q_heads + p->num_kv_heads > 1 << 24 || p->seq_len > 0x7FFFFFFF - 64) return FA_ERR_INVALID_ARGUMENT;
     if ((p->num_kv_heads > 0) != (p->k != nullptr) || (p->k != nullptr) != (p->k_out != nullptr)) return FA_ERR_INVALID_ARGUMENT;
     if (p->inverse != 0 && p->inverse != 1) return FA_ERR_INVALID_ARGUMENT;
     if (p->positions_stride < 0 || (long long)p->position_offset + p->seq_len - 1 > 0x7FFFFFFFll) return FA_ERR_INVALID_ARGUMENT;

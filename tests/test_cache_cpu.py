@@ -43,7 +43,7 @@ def _rope(fa, **kw):
     (dict(position_offset=2 ** 31 - 8 + 1), "INVALID_ARGUMENT"), (dict(positions=16, positions_stride=-1), "INVALID_ARGUMENT"),
     (dict(q=24), "MISALIGNED"), (dict(q_strides=(4096, 512, 68)), "MISALIGNED"), (dict(k_out_strides=(0, -64, 64)), "INVALID_ARGUMENT"),
     (dict(q_strides=(4096, 64, 256)), "INVALID_ARGUMENT"), (dict(k_out_strides=(4096, 64, 128)), "INVALID_ARGUMENT"),   # in place, elsewhere
-    (dict(num_q_heads=2 ** 30, num_kv_heads=2 ** 30), "INVALID_ARGUMENT"),
+    (dict(num_q_heads=2 ** 30, num_kv_heads=2 ** 30), "INVALID_ARGUMENT"), (dict(seq_len=2 ** 31 - 1), "INVALID_ARGUMENT"),
 ])
 def test_rope_refusals(fa, change, code):
     assert _rope(fa, **change) == getattr(fa, "FA_ERR_" + code)
