@@ -650,7 +650,7 @@ FA_EXPORT int fa_decode_gqa_default_splits(int batch_size, int num_kv_heads, int
 
 FA_EXPORT int fa_decode_gqa(const fa_decode_gqa_args* a) { return fa::decode_gqa(a, nullptr); }
 
-int fa::decode_gqa(const fa_decode_gqa_args* a, const float* score_factor) {
+int fa::decode_gqa(const fa_decode_gqa_args* a, const float* row_factor) {
     if (!a || !a->q || !a->k || !a->v || !a->o) return FA_ERR_INVALID_ARGUMENT;
     if (a->batch_size <= 0 || a->num_q_heads <= 0 || a->num_kv_heads <= 0 || a->seq_len_kv <= 0)
         return FA_ERR_INVALID_ARGUMENT;
@@ -722,7 +722,7 @@ int fa::decode_gqa(const fa_decode_gqa_args* a, const float* score_factor) {
     g.seq_lens = a->seq_lens;
     g.block_table = a->block_table; g.table_stride = a->block_table_stride;
     g.page_size = paged ? a->page_size : 0; g.n_pages = a->num_pages; g.page_stride = a->kv_page_stride;
-    g.q_scale = e4m3 ? a->q_scale : score_factor; g.k_scale = a->k_scale; g.v_scale = a->v_scale;
+    g.q_scale = e4m3 ? a->q_scale : row_factor; g.k_scale = a->k_scale; g.v_scale = a->v_scale;
     g.scale = a->scale; g.stream = stream;
     int rc = launch_decode_gqa(g, st);
     if (rc != FA_OK) return rc;

@@ -893,40 +893,32 @@ __global__ void __launch_bounds__(1024) u4_merge_kernel(const __grid_constant__ 
 }
 
 // ------------------------------------------------------------------------------------------ many tokens
-// bf16 q as fp16 for the 16-bit kernel: a power of two for each (sequence, KV head) puts its largest element at 2^14 .. 2^15 and
-// goes back into the scores' scale, as in u4_kernel.  `top`: the largest element's bits (a maximum, so in any order the same).
-__global__ void __launch_bounds__(256) q_top_kernel(const uint4* q, int* top, int per_head, int hkv, FastDiv by_hkv, FastDiv by_tokens) {
+// bf16 q as fp16 for the 16-bit kernel: a power of two for each row puts its largest element at 2^14 .. 2^15 and goes back
+// into the row's softmax scale, as in u4_kernel.  Of each row: what one row holds (a padded token's garbage, an infinity)
+// must not decide what is left of another.  A row is D / 8 lanes.
+template <int D>
+__global__ void __launch_bounds__(256) q_f16_kernel(const uint4* q, uint4* out, float* factor, long long pieces) {
+    constexpr int LPR = D / 8;
     grid_dependency_wait();
     grid_launch_dependents();
-    // block (sequence and token, KV head): `per_head` 16-byte pieces
-    const int bt = by_hkv.quot(blockIdx.x), h = blockIdx.x - bt * hkv, b = by_tokens.quot(bt);
-    uint32_t m = 0;
-    for (int i = threadIdx.x; i < per_head; i += blockDim.x) {
-        const uint4 u = q[(long long)blockIdx.x * per_head + i];
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const bool live = i < pieces;                              // of whole rows: the lanes of a row agree
+    const uint4 u = live ? q[i] : make_uint4(0, 0, 0, 0);
+    uint32_t w[4] = {u.x, u.y, u.z, u.w}, top = 0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) m = max(m, max(w[j] & 0x7FFFu, (w[j] >> 16) & 0x7FFFu));
-    }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0) atomicMax(top + b * hkv + h, (int)m);
-}
-__global__ void __launch_bounds__(256) q_f16_kernel(const uint4* q, uint4* out, const int* top, float* factor, int per_head, int hkv, FastDiv by_hkv, FastDiv by_tokens) {
-    grid_dependency_wait();
-    grid_launch_dependents();
-    const int bt = by_hkv.quot(blockIdx.x), h = blockIdx.x - bt * hkv, b = by_tokens.quot(bt);
-    const uint32_t e = max((uint32_t)top[b * hkv + h] >> 7, 15u);
+    for (int j = 0; j < 4; j++) top = max(top, max(w[j] & 0x7FFFu, (w[j] >> 16) & 0x7FFFu));
+#pragma unroll
+    for (int o = 1; o < LPR; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (!live) return;
+    const uint32_t e = max(top >> 7, 15u);                     // exponent field of the largest element
     const float up = __uint_as_float((268u - e) << 23);
-    if (threadIdx.x == 0) factor[b * hkv + h] = __uint_as_float((e - 14u) << 23);          // every token writes the same
-    for (int i = threadIdx.x; i < per_head; i += blockDim.x) {
-        const uint4 u = q[(long long)blockIdx.x * per_head + i];
-        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if (i % LPR == 0) factor[i / LPR] = __uint_as_float((e - 14u) << 23);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float2 f = unpack16<true>(w[j]);
-            w[j] = pack16<false>(f.x * up, f.y * up);
-        }
-        out[(long long)blockIdx.x * per_head + i] = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int j = 0; j < 4; j++) {
+        const float2 f = unpack16<true>(w[j]);
+        w[j] = pack16<false>(f.x * up, f.y * up);
     }
+    out[i] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 __global__ void __launch_bounds__(256) f16_to_bf16_kernel(uint4* o, long long n) {
     grid_dependency_wait();
@@ -1041,8 +1033,8 @@ int run_u4_rows(const U4Args& a, const Plan& p, DeviceState* st, cudaStream_t st
 struct ManyPlan {
     int batch;                                // sequences of a copy
     int splits;                               // KV splits of the 16-bit kernel
-    size_t cache, partial, q, factor;         // bytes: K's copy (V's as much), partial results, q in fp16, factors and tops
-    size_t bytes() const { return 2 * cache + partial + q + 2 * factor; }
+    size_t cache, partial, q, factor;         // bytes: K's copy (V's as much), partial results, q in fp16, its rows' factors
+    size_t bytes() const { return 2 * cache + partial + q + factor; }
 };
 bool many_rows(int hq, int hkv, int n_tok, int kv_len) {
     const long long rows = (long long)n_tok * (hq / hkv);
@@ -1058,7 +1050,7 @@ ManyPlan make_many_plan(int batch, int hq, int hkv, int n_tok, int kv_len, int d
     p.splits = fa_decode_gqa_default_splits(p.batch * n_qt, hkv, kv_len);
     p.partial = align256(fa_decode_workspace_bytes(p.batch, n_tok * hq, d_head, p.splits));
     p.q = align256((size_t)batch * n_tok * hq * d_head * 2);
-    p.factor = align256((size_t)batch * hkv * sizeof(float));
+    p.factor = align256((size_t)batch * n_tok * hq * sizeof(float));
     return p;
 }
 
@@ -1068,20 +1060,15 @@ int run_many(const fa_decode_gqa_u4_args* p, int n_tok, DeviceState* st) {
     uint8_t* at = static_cast<uint8_t*>(p->workspace);
     uint8_t *k16 = at, *v16 = k16 + m.cache, *partial = v16 + m.cache, *q16 = partial + m.partial;
     float* factor = reinterpret_cast<float*>(q16 + m.q);
-    int* top = reinterpret_cast<int*>(q16 + m.q + m.factor);
     const bool bf = p->dtype == FA_DTYPE_BF16;
     const size_t row = (size_t)p->num_q_heads * p->d_head;                       // elements of a token
-    const long long blocks = (long long)p->batch_size * n_tok * p->num_kv_heads, pieces = (long long)p->batch_size * n_tok * row / 8;
-    const int per_head = (int)(row / 8 / p->num_kv_heads), hkv = p->num_kv_heads;
-    const FastDiv by_hkv(hkv), by_tokens(n_tok);
+    const long long pieces = (long long)p->batch_size * n_tok * row / 8;         // of 16 bytes: below 2^35, 2^27 blocks of them
+    const int hkv = p->num_kv_heads;
     int rc;
     if (bf) {
-        FA_CUDA_TRY(cudaMemsetAsync(top, 0, (size_t)p->batch_size * hkv * sizeof(int), stream));
-        const uint4* q = static_cast<const uint4*>(p->q);
-        const int threads = per_head >= 256 ? 256 : (per_head + 31) / 32 * 32;
-        if ((rc = launch_dependent(q_top_kernel, (unsigned)blocks, threads, 0, stream, 1, q, top, per_head, hkv, by_hkv, by_tokens)) != FA_OK) return rc;
-        if ((rc = launch_dependent(q_f16_kernel, (unsigned)blocks, threads, 0, stream, 1, q, reinterpret_cast<uint4*>(q16), top, factor, per_head, hkv, by_hkv, by_tokens)) != FA_OK)
-            return rc;
+        auto kernel = p->d_head == 64 ? q_f16_kernel<64> : q_f16_kernel<128>;
+        rc = launch_dependent(kernel, (unsigned)((pieces + 255) / 256), 256, 0, stream, 1, static_cast<const uint4*>(p->q), reinterpret_cast<uint4*>(q16), factor, pieces);
+        if (rc != FA_OK) return rc;
     }
     for (int b0 = 0; b0 < p->batch_size; b0 += m.batch) {
         const int nb = p->batch_size - b0 < m.batch ? p->batch_size - b0 : m.batch;
@@ -1128,7 +1115,7 @@ int run_many(const fa_decode_gqa_u4_args* p, int n_tok, DeviceState* st) {
         g.workspace = partial;
         g.workspace_bytes = m.partial;
         g.stream = p->stream;
-        if ((rc = decode_gqa(&g, bf ? factor + (size_t)b0 * hkv : nullptr)) != FA_OK) return rc;
+        if ((rc = decode_gqa(&g, bf ? factor + (size_t)b0 * n_tok * p->num_q_heads : nullptr)) != FA_OK) return rc;
     }
     if (!bf) return FA_OK;
     const long long want = (pieces + 255) / 256, most = 16ll * st->sm_count;

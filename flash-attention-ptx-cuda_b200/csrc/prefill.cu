@@ -147,13 +147,14 @@ struct GqaDev {
 // head for the tokens from tok0 on.
 struct Item { int q_start, bh, n_kv, t0, split, kv_len, tok0, b, hkv; bool empty; };
 
-// Index of the partial result of tile row r: output row ((batch * n_tok + token) * Hq + query head),
-// then the KV split.
-__device__ __forceinline__ size_t gqa_partial_index(const GqaDev& gq, const Item& it, int r) {
+// Output row of tile row r: (batch * n_tok + token) * Hq + query head.  The index of its partial result: then the KV split.
+__device__ __forceinline__ size_t gqa_row(const GqaDev& gq, const Item& it, int r) {
     const int tl = r / gq.group, g = r - tl * gq.group;
-    const size_t row = (static_cast<size_t>(it.b) * gq.n_tok + it.tok0 + tl) * (gq.n_hkv * gq.group) + it.hkv * gq.group + g;
-    return row * gq.n_splits + it.split;
+    return (static_cast<size_t>(it.b) * gq.n_tok + it.tok0 + tl) * (gq.n_hkv * gq.group) + it.hkv * gq.group + g;
 }
+__device__ __forceinline__ size_t gqa_partial_index(const GqaDev& gq, const Item& it, int r) { return gqa_row(gq, it, r) * gq.n_splits + it.split; }
+// Whether tile row r carries a (token, head) pair.
+__device__ __forceinline__ bool gqa_live(const GqaDev& gq, const Item& it, int r) { return r < gq.live_rows && it.tok0 + r / gq.group < gq.n_tok; }
 
 template <bool CAUSAL, bool GQA, bool GROUPED>
 __device__ __forceinline__ bool get_item(int k, int n_items, int n_bh, int n_qtiles, int seq_len,
@@ -793,7 +794,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 // written here: row-strided stores from registers hold O in TMEM, and with it the next item's
                 // P V, for the time of 128 x 16 scattered 16-byte writes (B=8 Hq=32 Hkv=8 T=Skv=2048 D=128:
                 // 441 us against 412).  Up to 32 live rows one warp's stores are the shorter way.
-                const bool live = r_in_tile < gq.live_rows && it.tok0 + r_in_tile / gq.group < gq.n_tok;
+                const bool live = gqa_live(gq, it, r_in_tile);
                 const size_t pidx = gqa_partial_index(gq, it, r_in_tile);
                 // a token with no visible key (a sequence shorter than the token count): O = 0, LSE = -inf
                 seen = l_run > 0.0f;
@@ -909,7 +910,6 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 const int limit0 = min(it.kv_len, lim0 + row0 / gq.group), limit1 = min(it.kv_len, lim0 + (row0 + 8) / gq.group);
                 float scale_log2 = scale_log2_in;
                 if constexpr (FP8) scale_log2 *= q_scale[it.bh] * k_scale[it.bh];
-                else if (GQA && q_scale != nullptr) scale_log2 *= q_scale[it.bh];
                 const uint64_t scale2 = pack2(scale_log2, scale_log2);
                 float m0 = -1e30f, m1 = -1e30f;           // reference max of this thread's partial sums
                 uint64_t sum0 = pack2(0.0f, 0.0f), sum1 = sum0;
@@ -1073,7 +1073,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                                        : GQA  ? max(0, min(it.kv_len, it.kv_len - gq.n_tok + 1 + it.tok0)) : it.kv_len;
             float scale_log2 = scale_log2_in;
             if constexpr (FP8) scale_log2 *= q_scale[it.bh] * k_scale[it.bh];
-            else if (GQA && q_scale != nullptr) scale_log2 *= q_scale[it.bh];
+            else if (GQA && q_scale != nullptr && gqa_live(gq, it, r_in_tile)) scale_log2 *= q_scale[gqa_row(gq, it, r_in_tile)];
             const uint64_t scale2 = pack2(scale_log2, scale_log2);
             // Running state of THIS thread: the reference max its partial row sum is expressed in.
             // The row's two threads alternate tiles; the max in use travels from tile to tile
@@ -1389,6 +1389,7 @@ int launch_decode_gqa(const GqaLaunch& g, DeviceState* st) {
                                  g.head_stride, bstride, box_cols, box_rows)) != FA_OK) return rc;
     const int tok_per_tile = kBM / g.group < g.n_tok ? kBM / g.group : g.n_tok;
     const bool small = tok_per_tile * g.group <= 16;
+    if (small && !e4m3 && g.q_scale != nullptr) return FA_ERR_UNSUPPORTED;       // factors of rows: for full query tiles only
     const bool bf = g.dtype == FA_DTYPE_BF16;
 #define FA_GQA(DH, BF, F8) (small ? launch_gqa_instance<DH, BF, F8, true>(g, st, tq, tk, tv, to) : launch_gqa_instance<DH, BF, F8, false>(g, st, tq, tk, tv, to))
     if (e4m3) return FA_GQA(128, true, true);

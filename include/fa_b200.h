@@ -498,7 +498,7 @@ int fa_cache_read_u4(const fa_cache_read_args* args);
  * 12 MB of workspace.  Many: fa_decode_gqa's kernel over a copy of K and V in fp16 (so they are
  * rounded once more, as a 16-bit cache of the same values would hold them), up to 256 MB of them or one
  * sequence's at a time, in the workspace; bf16 queries reach it as fp16 times a power of two for each
- * (sequence, KV head).
+ * query row.
  */
 typedef struct fa_decode_gqa_u4_args {
     const void*     q;
