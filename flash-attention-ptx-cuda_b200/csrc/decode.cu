@@ -722,6 +722,7 @@ int fa::decode_gqa(const fa_decode_gqa_args* a, const float* row_factor) {
     g.seq_lens = a->seq_lens;
     g.block_table = a->block_table; g.table_stride = a->block_table_stride;
     g.page_size = paged ? a->page_size : 0; g.n_pages = a->num_pages; g.page_stride = a->kv_page_stride;
+    g.o_dtype = e4m3 || row_factor ? FA_DTYPE_BF16 : a->dtype;
     g.q_scale = e4m3 ? a->q_scale : row_factor; g.k_scale = a->k_scale; g.v_scale = a->v_scale;
     g.scale = a->scale; g.stream = stream;
     int rc = launch_decode_gqa(g, st);
@@ -730,7 +731,7 @@ int fa::decode_gqa(const fa_decode_gqa_args* a, const float* row_factor) {
     CombineOut out;
     out.o = a->o; out.lse = a->lse;
     return launch_combine(o_part, lse_part, splits, a->d_head, (long long)splits * a->d_head, 1, splits,
-                          (int)rows, a->d_head, out, e4m3 ? FA_DTYPE_BF16 : a->dtype, st->sm_count, stream);
+                          (int)rows, a->d_head, out, g.o_dtype, st->sm_count, stream);
 }
 
 FA_EXPORT int fa_combine(const float* o_parts, const float* lse_parts, int n_parts, int rows,

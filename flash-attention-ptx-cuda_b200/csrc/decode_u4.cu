@@ -920,20 +920,6 @@ __global__ void __launch_bounds__(256) q_f16_kernel(const uint4* q, uint4* out, 
     }
     out[i] = make_uint4(w[0], w[1], w[2], w[3]);
 }
-__global__ void __launch_bounds__(256) f16_to_bf16_kernel(uint4* o, long long n) {
-    grid_dependency_wait();
-    grid_launch_dependents();
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const uint4 u = o[i];
-        uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float2 f = unpack16<false>(w[j]);
-            w[j] = pack16<true>(f.x, f.y);
-        }
-        o[i] = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-}
 
 // ------------------------------------------------------------------------------------------ host
 struct Plan {
@@ -1054,6 +1040,7 @@ ManyPlan make_many_plan(int batch, int hq, int hkv, int n_tok, int kv_len, int d
     return p;
 }
 
+// bf16: q goes in as fp16 with a factor a row, O comes out as bf16 from the kernel and its merge, rounded once.
 int run_many(const fa_decode_gqa_u4_args* p, int n_tok, DeviceState* st) {
     const ManyPlan m = make_many_plan(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->d_head);
     cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
@@ -1117,9 +1104,7 @@ int run_many(const fa_decode_gqa_u4_args* p, int n_tok, DeviceState* st) {
         g.stream = p->stream;
         if ((rc = decode_gqa(&g, bf ? factor + (size_t)b0 * n_tok * p->num_q_heads : nullptr)) != FA_OK) return rc;
     }
-    if (!bf) return FA_OK;
-    const long long want = (pieces + 255) / 256, most = 16ll * st->sm_count;
-    return launch_dependent(f16_to_bf16_kernel, (unsigned)(want < most ? want : most), 256, 0, stream, 1, static_cast<uint4*>(p->o), pieces);
+    return FA_OK;
 }
 
 }  // namespace

@@ -126,7 +126,7 @@ struct GqaLaunch {
     const void* q; const void* k; const void* v;
     float* o_part; float* lse_part;           // [row][split][D] and [row][split], row = (b * T + t) * Hq + hq
     void* o_final; float* lse_final;          // the caller's o / lse: written directly when n_splits == 1
-    int batch, n_kv_heads, group, kv_len, d_head, dtype;
+    int batch, n_kv_heads, group, kv_len, d_head, dtype, o_dtype;
     int n_tok;                                // query tokens per sequence (1 = plain decode)
     int n_splits, tiles_per_split;
     long long row_stride, head_stride, batch_stride;   // of the KV cache, in elements
@@ -134,7 +134,7 @@ struct GqaLaunch {
     const int* block_table;                   // paged cache: [batch][table_stride] page numbers, or null
     int table_stride, page_size, n_pages;
     long long page_stride;                    // elements between pages
-    const float* q_scale; const float* k_scale; const float* v_scale;   // e4m3: per (batch, KV head); 16 bits: q_scale a factor per query row, or null
+    const float* q_scale; const float* k_scale; const float* v_scale;   // e4m3: per (batch, KV head); fp16 with bf16 O: q_scale a factor per query row
     float scale;
     cudaStream_t stream;
 };
@@ -147,8 +147,8 @@ int check_layout(const fa_cache_layout& l, int cache, int d_head, int seq_len_kv
 // The kernel of fa_cache_read_u4 with any strides of the outputs (elements).  `live_only`: rows that a sequence does not have
 // are not written.
 int launch_read_u4(const fa_cache_read_args& p, long long o_batch, long long o_row, long long o_head, bool live_only, DeviceState* st);
-// fa_decode_gqa with a factor on the scores of each query row [B, T, Hq] (16-bit types, more than 16 rows a query tile; device, may
-// be null).
+// fa_decode_gqa; with `row_factor` (fp16, more than 16 rows a query tile; device) each query row [B, T, Hq] has a factor on its
+// scores, and O is bf16.
 int decode_gqa(const fa_decode_gqa_args* a, const float* row_factor);
 
 }  // namespace fa

@@ -231,7 +231,9 @@ __device__ __forceinline__ bool get_item(int k, int n_items, int n_bh, int n_qti
 // The Q and K scales fold into the softmax scale, the V scale into the final normalisation;
 // the output is bf16.
 // SMALL (grouped-query decode): at most 16 live rows in a query tile.
-template <int D, bool CAUSAL, bool BF16, bool FP8, bool GQA, bool GROUPED, bool SMALL>
+// OBF: O is bf16.  fp16 operands with bf16 O: a bf16 caller whose queries come in fp16 times a factor for each row, which
+// q_scale holds ([B, T, Hq], grouped-query) and which goes into that row's softmax scale.
+template <int D, bool CAUSAL, bool BF16, bool FP8, bool GQA, bool GROUPED, bool SMALL, bool OBF = BF16>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
@@ -244,6 +246,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     constexpr bool V8 = FP8 && GQA;                       // V arrives as e4m3 and is converted in shared memory
     using L = PrefillSmem<D, FP8, V8, SMALL>;
     static_assert(!SMALL || GQA, "few rows: decode only");
+    constexpr bool ROW_FACTOR = OBF && !BF16;
+    static_assert(!ROW_FACTOR || (GQA && !SMALL), "factors of rows: grouped-query attention of full query tiles");
     constexpr int ROWS = SMALL ? 16 : 128;                // rows with statistics
     constexpr int kRing = (D == 64 && SMALL) ? 8 : 4;     // entries of the Q K^T / P V completion rings
     constexpr int NBOX = L::kNBox, NK = L::NK, NV = L::NV;
@@ -767,7 +771,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                         uint32_t w4[4];
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            w4[e] = pack_16<BF16>(__uint_as_float(oa[g8 * 8 + 2 * e]), __uint_as_float(oa[g8 * 8 + 2 * e + 1]));
+                            w4[e] = pack_16<OBF>(__uint_as_float(oa[g8 * 8 + 2 * e]), __uint_as_float(oa[g8 * 8 + 2 * e + 1]));
                         const int c16 = c * 2 + g8;       // 8-element (16-byte) group index in the row
                         const uint32_t addr = o_s + (c16 >> 3) * L::kBox + r_in_tile * 128 +
                                               (((c16 & 7) ^ (r_in_tile & 7)) << 4);
@@ -824,10 +828,10 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 #pragma unroll
                             for (int e = 0; e < 4; e++)
                                 dst[e] = make_uint4(
-                                    pack_16<BF16>(__uint_as_float(o[8 * e]) * inv_l, __uint_as_float(o[8 * e + 1]) * inv_l),
-                                    pack_16<BF16>(__uint_as_float(o[8 * e + 2]) * inv_l, __uint_as_float(o[8 * e + 3]) * inv_l),
-                                    pack_16<BF16>(__uint_as_float(o[8 * e + 4]) * inv_l, __uint_as_float(o[8 * e + 5]) * inv_l),
-                                    pack_16<BF16>(__uint_as_float(o[8 * e + 6]) * inv_l, __uint_as_float(o[8 * e + 7]) * inv_l));
+                                    pack_16<OBF>(__uint_as_float(o[8 * e]) * inv_l, __uint_as_float(o[8 * e + 1]) * inv_l),
+                                    pack_16<OBF>(__uint_as_float(o[8 * e + 2]) * inv_l, __uint_as_float(o[8 * e + 3]) * inv_l),
+                                    pack_16<OBF>(__uint_as_float(o[8 * e + 4]) * inv_l, __uint_as_float(o[8 * e + 5]) * inv_l),
+                                    pack_16<OBF>(__uint_as_float(o[8 * e + 6]) * inv_l, __uint_as_float(o[8 * e + 7]) * inv_l));
                         } else if (live) {
                             float4* dst = reinterpret_cast<float4*>(gq.o_part + pidx * D + c * 32);
 #pragma unroll
@@ -861,7 +865,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                     uint32_t w[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        w[e] = pack_16<BF16>(__uint_as_float(o[g8 * 8 + 2 * e]) * inv_l,
+                        w[e] = pack_16<OBF>(__uint_as_float(o[g8 * 8 + 2 * e]) * inv_l,
                                              __uint_as_float(o[g8 * 8 + 2 * e + 1]) * inv_l);
                     const int c16 = c * 4 + g8;           // 8-element (16-byte) group index in the row
                     const uint32_t addr = o_s + (c16 >> 3) * L::kBox + r_in_tile * 128 +
@@ -1073,7 +1077,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                                        : GQA  ? max(0, min(it.kv_len, it.kv_len - gq.n_tok + 1 + it.tok0)) : it.kv_len;
             float scale_log2 = scale_log2_in;
             if constexpr (FP8) scale_log2 *= q_scale[it.bh] * k_scale[it.bh];
-            else if (GQA && q_scale != nullptr && gqa_live(gq, it, r_in_tile)) scale_log2 *= q_scale[gqa_row(gq, it, r_in_tile)];
+            if constexpr (ROW_FACTOR)
+                if (gqa_live(gq, it, r_in_tile)) scale_log2 *= q_scale[gqa_row(gq, it, r_in_tile)];
             const uint64_t scale2 = pack2(scale_log2, scale_log2);
             // Running state of THIS thread: the reference max its partial row sum is expressed in.
             // The row's two threads alternate tiles; the max in use travels from tile to tile
@@ -1285,11 +1290,11 @@ int launch_instance(const fa_prefill_args& a, DeviceState* st, const CUtensorMap
                             st->status, order);
 }
 
-template <int D, bool BF16, bool FP8, bool SMALL>
+template <int D, bool BF16, bool FP8, bool SMALL, bool OBF = BF16>
 int launch_gqa_instance(const GqaLaunch& g, DeviceState* st, const CUtensorMap& tq, const CUtensorMap& tk,
                         const CUtensorMap& tv, const CUtensorMap& to) {
     using L = PrefillSmem<D, FP8, FP8, SMALL>;
-    auto kernel = prefill_kernel<D, false, BF16, FP8, true, false, SMALL>;
+    auto kernel = prefill_kernel<D, false, BF16, FP8, true, false, SMALL, OBF>;
     static bool configured[64] = {};
     if (!configured[st->device]) {
         FA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
@@ -1375,7 +1380,7 @@ int launch_decode_gqa(const GqaLaunch& g, DeviceState* st) {
     if ((rc = make_tensor_map_q5(&tq, g.q, g.dtype, g.d_head, g.group, g.n_tok, g.n_kv_heads, g.batch, box_cols)) != FA_OK)
         return rc;
     // O has Q's shape: with one KV split the epilogue stores its tiles through this map
-    if ((rc = make_tensor_map_q5(&to, g.o_final, e4m3 ? FA_DTYPE_BF16 : g.dtype, g.d_head, g.group, g.n_tok, g.n_kv_heads,
+    if ((rc = make_tensor_map_q5(&to, g.o_final, g.o_dtype, g.d_head, g.group, g.n_tok, g.n_kv_heads,
                                  g.batch, 64)) != FA_OK) return rc;
     // dense / strided cache: (d, key, KV head, batch); paged: (d, key in page, KV head, page)
     const bool paged = g.block_table != nullptr;
@@ -1389,7 +1394,11 @@ int launch_decode_gqa(const GqaLaunch& g, DeviceState* st) {
                                  g.head_stride, bstride, box_cols, box_rows)) != FA_OK) return rc;
     const int tok_per_tile = kBM / g.group < g.n_tok ? kBM / g.group : g.n_tok;
     const bool small = tok_per_tile * g.group <= 16;
-    if (small && !e4m3 && g.q_scale != nullptr) return FA_ERR_UNSUPPORTED;       // factors of rows: for full query tiles only
+    if (g.o_dtype == FA_DTYPE_BF16 && g.dtype == FA_DTYPE_F16) {                // factors of rows: for full query tiles only
+        if (small || g.q_scale == nullptr) return FA_ERR_UNSUPPORTED;
+        return g.d_head == 64 ? launch_gqa_instance<64, false, false, false, true>(g, st, tq, tk, tv, to)
+                              : launch_gqa_instance<128, false, false, false, true>(g, st, tq, tk, tv, to);
+    }
     const bool bf = g.dtype == FA_DTYPE_BF16;
 #define FA_GQA(DH, BF, F8) (small ? launch_gqa_instance<DH, BF, F8, true>(g, st, tq, tk, tv, to) : launch_gqa_instance<DH, BF, F8, false>(g, st, tq, tk, tv, to))
     if (e4m3) return FA_GQA(128, true, true);

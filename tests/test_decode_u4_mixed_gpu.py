@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from cache_reference import u4_unpack
-from test_decode_u4_gpu import make, reference, run
+from test_decode_u4_gpu import Cache, make, reference, run
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +76,23 @@ def test_padding_of_a_batch_holds_anything(op, dev, t):
     for i, n in enumerate(lens):
         pad = max(t - n, 0)
         assert not o[i, :pad].any() and torch.isinf(lse[i, :pad]).all()
+
+
+@pytest.mark.parametrize("d,t,skv", [(64, 5, 1024), (64, 40, 1024), (128, 40, 1024), (128, 64, 9000), (64, 48, 20000)])
+def test_results_far_below_fp16(op, dev, d, t, skv):
+    """V of 1e-6 and bf16: O is rounded once, to bf16, also where few keys are split over many CTAs and merged.  All of V^ is
+    positive, so O = sum p V^ carries the relative errors of its terms: V^ is a multiple of 2^-24 and exact in fp16, P is off by 2^-12
+    (below 2^-14 by 2^-25, on a sum of P of 1 and more), and by the scores' error d as in check_rows; then half a step of bf16."""
+    b, hq, hkv = 1, 8, 2
+    g = torch.Generator(device=dev).manual_seed(d + t)
+    q = torch.randn((b, t, hq, d), generator=g, device=dev).bfloat16()
+    k = torch.randn((b, skv, hkv, d), generator=g, device=dev).bfloat16()
+    v = (1e-6 + 1e-6 * torch.rand((b, skv, hkv, d), generator=g, device=dev)).bfloat16()
+    cache = Cache(dev, k, v, [skv])
+    o, lse = run(op, q, cache, 0.05)
+    want, _, _, _ = reference(q, cache, 0.05)
+    kk = u4_unpack(*cache.packed[0][0])
+    dev_s = 0.05 * float(torch.einsum("thgd,hd->thg", q[0].double().abs().view(t, hkv, hq // hkv, d), kk.abs().amax(0)).max()) * (2.0 ** -12 + 2.0 ** -20)
+    terms = 2.0 ** -12 + skv * 2.0 ** -25 + 2.0 ** -18 + float(torch.expm1(torch.tensor(2 * dev_s)))
+    rel = ((o.double() - want).abs() / want).max()
+    assert rel <= (1 + terms) * (1 + 2.0 ** -8) - 1, float(rel)
