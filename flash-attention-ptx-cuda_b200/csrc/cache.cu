@@ -433,9 +433,10 @@ __device__ __forceinline__ uint4 from_u4(uint32_t codes, __half2 param) {
     uint32_t y[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        float a = fmaf(s, (float)((codes >> (8 * i)) & 15u), z), b = fmaf(s, (float)((codes >> (8 * i + 4)) & 15u), z);
-        if constexpr (!BF16) { a = min_nan(a, kU4Max); b = min_nan(b, kU4Max); }    // a scale rounded up: -65504 + 15 * 8736 = 65536
-        y[i] = pack16<BF16>(a, b);
+        const float a = fmaf(s, (float)((codes >> (8 * i)) & 15u), z), b = fmaf(s, (float)((codes >> (8 * i + 4)) & 15u), z);
+        // fp16: at most 65504 at either end (a scale rounded up: -65504 + 15 * 8736 = 65536, and the same with the signs turned)
+        if constexpr (BF16) y[i] = pack16<true>(a, b);
+        else asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(y[i]) : "f"(b), "f"(a));
     }
     return make_uint4(y[0], y[1], y[2], y[3]);
 }

@@ -394,8 +394,9 @@ int fa_rope_inv_freq(const fa_rope_scaling* scaling, int rotary_dim, double* inv
  *
  * FA_CACHE_U4, a cache in 4 bits: two codes to a byte, the even element of the row in the low
  * half; every 64 elements have a pair (scale, offset) of fp16, value = offset + scale * code, code
- * 0..15 (a cache of other origin may have scales of either sign).  4.5 bits an element.  The pairs of a row are contiguous (d_head / 64 of them); the
- * param strides count pairs and are multiples of d_head / 64.  What fa_cache_append stores, with
+ * 0..15 (a cache of other origin may have scales of either sign; its values past +-65504 count as +-65504 where they become
+ * fp16: rows read in f16, and attention of many query rows).  4.5 bits an element.  The pairs of a row are
+ * contiguous (d_head / 64 of them); the param strides count pairs and are multiples of d_head / 64.  What fa_cache_append stores, with
  * x the 16-bit element (clamped to +-65504, a NaN makes its 64 elements NaN):
  *     offset = fp16(min x), scale = fp16((max x - offset) / 15),
  *     code = round((x - offset) * (1 / scale)) in 0..15, ties to even (0 where scale = 0)
@@ -462,7 +463,7 @@ int fa_cache_append(const fa_cache_append_args* args);
 
 /*
  * fa_cache_read_u4: num_rows rows of each sequence from a 4-bit cache as 16-bit values,
- * offset + scale * code rounded once (f16: at most 65504).  k_out, v_out: [B, num_rows, Hkv, D] dense in `dtype`; row n is the
+ * offset + scale * code rounded once (f16: to at most +-65504).  k_out, v_out: [B, num_rows, Hkv, D] dense in `dtype`; row n is the
  * cache's row first_rows[b] + n (device [B]; NULL = 0), zero where the sequence has no such row.
  * For a prefix that the 16-bit entry points take, a cache that moves, or a check.
  */
