@@ -300,7 +300,7 @@ def rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, positions: to
     ``torch.ops.fa_b200.rope`` is the same; plain tensors in eager mode go to the kernel without the dispatcher, whose
     20 us a call (50 with a gradient) a short prompt would feel."""
     if (type(q) in _PLAIN and type(k) in _PLAIN and not torch.compiler.is_compiling() and not is_in_torch_dispatch_mode()
-            and not torch._C._are_functorch_transforms_active()):
+            and not torch._C._is_tracing() and not torch._C._are_functorch_transforms_active()):
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
             return _Rope.apply(q, k, inv_freq, positions, interleaved, amplitude, inverse)
         return _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse)
