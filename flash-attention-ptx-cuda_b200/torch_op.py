@@ -23,6 +23,7 @@ import contextlib
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.utils._python_dispatch import is_in_torch_dispatch_mode
 
 import fa_b200 as _fa
@@ -256,6 +257,8 @@ def _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse):
 @torch.library.custom_op("fa_b200::rope", mutates_args=())
 def _rope_op(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,
              interleaved: bool = False, amplitude: float = 1.0, inverse: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    if forward_ad._current_level >= 0:                         # a tangent need not be visible down here, and would be lost
+        raise NotImplementedError("fa_b200::rope: the registered operator has no forward-mode derivative; call rope() of this module")
     return _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse)
 
 
@@ -290,6 +293,32 @@ class _Rope(torch.autograd.Function):
         return _rope_backward(ctx, d_q, d_k)
 
 
+class _RopeForwardMode(torch.autograd.Function):
+    """_Rope in the form that forward-mode differentiation takes, at two to three times its host time a call."""
+
+    @staticmethod
+    def forward(q, k, inv_freq, positions, interleaved, amplitude, inverse):
+        return _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _rope_setup_context(ctx, inputs, output)
+        ctx.save_for_forward(inputs[2], inputs[3])
+        ctx.zeros = inputs[0].new_zeros, inputs[0].shape, inputs[1].shape
+
+    @staticmethod
+    def backward(ctx, d_q, d_k):
+        return _rope_backward(ctx, d_q, d_k)
+
+    @staticmethod
+    def jvp(ctx, d_q, d_k, *_):
+        """The map is linear: its tangents are those of its inputs, turned."""
+        zeros, q_shape, k_shape = ctx.zeros
+        d_q, d_k = zeros(q_shape) if d_q is None else d_q, zeros(k_shape) if d_k is None else d_k
+        interleaved, amplitude, back = ctx.how
+        return rope(d_q, d_k, *ctx.saved_tensors, interleaved, amplitude, not back)
+
+
 def rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,
          interleaved: bool = False, amplitude: float = 1.0, inverse: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """Rotary positions (``fa_rope``) of q ``[B, Hq, S, D]`` and k ``[B, Hkv, S, D]`` (any strides; Hkv may be 0).
@@ -298,7 +327,9 @@ def rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, positions: to
     default 0 .. S-1; ``inverse`` turns back.  Returns the rotated (q, k), contiguous.
 
     ``torch.ops.fa_b200.rope`` is the same; plain tensors in eager mode go to the kernel without the dispatcher, whose
-    20 us a call (50 with a gradient) a short prompt would feel."""
+    20 us a call (50 with a gradient) a short prompt would feel; and forward-mode tangents are known here alone."""
+    if forward_ad._current_level >= 0 and not torch.compiler.is_compiling():
+        return _RopeForwardMode.apply(q, k, inv_freq, positions, interleaved, amplitude, inverse)
     if (type(q) in _PLAIN and type(k) in _PLAIN and not torch.compiler.is_compiling() and not is_in_torch_dispatch_mode()
             and not torch._C._is_tracing() and not torch._C._are_functorch_transforms_active()):
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
