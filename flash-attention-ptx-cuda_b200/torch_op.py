@@ -350,6 +350,8 @@ def u4_cache(blocks: int, rows: int, num_kv_heads: int, d_head: int, device="cud
 def _param_strides(p: torch.Tensor, codes: torch.Tensor, d: int) -> tuple[int, int, int]:
     """(block, head, row) strides of the params of a 4-bit cache, in pairs."""
     g = d // 64
+    if p.device != codes.device:
+        raise ValueError("fa_b200: codes and params of a 4-bit cache are on one device")
     if p.dtype != torch.float16 or tuple(p.shape) != (*codes.shape[:3], g, 2):
         raise ValueError("fa_b200: params of a 4-bit cache are float16 [blocks, rows, Hkv, D/64, 2]")
     st = [2 * g if n == 1 else s for n, s in zip(p.shape[:3], p.stride()[:3])]
