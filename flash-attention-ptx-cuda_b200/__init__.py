@@ -431,15 +431,30 @@ def backward(*args, **kw) -> None:
 
 
 def _adr(x) -> int:
-    """Address of a tensor or a ctypes array, or the address given; 0 for None."""
+    """Address of a tensor, or the address given; 0 for None."""
+    if x is None:
+        return 0
+    return x if x.__class__ is int else x.data_ptr()
+
+
+def _host_doubles(x, rotary_dim) -> int:
+    """Address of the rotary_dim / 2 doubles in host memory that the library reads during the call: a tensor's or a ctypes
+    array's, which are checked, or the address given."""
     if x is None:
         return 0
     if x.__class__ is int:
         return x
-    try:
-        return x.data_ptr()
-    except AttributeError:
-        return ctypes.addressof(x)
+    if isinstance(x, ctypes.Array):
+        ok, n, at = x._type_ is ctypes.c_double, len(x), ctypes.addressof(x)
+    elif hasattr(x, "data_ptr"):
+        ok, n, at = x.device.type == "cpu" and x.is_floating_point() and x.element_size() == 8 and x.is_contiguous(), x.numel(), x.data_ptr()
+    else:
+        ok = False
+    if not ok:
+        raise TypeError("fa_b200: frequencies are contiguous doubles in host memory (a tensor, a ctypes array or an address)")
+    if 2 * n < rotary_dim:
+        raise ValueError("fa_b200: fewer frequencies than rotary_dim / 2")
+    return at
 
 
 def rope_inv_freq(rotary_dim, base=10000.0, scaling="plain", factor=1.0, original_length=0.0, slow=0.0, fast=0.0):
@@ -463,7 +478,7 @@ def rope_raw(q, k, q_out, k_out, batch_size, num_q_heads, num_kv_heads, seq_len,
     return (_lib or lib()).fa_rope(_pack_rope(
         _adr(q), _adr(k), _adr(q_out), _adr(k_out), *q_strides, *k_strides, *q_out_strides, *k_out_strides, batch_size,
         num_q_heads, num_kv_heads, seq_len, d_head, DTYPES.get(dtype, dtype), _adr(positions), positions_stride,
-        position_offset, inverse, _adr(inv_freq), rotary_dim, interleaved, amplitude, _stream_handle(stream) or 0))
+        position_offset, inverse, _host_doubles(inv_freq, rotary_dim), rotary_dim, interleaved, amplitude, _stream_handle(stream) or 0))
 
 
 def rope(*args, **kw) -> None:
@@ -489,7 +504,7 @@ def cache_append_raw(k, v, k_cache, v_cache, batch_size, num_tokens, num_kv_head
         _adr(q), _adr(k), _adr(v), _adr(q_out), _adr(k_cache), _adr(v_cache), _adr(k_params), _adr(v_params),
         *token_strides, batch_size, num_tokens, num_q_heads, num_kv_heads, seq_len_kv, d_head, DTYPES.get(dtype, dtype),
         CACHES.get(cache_dtype, cache_dtype), *kv_strides, *param_strides, _adr(block_table), block_table_stride, page_size,
-        num_pages, _adr(seq_lens), _adr(num_new), _adr(positions), _adr(inv_freq), rotary_dim, interleaved, amplitude,
+        num_pages, _adr(seq_lens), _adr(num_new), _adr(positions), _host_doubles(inv_freq, rotary_dim), rotary_dim, interleaved, amplitude,
         _adr(q_scale), _adr(k_scale), _adr(v_scale), _stream_handle(stream) or 0))
 
 

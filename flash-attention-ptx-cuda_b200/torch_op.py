@@ -249,7 +249,7 @@ def _run_rope(q, k, inv_freq, positions, interleaved, amplitude, inverse):
         positions = positions.to(torch.int32).contiguous()
         pos_stride = s if positions.dim() == 2 else 0
     with _on(device):
-        _fa.rope(q, k if hkv else None, q_out, k_out if hkv else None, b, hq, hkv, s, d, inv_freq, 2 * inv_freq.numel(),
+        _fa.rope(q, k if hkv else None, q_out, k_out if hkv else None, b, hq, hkv, s, d, inv_freq.data_ptr(), 2 * inv_freq.numel(),
                  interleaved, amplitude, _DTYPES[dtype], positions, pos_stride, 0, inverse, qs, ks, stream=_stream(device))
     return q_out, k_out
 
@@ -448,7 +448,7 @@ def cache_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: tor
         kw["positions"] = positions.to(device=q.device, dtype=torch.int32).contiguous()
     if inv_freq is not None:
         inv_freq = _inv_freq(inv_freq)
-        kw.update(inv_freq=inv_freq, rotary_dim=2 * inv_freq.numel(), interleaved=interleaved, amplitude=float(amplitude))
+        kw.update(inv_freq=inv_freq.data_ptr(), rotary_dim=2 * inv_freq.numel(), interleaved=interleaved, amplitude=float(amplitude))
     q_out = torch.empty((b, t, hq, d), device=q.device, dtype=k_cache.dtype if e4m3 else q.dtype)
     with _on(q.device):
         _fa.cache_append(tokens[1], tokens[2], k_cache, v_cache, b, t, hkv, skv, d, dtype=_DTYPES[q.dtype],
