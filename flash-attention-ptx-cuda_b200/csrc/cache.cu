@@ -525,6 +525,10 @@ bool strides_ok(const fa_strides& s) { return s.batch >= 0 && s.head >= 0 && s.r
 bool in_place_ok(const void* in, const void* out, const fa_strides& is, const fa_strides& os, int batch, int heads, int seq_len) {
     return in != out || ((batch == 1 || is.batch == os.batch) && (heads == 1 || is.head == os.head) && (seq_len == 1 || is.row == os.row));
 }
+// Results whose rows do not fall together by a stride of 0 (what is read may: an expanded tensor).
+bool rows_apart(const fa_strides& s, int batch, int heads, int seq_len) {
+    return (batch == 1 || s.batch > 0) && (heads == 1 || s.head > 0) && (seq_len == 1 || s.row > 0);
+}
 bool strides_aligned(const fa_strides& s) { return s.batch % 8 == 0 && s.head % 8 == 0 && s.row % 8 == 0; }
 fa_strides or_dense(const fa_strides& s, int heads, int seq_len, int d_head) {
     if (s.batch || s.head || s.row) return s;
@@ -584,6 +588,9 @@ FA_EXPORT int fa_rope(const fa_rope_args* p) {
     if (p->inverse != 0 && p->inverse != 1) return FA_ERR_INVALID_ARGUMENT;
     if (p->positions_stride < 0 || (long long)p->position_offset + p->seq_len - 1 > 0x7FFFFFFFll) return FA_ERR_INVALID_ARGUMENT;
     if (!strides_ok(p->q_strides) || !strides_ok(p->k_strides) || !strides_ok(p->q_out_strides) || !strides_ok(p->k_out_strides))
+        return FA_ERR_INVALID_ARGUMENT;
+    if (!rows_apart(or_dense(p->q_out_strides, p->num_q_heads, p->seq_len, p->d_head), p->batch_size, p->num_q_heads, p->seq_len) ||
+        (p->k && !rows_apart(or_dense(p->k_out_strides, p->num_kv_heads, p->seq_len, p->d_head), p->batch_size, p->num_kv_heads, p->seq_len)))
         return FA_ERR_INVALID_ARGUMENT;
     if (p->d_head != 64 && p->d_head != 128) return FA_ERR_UNSUPPORTED;
     if (p->dtype != FA_DTYPE_F16 && p->dtype != FA_DTYPE_BF16) return FA_ERR_UNSUPPORTED;

@@ -328,7 +328,8 @@ typedef struct fa_rotary {
 } fa_rotary;
 
 /* Offsets in elements of entry (batch, head, row) of a tensor whose last dimension is
- * contiguous; multiples of 8.  All zero = dense [B, H, S, D]. */
+ * contiguous; multiples of 8, not negative.  All zero = dense [B, H, S, D].  A result's stride may be 0 only where
+ * there is one entry (an input may be expanded). */
 typedef struct fa_strides {
     long long batch;
     long long head;
