@@ -454,8 +454,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
                     }
                     u[c] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                sc[n][0] = a.scale_log2 * __shfl_sync(0xffffffffu, down, 8 * t);
-                sc[n][1] = a.scale_log2 * __shfl_sync(0xffffffffu, down, 8 * t + 4);
+                sc[n][0] = row_scale(a.scale_log2, __shfl_sync(0xffffffffu, down, 8 * t));
+                sc[n][1] = row_scale(a.scale_log2, __shfl_sync(0xffffffffu, down, 8 * t + 4));
             } else {
                 sc[n][0] = sc[n][1] = a.scale_log2;
             }

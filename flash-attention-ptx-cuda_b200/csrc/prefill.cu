@@ -1078,7 +1078,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             float scale_log2 = scale_log2_in;
             if constexpr (FP8) scale_log2 *= q_scale[it.bh] * k_scale[it.bh];
             if constexpr (ROW_FACTOR)
-                if (gqa_live(gq, it, r_in_tile)) scale_log2 *= q_scale[gqa_row(gq, it, r_in_tile)];
+                if (gqa_live(gq, it, r_in_tile)) scale_log2 = row_scale(scale_log2, q_scale[gqa_row(gq, it, r_in_tile)]);
             const uint64_t scale2 = pack2(scale_log2, scale_log2);
             // Running state of THIS thread: the reference max its partial row sum is expressed in.
             // The row's two threads alternate tiles; the max in use travels from tile to tile

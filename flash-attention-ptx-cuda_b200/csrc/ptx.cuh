@@ -484,4 +484,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// Softmax scale of a query row that was brought to fp16 by a power of two; `factor` undoes it.  The product of a row of zeros (factor 2^-126)
+// leaves 32 bits with a scale below 2^-24, and 0 times a masked score of -inf is not a number: 2^-126 instead, at which scores of
+// up to 2^39 still weigh the same.
+__device__ __forceinline__ float row_scale(float scale_log2, float factor) { return fmaxf(scale_log2 * factor, 1.17549435e-38f); }
+
 }  // namespace fa

@@ -96,3 +96,16 @@ def test_results_far_below_fp16(op, dev, d, t, skv):
     terms = 2.0 ** -12 + skv * 2.0 ** -25 + 2.0 ** -18 + float(torch.expm1(torch.tensor(2 * dev_s)))
     rel = ((o.double() - want).abs() / want).max()
     assert rel <= (1 + terms) * (1 + 2.0 ** -8) - 1, float(rel)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("scale", [0.125, 1e-9, 1e-30])
+@pytest.mark.parametrize("t", [5, 40])
+def test_queries_of_zeros(op, dev, dtype, scale, t):
+    """Every score is 0 whatever the scale: O is the mean of the V^ that a token sees, LSE the logarithm of their number.  Rows of
+    zeros, of numbers so small that their power of two times the scale leaves 32 bits, and of ordinary ones."""
+    q, cache = make(dev, dtype, 2, t, 8, 2, 600, 64, [600, 514], seed=t)
+    q[:, :, 0::4] = 0
+    q[:, :, 1::4] = 1e-38 if dtype == "bf16" else 6e-8
+    o, lse = run(op, q, cache, scale)
+    check_rows(q, cache, o, lse, scale, torch.ones(q.shape[:3], dtype=torch.bool, device=dev))
