@@ -223,7 +223,7 @@ __device__ __forceinline__ Token token(const AppendArgs& a, int n) {
     r.b = a.by_tokens.quot(n);
     const int t = n - r.b * a.n_tokens;
     r.row = sequence_length(a.seq_lens, r.b, a.seq_len_kv) - a.n_tokens + t;
-    r.live = r.row >= 0 && (a.num_new == nullptr || t >= a.n_tokens - a.num_new[r.b]);
+    r.live = r.row >= 0 && (a.num_new == nullptr || a.n_tokens - t <= a.num_new[r.b]);     // any number: nothing is taken from it
     r.position = a.positions == nullptr ? r.row : a.positions[n];
     return r;
 }
