@@ -9,7 +9,8 @@
 //       = 2^E sum_k [P_k s_kg 2^-E] (c_kd - 8)  +  sum_k P_k (z_kg + 8 s_kg)
 // The sums over d and over k with c run on the tensor core: c - 8 is a whole number, exact in both 16-bit types, q is
 // the caller's 16-bit q, and the bracket is rounded to fp16, the one rounding on the way to O (2^-12 of a term, half
-// a step; 2^E follows the scales so that no bracket leaves fp16).  Everything else is held in 32 bits.
+// a step; 2^E follows the scales of a warp's tile up and down, so that no bracket leaves fp16; beside one whose scale is 2^18 times its
+// own a key of the same tile gets fp16's last digits, 2^-26 of the largest scale at most).  Everything else is held in 32 bits.
 //
 // What bounds it.  With a few query rows a key (T * group) HBM does: 4.5 bits an element.  The codes must be unpacked
 // between memory and tensor core, and the registers are where that costs no second trip through shared memory;
@@ -50,6 +51,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kClusterTiles = 1;               // see make_plan
 constexpr int kManyRows = 96, kManyKeys = 512;    // see many_rows
 constexpr size_t kCopyBytes = 256u << 20;      // of K and V in fp16 at a time
+constexpr float kScaleRange = 0x1p-12f;        // V's scales may fall this far below what 2^E allows before E follows them
 constexpr float kGrow = 8.0f;                  // a running max may be exceeded by this much (in powers of two) before it is raised
 
 struct U4Args {
@@ -495,25 +497,28 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
                 for (int gi = 0; gi < G; gi++) zs[n][gi][c] = 0.0f;
             }
         }
-        float s_limit = 0.0f, s_down = 0.0f;                   // 128 * 2^E, 2^-E of V's scales
+        float s_limit = 0.0f, s_low = 0.0f, s_down = 0.0f;     // V's scales: the largest and least that E is kept for, 2^-E
 
         const int first_hidden = it.len - a.n_tok + a.by_group.quot(row0) + 1;       // first key that the block's first token does not see
         for (int tile = tile0; tile < tile1 && alive; tile++) {
             // this tile's factors: K's scale and offset of code 8 over -72, as it meets q_init; V's offset of code 8, and its scale
             // over 2^E, E such that the largest becomes 16 .. 32 when it is set: with P up to 2^8 and scales up to 2^7 times
-            // 2^E a bracket stays below 2^15
+            // 2^E a bracket stays below 2^15.  Below 2^-14 brackets lose digits, so E comes down again for a tile whose
+            // scales are all far below what it allows (kScaleRange): a row of huge V^ costs its own tile alone.  (The second
+            // vote: B=32 Hkv=8 Skv=16384 126.2 -> 126.6 us with 4 heads a KV head, 125.7 -> 127.0 in bf16, 197 -> 198 with 16 rows.)
             float s_max = 0.0f;
 #pragma unroll
             for (int i = 0; i < KPL; i++)
 #pragma unroll
                 for (int gi = 0; gi < G; gi++) s_max = fmaxf(s_max, fabsf(unpack16<false>(vraw[i][gi]).x));
-            if (__any_sync(0xffffffffu, s_max > s_limit)) {
+            if (__any_sync(0xffffffffu, s_max > s_limit) || (__all_sync(0xffffffffu, s_max < s_low) && __any_sync(0xffffffffu, s_max > 0.0f))) {
 #pragma unroll
                 for (int off = 16; off > 0; off >>= 1) s_max = fmaxf(s_max, __shfl_xor_sync(0xffffffffu, s_max, off));
                 const float down = __uint_as_float(((254u + 4u) << 23) - (__float_as_uint(s_max) & 0x7F800000u));
                 const float ratio = s_down == 0.0f ? 1.0f : down / s_down;
                 s_down = down;
                 s_limit = 128.0f / down;
+                s_low = s_limit * kScaleRange;
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll

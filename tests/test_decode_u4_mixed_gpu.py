@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from cache_reference import u4_unpack
-from test_decode_u4_gpu import Cache, make, reference, run
+from test_decode_u4_gpu import Cache, check, make, reference, run
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,53 @@ def test_queries_of_zeros(op, dev, dtype, scale, t):
     q[:, :, 1::4] = 1e-38 if dtype == "bf16" else 6e-8
     o, lse = run(op, q, cache, scale)
     check_rows(q, cache, o, lse, scale, torch.ones(q.shape[:3], dtype=torch.bool, device=dev))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("t", [1, 3])
+@pytest.mark.parametrize("small", [-6, -11, -15])
+def test_a_v_row_of_no_weight_and_a_huge_scale(op, dev, d, t, small):
+    """One key of V^ up to 65504 whose weight is about 2^-60, between keys of values 2^small.  P times V's scale is rounded to fp16 in
+    units of 2^E with 2^E at most a 16th of the largest scale, so below 2^-14 by 2^-25 of such a unit: times a code of up to 8,
+    at most 2^-26 of the largest scale for each key, on a sum of P of at least sum exp(s - max s).  That beside the file's
+    2^-12 of the terms, as in `check` there."""
+    b, hq, hkv, n = 2, 4, 1, 200
+    g = torch.Generator(device=dev).manual_seed(t)
+    base = torch.randn((d,), generator=g, device=dev).sign()
+    q = (base + 0.3 * torch.randn((b, t, hq, d), generator=g, device=dev)).half()
+    k = torch.randn((b, n, hkv, d), generator=g, device=dev) * 0.7
+    v = torch.rand((b, n, hkv, d), generator=g, device=dev) * 2.0 ** small * 7.5
+    k[:, 70] = -base * 0.5 * (128 / d)
+    v[:, 70, :, ::2], v[:, 70, :, 1::2] = 65504.0, -65504.0
+    cache = Cache(dev, k.half(), v.half(), [n] * b)
+    scale = 0.65
+    o, lse = run(op, q, cache, scale)
+    want, want_l, amount, worst = reference(q, cache, scale)
+    off = 16 * 2.0 ** -23 * 79 * worst + 2.0 ** -22
+    steps = (n // 16 + 16) * 2.0 ** -23
+    for i in range(b):
+        (kc, kp), (vc, vp) = cache.packed[0][i], cache.packed[1][i]
+        s = torch.einsum("thd,nd->thn", q[i].double(), u4_unpack(kc, kp)[:, 0]) * scale
+        see = torch.arange(n, device=dev)[None] <= (n - t + torch.arange(t, device=dev))[:, None]
+        s = s.masked_fill(~see[:, None], float("-inf"))
+        assert (s[..., 70] - torch.logsumexp(s, -1) < -30).all()
+        l = torch.exp(s - s.amax(-1, keepdim=True)).sum(-1)
+        tol = amount[i] * (2.0 ** -12 + 2 * off + steps) + want[i].abs() * 2.0 ** -11 + 2.0 ** -25 + (n * 2.0 ** -26 * float(vp[..., 0].max()) / l)[..., None]
+        assert ((o[i].double() - want[i]).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("d,hq", [(64, 8), (128, 24), (64, 80)])
+def test_a_huge_v_row_costs_its_own_tile_alone(op, dev, d, hq):
+    """Keys 64 .. 127 have weights below 2^-60 and one of them V^ up to 65504; the thousands after it, of values 2^-13, keep every digit
+    within `check`'s bound, which has no absolute term (but O's own half step, 2^-25)."""
+    b, hkv, n = 32, 8, 4000
+    g = torch.Generator(device=dev).manual_seed(d)
+    base = torch.randn((d,), generator=g, device=dev).sign()
+    q = (base + 0.3 * torch.randn((b, 1, hq, d), generator=g, device=dev)).half()
+    k = torch.randn((b, n, hkv, d), generator=g, device=dev) * 0.7
+    v = torch.rand((b, n, hkv, d), generator=g, device=dev) * 2.0 ** -13 * 7.5
+    k[:, 64:128] = -base * 0.5 * (128 / d)
+    v[:, 70, :, ::2], v[:, 70, :, 1::2] = 65504.0, -65504.0
+    cache = Cache(dev, k.half(), v.half(), [n] * b)
+    o, lse = run(op, q, cache, 0.65)
+    check(q, cache, o, lse, 0.65, n)
