@@ -159,3 +159,24 @@ def test_a_huge_v_row_costs_its_own_tile_alone(op, dev, d, hq):
     cache = Cache(dev, k.half(), v.half(), [n] * b)
     o, lse = run(op, q, cache, 0.65)
     check(q, cache, o, lse, 0.65, n)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("t", [3, 40])
+def test_rows_that_are_not_numbers(op, dev, dtype, t):
+    """A NaN in a query, or in a key that a token sees: NaN with few rows; O = 0 and LSE = -inf with many, as fa_decode_gqa has it.
+    Tokens and heads that do not meet it keep every bit."""
+    q, cache = make(dev, dtype, 2, t, 8, 2, 640, 64, seed=2)
+    clean, clean_l = run(op, q, cache, 0.125, lens=False)
+    q[1, 1, 2, 5] = float("nan")
+    kp = cache.tensors[1]
+    kp[0, 639, 1] = float("nan")                               # the last token's own key, KV head 1
+    o, lse = run(op, q, cache, 0.125, lens=False)
+    hit = torch.zeros(q.shape[:3], dtype=torch.bool, device=dev)
+    hit[1, 1, 2] = True
+    hit[0, t - 1, 4:] = True
+    assert torch.equal(o[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_l[~hit])
+    if t == 3:
+        assert o[hit].isnan().all() and lse[hit].isnan().all()
+    else:
+        assert not o[hit].any() and (lse[hit] == float("-inf")).all()
