@@ -44,7 +44,7 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kMaxCluster = 8;                 // portable cluster size
 // Keys of a tile.  The longer one has a third fewer instructions a key besides the products and twice the independent ones
-// to fill a product's latency with (B=32 Hkv=8 Skv=16384: 151 us with 32, 126 with 64); with two columns of 8 rows there are
+// to fill a product's latency with (B=32 Hkv=8 Skv=16384: 149 us with 32, 126 with 64); with two columns of 8 rows there are
 // enough of those, and no registers.
 constexpr int tile_keys(int nt) { return nt == 1 ? 64 : 32; }
 constexpr float kLn2 = 0.6931471805599453f;
@@ -55,7 +55,7 @@ constexpr float kScaleRange = 0x1p-12f;        // V's scales may fall this far b
 constexpr float kGrow = 8.0f;                  // a running max may be exceeded by this much (in powers of two) before it is raised
 
 struct U4Args {
-    CUtensorMap tk, tv;                        // codes: (bytes of a row, rows of a block, KV heads, blocks), boxes of up to 32 rows
+    CUtensorMap tk, tv;                        // codes: (bytes of a row, rows of a block, KV heads, blocks), boxes of a tile's rows or a page's
     const uint16_t* q;
     const __half2 *kp, *vp;
     uint16_t* o;
@@ -213,7 +213,7 @@ __device__ __forceinline__ void store_quad(const U4Args& a, long long row, int d
 }
 
 struct Item {
-    int b, h, rb, len, tiles;      // sequence, KV head, row block, its keys, tiles of 32 of them (at least one)
+    int b, h, rb, len, tiles;      // sequence, KV head, row block, its keys, tiles of them (at least one)
 };
 template <int KEYS>
 __device__ __forceinline__ int tiles_of(int len) { return max(1, (len + KEYS - 1) / KEYS); }
@@ -538,10 +538,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
                     fv[gi] = v.x * s_down;
                     fv[G + gi] = fmaf(8.0f, v.x, v.y);
                 }
-                if (S::Keys >= 32 || lane < S::Keys) {
-                    sts_factors<G>(factors + (i * 32 + lane) * 8 * G, fk);
-                    sts_factors<G>(factors + S::Keys * 8 * G + (i * 32 + lane) * 8 * G, fv);
-                }
+                sts_factors<G>(factors + (i * 32 + lane) * 8 * G, fk);
+                sts_factors<G>(factors + S::Keys * 8 * G + (i * 32 + lane) * 8 * G, fv);
             }
             alive = mbar_wait(full0 + stage * 8, phase, ctl, 1);       // the warp votes
             if (!alive) break;
@@ -1017,10 +1015,12 @@ int run_u4_rows(const U4Args& a, const Plan& p, DeviceState* st, cudaStream_t st
 // Many query rows: the 16-bit kernel (tcgen05) over a copy of the cache in fp16.  mma.sync runs at a quarter of tcgen05's rate,
 // and a block of 16 rows reads and unpacks the whole cache again; the copy costs 4.5 bytes an element once.  (us in a graph, row
 // blocks / copy, f16 D=128 Hkv=8: B=8 Skv=4096 64 rows 61 / 66, 128 rows 109 / 71, 256 rows 203 / 73; B=1 Skv=4096 64 rows 17 / 19,
-// 128 rows 23 / 22, 256 rows 38 / 22; B=1 Skv=512 256 rows 12.3 / 11.7.  Blocks of 32 rows need more registers than
-// there are: 97 and 163 where those of 16 take 61 and 109.)  The copy rounds K^ and V^ to fp16, what a 16-bit cache of the
-// same values would hold: O is off by 4e-4 of its norm where the row blocks' is by 3e-4 and fp16 itself by 2e-4, and the LSE of a row
-// that sees few keys by up to 1e-4, which is why short caches stay with the row blocks.
+// 128 rows 23 / 22, 256 rows 38 / 22.  Blocks of 32 rows need more registers than there are: 97 and 163 where those of 16 take 61
+// and 109.)  The copy rounds K^ and V^ to fp16, what a 16-bit cache of the same values would hold: O is off by 4e-4 of its norm where
+// the row blocks' is by 3e-4 and fp16 itself by 2e-4, and the LSE of a row by up to 1e-4 where it sees few keys, less where it
+// sees many.  That is the price of speed where time grows with the cache.  In caches of fewer than 512 rows it is bounded, so they keep the
+// exact codes, although the copy would be faster there as well (511 rows: B=1 256 query rows 10.5 / 11.8, 2000 54.9 / 15.6; B=8 96
+// 27.8 / 17.0, 2000 239 / 45).  The rule asks for the cache's capacity, which the host knows; the lengths are on the device.
 struct ManyPlan {
     int batch;                                // sequences of a copy
     int splits;                               // KV splits of the 16-bit kernel

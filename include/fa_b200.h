@@ -426,8 +426,8 @@ typedef struct fa_cache_layout {
  *       contiguous, tokens lie token_stride elements apart (multiples of 8, 0 = dense), so that the three
  *       can be parts of one projection's output.
  *   q_out [B, T, Hq, D] dense: rotated q, in `dtype`; for an e4m3 cache its codes, rounded from the
- *       rotated 16-bit value times 1 / q_scale[b * Hkv + kv head].  Zero for tokens that are not
- *       stored.  May be q itself if q is dense and the cache is not e4m3 (refused otherwise).
+ *       rotated 16-bit value times 1 / q_scale[b * Hkv + kv head].  Zero for tokens without a row and those before
+ *       the last num_new[b]; a token whose page does not exist keeps its rotated q.  May be q itself if q is dense and the cache is not e4m3 (refused otherwise).
  *   k rotated and v go into the caches: FA_CACHE_16BIT in `dtype`; FA_CACHE_E4M3 (d_head 128, up to 1024 KV heads) as codes of
  *       the 16-bit value times 1 / {k,v}_scale[b * Hkv + kv head], saturating; FA_CACHE_U4 as above.
  * Everything else in the caches stays as it is.
@@ -502,6 +502,9 @@ int fa_cache_read_u4(const fa_cache_read_args* args);
  * rounded once more, as a 16-bit cache of the same values would hold them), up to 256 MB of them or one
  * sequence's at a time, in the workspace; bf16 queries reach it as fp16 times a power of two for each
  * query row.  There a row whose q or keys hold a NaN yields O = 0, LSE = -inf, as in fa_decode_gqa; with few rows, NaN.
+ *
+ * A caller who wants the codes exact for many tokens too passes them in calls of fewer than 96 rows a KV head, the earlier
+ * ones first (seq_lens says how far each call sees).
  *
  * Either way a row's scores (scale * q . K^) have to stay below 2^24 in magnitude: the maximum is taken off after a product of 32
  * bits.  What one row holds, NaN and infinities too, does not reach another.
