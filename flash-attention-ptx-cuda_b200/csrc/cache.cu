@@ -419,7 +419,7 @@ struct ReadArgs {
     const __half2 *kp, *vp;
     uint16_t *k_out, *v_out;
     long long o_batch, o_row, o_head;                         // elements between the outputs' sequences, rows and heads
-    bool live_only;                                           // rows that a sequence does not have stay as they are, instead of zero
+    long long remainder;                                      // elements from a value to its remainder
     int hkv, seq_len_kv, n_rows, tiles;
     CacheMap map;
     long long block_stride, head_stride, row_stride;          // bytes
@@ -441,10 +441,27 @@ __device__ __forceinline__ uint4 from_u4(uint32_t codes, __half2 param) {
     return make_uint4(y[0], y[1], y[2], y[3]);
 }
 
+// What is left of the values beside their fp16 forms y, in fp16 (2^-22 of a value, at least 2^-25).
+__device__ __forceinline__ uint4 remainder_u4(uint32_t codes, __half2 param, const uint4& y) {
+    const float s = __low2float(param), z = __high2float(param);
+    const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 h = unpack16<false>(w[i]);
+        const float a = fmaf(s, (float)((codes >> (8 * i)) & 15u), z), b = fmaf(s, (float)((codes >> (8 * i + 4)) & 15u), z);
+        // a value past fp16 counts as the largest: nothing is left of it
+        r[i] = pack16<false>(max_nan(min_nan(a, kU4Max), -kU4Max) - h.x, max_nan(min_nan(b, kU4Max), -kU4Max) - h.y);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
 // A block takes kUnroll groups of consecutive rows of one head: the codes and pairs of consecutive rows lie together where the cache
 // is laid out for attention, and what it writes are whole rows either way.  HBM bounds it, by its writes: 4 sequences of 16384 rows,
 // Hkv=8 D=128, 344 MB in 57 us, 6.0 TB/s.
-template <int D, bool BF16>
+// COPY, for attention of many tokens: rows that a sequence does not have stay as they are, instead of zero; REMAINDER: what is left of a
+// value goes a.remainder elements behind it.
+template <int D, bool BF16, bool COPY, bool REMAINDER>
 __global__ void __launch_bounds__(kThreads) read_u4_kernel(const __grid_constant__ ReadArgs a) {
     constexpr int LPR = D / 8, SLOTS = kThreads / LPR;
     const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR;
@@ -479,10 +496,15 @@ __global__ void __launch_bounds__(kThreads) read_u4_kernel(const __grid_constant
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) {
         const int n = (tile * kUnroll + u) * SLOTS + slot;
-        if (n < a.n_rows && (live[u] || !a.live_only)) {
+        if (n < a.n_rows && (live[u] || !COPY)) {
             const long long o = b * a.o_batch + n * a.o_row + h * a.o_head + lane * 8;
-            *reinterpret_cast<uint4*>(a.k_out + o) = from_u4<BF16>(kc[u], kp[u]);
-            *reinterpret_cast<uint4*>(a.v_out + o) = from_u4<BF16>(vc[u], vp[u]);
+            const uint4 k = from_u4<BF16>(kc[u], kp[u]), v = from_u4<BF16>(vc[u], vp[u]);
+            *reinterpret_cast<uint4*>(a.k_out + o) = k;
+            *reinterpret_cast<uint4*>(a.v_out + o) = v;
+            if constexpr (REMAINDER) {
+                *reinterpret_cast<uint4*>(a.k_out + o + a.remainder) = remainder_u4(kc[u], kp[u], k);
+                *reinterpret_cast<uint4*>(a.v_out + o + a.remainder) = remainder_u4(vc[u], vp[u], v);
+            }
         }
     }
 }
@@ -550,6 +572,13 @@ int run_append_to(const AppendArgs& a, int cache, unsigned blocks, cudaStream_t 
     if constexpr (D == 128)
         if (cache == FA_CACHE_E4M3) return run_append<D, BF16, INTER, FA_CACHE_E4M3>(a, blocks, stream);
     return run_append<D, BF16, INTER, FA_CACHE_16BIT>(a, blocks, stream);
+}
+
+template <int D>
+int run_read_u4(const ReadArgs& a, bool bf, bool copy, unsigned blocks, cudaStream_t stream) {
+    auto kernel = !copy ? (bf ? read_u4_kernel<D, true, false, false> : read_u4_kernel<D, false, false, false>)
+                        : a.remainder != 0 ? read_u4_kernel<D, false, true, true> : read_u4_kernel<D, false, true, false>;
+    return launch_dependent(kernel, blocks, kThreads, 0, stream, 1, a);
 }
 
 }  // namespace
@@ -752,8 +781,8 @@ FA_EXPORT int fa_cache_append(const fa_cache_append_args* p) {
               : (inter ? run_append_to<128, false, true>(a, p->cache, blocks, stream) : run_append_to<128, false, false>(a, p->cache, blocks, stream));
 }
 
-// Rows of a 4-bit cache in 16 bits at any strides: fa_cache_read_u4, and the caches that attention of many tokens works on.
-int fa::launch_read_u4(const fa_cache_read_args& p, long long o_batch, long long o_row, long long o_head, bool live_only, DeviceState*) {
+// Rows of a 4-bit cache in 16 bits at any strides: fa_cache_read_u4, and the copies that attention of many tokens works on.
+static int launch_read_u4(const fa_cache_read_args& p, long long o_batch, long long o_row, long long o_head, bool copy, long long remainder) {
     ReadArgs a;
     const int rc = check_layout(p.layout, FA_CACHE_U4, p.d_head, p.seq_len_kv, 0, &a.map);
     if (rc != FA_OK) return rc;
@@ -770,7 +799,7 @@ int fa::launch_read_u4(const fa_cache_read_args& p, long long o_batch, long long
     a.o_batch = o_batch;
     a.o_row = o_row;
     a.o_head = o_head;
-    a.live_only = live_only;
+    a.remainder = remainder;
     a.hkv = p.num_kv_heads;
     a.seq_len_kv = p.seq_len_kv;
     a.n_rows = p.num_rows;
@@ -784,8 +813,12 @@ int fa::launch_read_u4(const fa_cache_read_args& p, long long o_batch, long long
     a.seq_lens = p.layout.seq_lens;
     a.first_rows = p.first_rows;
     const bool bf = p.dtype == FA_DTYPE_BF16;
-    auto kernel = p.d_head == 64 ? (bf ? read_u4_kernel<64, true> : read_u4_kernel<64, false>) : (bf ? read_u4_kernel<128, true> : read_u4_kernel<128, false>);
-    return launch_dependent(kernel, (unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(p.stream), 1, a);
+    if (p.d_head == 64) return run_read_u4<64>(a, bf, copy, (unsigned)blocks, static_cast<cudaStream_t>(p.stream));
+    return run_read_u4<128>(a, bf, copy, (unsigned)blocks, static_cast<cudaStream_t>(p.stream));
+}
+
+int fa::launch_copy_u4(const fa_cache_read_args& p, long long o_batch, long long o_row, long long o_head, long long remainder) {
+    return launch_read_u4(p, o_batch, o_row, o_head, true, remainder);
 }
 
 FA_EXPORT int fa_cache_read_u4(const fa_cache_read_args* p) {
@@ -803,5 +836,5 @@ FA_EXPORT int fa_cache_read_u4(const fa_cache_read_args* p) {
     if (!st) return FA_ERR_CUDA;
     if (st->cc_major != 10) return FA_ERR_NOT_SM100;
     const long long row = (long long)p->num_kv_heads * p->d_head;
-    return launch_read_u4(*p, row * p->num_rows, row, p->d_head, false, st);
+    return launch_read_u4(*p, row * p->num_rows, row, p->d_head, false, 0);
 }

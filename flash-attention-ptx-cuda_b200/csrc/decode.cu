@@ -648,9 +648,9 @@ FA_EXPORT int fa_decode_gqa_default_splits(int batch_size, int num_kv_heads, int
     return gqa_splits(st ? st->sm_count : 148, (long long)batch_size * num_kv_heads, seq_len_kv);
 }
 
-FA_EXPORT int fa_decode_gqa(const fa_decode_gqa_args* a) { return fa::decode_gqa(a, nullptr); }
+FA_EXPORT int fa_decode_gqa(const fa_decode_gqa_args* a) { return fa::decode_gqa(a, nullptr, false); }
 
-int fa::decode_gqa(const fa_decode_gqa_args* a, const float* row_factor) {
+int fa::decode_gqa(const fa_decode_gqa_args* a, const float* row_factor, bool remainders) {
     if (!a || !a->q || !a->k || !a->v || !a->o) return FA_ERR_INVALID_ARGUMENT;
     if (a->batch_size <= 0 || a->num_q_heads <= 0 || a->num_kv_heads <= 0 || a->seq_len_kv <= 0)
         return FA_ERR_INVALID_ARGUMENT;
@@ -724,6 +724,7 @@ int fa::decode_gqa(const fa_decode_gqa_args* a, const float* row_factor) {
     g.page_size = paged ? a->page_size : 0; g.n_pages = a->num_pages; g.page_stride = a->kv_page_stride;
     g.o_dtype = e4m3 || row_factor ? FA_DTYPE_BF16 : a->dtype;
     g.q_scale = e4m3 ? a->q_scale : row_factor; g.k_scale = a->k_scale; g.v_scale = a->v_scale;
+    g.remainders = remainders;
     g.scale = a->scale; g.stream = stream;
     int rc = launch_decode_gqa(g, st);
     if (rc != FA_OK) return rc;

@@ -8,7 +8,7 @@
 //     O = sum_k P_k V^_k  with  V^_k = s_kg (c_kd - 8) + (z_kg + 8 s_kg)
 //       = 2^E sum_k [P_k s_kg 2^-E] (c_kd - 8)  +  sum_k P_k (z_kg + 8 s_kg)
 // The sums over d and over k with c run on the tensor core: c - 8 is a whole number, exact in both 16-bit types, q is
-// the caller's 16-bit q, and the bracket is rounded to fp16, the one rounding on the way to O (2^-12 of a term, half
+// the caller's 16-bit q, and the bracket is rounded to fp16, the one rounding on the way to O (2^-11 of a term, half
 // a step; 2^E follows the scales of a warp's tile up and down, so that no bracket leaves fp16; beside one whose scale is 2^18 times its
 // own a key of the same tile gets fp16's last digits, 2^-26 of the largest scale at most).  Everything else is held in 32 bits.
 //
@@ -49,7 +49,7 @@ constexpr int kMaxCluster = 8;                 // portable cluster size
 constexpr int tile_keys(int nt) { return nt == 1 ? 64 : 32; }
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kClusterTiles = 1;               // see make_plan
-constexpr int kManyRows = 96, kManyKeys = 512;    // see many_rows
+constexpr int kManyRows = 96, kManyRowsF16 = 128, kManyKeys = 512;    // see many_rows
 constexpr size_t kCopyBytes = 256u << 20;      // of K and V in fp16 at a time
 constexpr float kScaleRange = 0x1p-12f;        // V's scales may fall this far below what 2^E allows before E follows them
 constexpr float kGrow = 8.0f;                  // a running max may be exceeded by this much (in powers of two) before it is raised
@@ -1013,41 +1013,57 @@ int run_u4_rows(const U4Args& a, const Plan& p, DeviceState* st, cudaStream_t st
 }
 
 // Many query rows: the 16-bit kernel (tcgen05) over a copy of the cache in fp16.  mma.sync runs at a quarter of tcgen05's rate,
-// and a block of 16 rows reads and unpacks the whole cache again; the copy costs 4.5 bytes an element once.  (us in a graph, row
-// blocks / copy, f16 D=128 Hkv=8: B=8 Skv=4096 64 rows 61 / 66, 128 rows 109 / 71, 256 rows 203 / 73; B=1 Skv=4096 64 rows 17 / 19,
-// 128 rows 23 / 22, 256 rows 38 / 22.  Blocks of 32 rows need more registers than there are: 97 and 163 where those of 16 take 61
-// and 109.)  The copy rounds K^ and V^ to fp16, what a 16-bit cache of the same values would hold: O is off by 4e-4 of its norm where
-// the row blocks' is by 3e-4 and fp16 itself by 2e-4, and the LSE of a row by up to 1e-4 where it sees few keys, less where it
-// sees many.  That is the price of speed where time grows with the cache.  In caches of fewer than 512 rows it is bounded, so they keep the
-// exact codes, although the copy would be faster there as well (511 rows: B=1 256 query rows 10.5 / 11.8, 2000 54.9 / 15.6; B=8 96
-// 27.8 / 17.0, 2000 239 / 45).  The rule asks for the cache's capacity, which the host knows; the lengths are on the device.
+// and a block of 16 rows reads and unpacks the whole cache again; the copy is written once.  For f16 the copy holds K^ and V^ as fp16
+// values and fp16 remainders, and both go through the products (22 bits of them count): rounded to fp16 alone they cost half of
+// the digits that an fp16 O can show (4.1e-4 of its norm off instead of 2.9e-4, of which P and O's own rounding are all), at
+// 290 instead of 459 us for 8 x 512 tokens on 3584 keys, Hq=32 Hkv=8 D=128.  A bf16 O has no such digits (1.7e-3 either way, its LSE off by up to
+// 1e-4 where a row sees few keys): there the values alone go in.
+// From which number of rows, us in a graph, row blocks / copy, Hkv=8: bf16 D=128 B=8 Skv=4096 80 rows 76 / 65, 96 88 / 66, B=1 Skv=4096
+// 80 17.5 / 18.9, 96 26 / 19.5; D=64 B=8 Skv=4096 80 53 / 41, B=1 Skv=4096 80 12.7 / 15.1, 96 19 / 15; f16 D=128 B=8 Skv=4096 96 85 / 106, 128
+// 110 / 108, B=1 Skv=16384 96 49 / 55, 128 60 / 57; D=64 B=8 Skv=4096 80 53 / 55, 96 61 / 55.  (Blocks of 32 rows need more registers than there
+// are: 97 and 163 us where those of 16 take 61 and 109.)  Caches of fewer than 512 rows keep the exact codes in bf16 and one
+// launch in either type, although the copy is faster there with a batch (511 rows, bf16 values: B=1 256 query rows 10.5 / 11.8, 2000 54.9 /
+// 15.6; B=8 96 27.8 / 17.0, 2000 239 / 45): what that costs is bounded.  The rule asks for the cache's capacity, which the host knows;
+// the lengths are on the device.
 struct ManyPlan {
     int batch;                                // sequences of a copy
     int splits;                               // KV splits of the 16-bit kernel
     size_t cache, partial, q, factor;         // bytes: K's copy (V's as much), partial results, q in fp16, its rows' factors
     size_t bytes() const { return 2 * cache + partial + q + factor; }
 };
-bool many_rows(int hq, int hkv, int n_tok, int kv_len) {
+bool many_rows(int hq, int hkv, int n_tok, int kv_len, int d_head, bool bf) {
     const long long rows = (long long)n_tok * (hq / hkv);
-    return rows >= kManyRows && kv_len >= kManyKeys && hq / hkv <= 128;
+    return rows >= (d_head == 128 && !bf ? kManyRowsF16 : kManyRows) && kv_len >= kManyKeys && hq / hkv <= 128;
 }
-ManyPlan make_many_plan(int batch, int hq, int hkv, int n_tok, int kv_len, int d_head) {
+ManyPlan make_many_plan(int batch, int hq, int hkv, int n_tok, int kv_len, int d_head, bool bf) {
     ManyPlan p;
-    const size_t one = (size_t)hkv * kv_len * d_head * 2;
+    const size_t one = (size_t)hkv * kv_len * d_head * 2 * (bf ? 1 : 2);         // f16: values and remainders
     const size_t fit = kCopyBytes / (2 * one);
     p.batch = fit < 1 ? 1 : fit < (size_t)batch ? (int)fit : batch;
     p.cache = align256(one * p.batch);
     const int group = hq / hkv, per_tile = 128 / group < n_tok ? 128 / group : n_tok, n_qt = (n_tok + per_tile - 1) / per_tile;
     p.splits = fa_decode_gqa_default_splits(p.batch * n_qt, hkv, kv_len);
     p.partial = align256(fa_decode_workspace_bytes(p.batch, n_tok * hq, d_head, p.splits));
-    p.q = align256((size_t)batch * n_tok * hq * d_head * 2);
-    p.factor = align256((size_t)batch * n_tok * hq * sizeof(float));
+    p.q = bf ? align256((size_t)batch * n_tok * hq * d_head * 2) : 0;
+    p.factor = bf ? align256((size_t)batch * n_tok * hq * sizeof(float)) : 0;
     return p;
 }
 
-// bf16: q goes in as fp16 with a factor a row, O comes out as bf16 from the kernel and its merge, rounded once.
+// Workspace of a call of either type: the caller is not asked for it.
+size_t workspace_bytes(int batch, int hq, int hkv, int n_tok, int kv_len, int d_head, DeviceState* st) {
+    size_t most = 0;
+    for (const bool bf : {false, true}) {
+        const size_t n = many_rows(hq, hkv, n_tok, kv_len, d_head, bf) ? make_many_plan(batch, hq, hkv, n_tok, kv_len, d_head, bf).bytes()
+                                                                       : make_plan(batch, hq, hkv, n_tok, kv_len, false, d_head, st).bytes;
+        most = n > most ? n : most;
+    }
+    return most;
+}
+
+// f16: values and remainders of K^ and V^.  bf16: q goes in as fp16 with a factor a row, O comes out as bf16 from the kernel and its
+// merge, rounded once.
 int run_many(const fa_decode_gqa_u4_args* p, int n_tok, DeviceState* st) {
-    const ManyPlan m = make_many_plan(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->d_head);
+    const ManyPlan m = make_many_plan(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->d_head, p->dtype == FA_DTYPE_BF16);
     cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
     uint8_t* at = static_cast<uint8_t*>(p->workspace);
     uint8_t *k16 = at, *v16 = k16 + m.cache, *partial = v16 + m.cache, *q16 = partial + m.partial;
@@ -1083,7 +1099,7 @@ int run_many(const fa_decode_gqa_u4_args* p, int n_tok, DeviceState* st) {
         r.dtype = FA_DTYPE_F16;
         r.stream = p->stream;
         const long long head = (long long)p->seq_len_kv * p->d_head;
-        if ((rc = launch_read_u4(r, head * hkv, p->d_head, head, true, st)) != FA_OK) return rc;
+        if ((rc = launch_copy_u4(r, head * hkv, p->d_head, head, bf ? 0 : nb * hkv * head)) != FA_OK) return rc;
         fa_decode_gqa_args g = {};
         const size_t q0 = (size_t)b0 * n_tok * row;
         g.q = bf ? static_cast<const void*>(q16 + 2 * q0) : static_cast<const uint16_t*>(p->q) + q0;
@@ -1107,7 +1123,7 @@ int run_many(const fa_decode_gqa_u4_args* p, int n_tok, DeviceState* st) {
         g.workspace = partial;
         g.workspace_bytes = m.partial;
         g.stream = p->stream;
-        if ((rc = decode_gqa(&g, bf ? factor + (size_t)b0 * n_tok * p->num_q_heads : nullptr)) != FA_OK) return rc;
+        if ((rc = decode_gqa(&g, bf ? factor + (size_t)b0 * n_tok * p->num_q_heads : nullptr, !bf)) != FA_OK) return rc;
     }
     return FA_OK;
 }
@@ -1124,9 +1140,7 @@ FA_EXPORT size_t fa_decode_gqa_u4_workspace_bytes(int batch_size, int num_q_head
     if (d_head != 64 && d_head != 128) return 0;
     DeviceState* st = device_state();
     const int n_tok = num_q_tokens > 0 ? num_q_tokens : 1;
-    if (many_rows(num_q_heads, num_kv_heads, n_tok, seq_len_kv))
-        return make_many_plan(batch_size, num_q_heads, num_kv_heads, n_tok, seq_len_kv, d_head).bytes();
-    return make_plan(batch_size, num_q_heads, num_kv_heads, n_tok, seq_len_kv, false, d_head, st).bytes;
+    return workspace_bytes(batch_size, num_q_heads, num_kv_heads, n_tok, seq_len_kv, d_head, st);
 }
 
 FA_EXPORT int fa_decode_gqa_u4(const fa_decode_gqa_u4_args* p) {
@@ -1148,14 +1162,13 @@ FA_EXPORT int fa_decode_gqa_u4(const fa_decode_gqa_u4_args* p) {
     DeviceState* st = device_state();
     if (!st) return FA_ERR_CUDA;
     if (st->cc_major != 10) return FA_ERR_NOT_SM100;
-    if (many_rows(p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv)) {
-        const size_t need = make_many_plan(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->d_head).bytes();
-        if (!p->workspace || p->workspace_bytes < need || !aligned16(p->workspace)) return FA_ERR_WORKSPACE;
-        return run_many(p, n_tok, st);
-    }
+    const bool many = many_rows(p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->d_head, p->dtype == FA_DTYPE_BF16);
+    const size_t need = workspace_bytes(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->d_head, st);
+    const bool room = p->workspace && p->workspace_bytes >= need && aligned16(p->workspace);
+    if (many) return room ? run_many(p, n_tok, st) : FA_ERR_WORKSPACE;
     const Plan plan = make_plan(p->batch_size, p->num_q_heads, p->num_kv_heads, n_tok, p->seq_len_kv, p->layout.seq_lens != nullptr, p->d_head, st);
     if (plan.tiles > 0x7FFF0000ll) return FA_ERR_INVALID_ARGUMENT;
-    if (!p->workspace || p->workspace_bytes < plan.bytes || !aligned16(p->workspace)) return FA_ERR_WORKSPACE;
+    if (!room) return FA_ERR_WORKSPACE;
     const bool paged = p->layout.block_table != nullptr;
     const int keys = tile_keys(plan.nt), box_rows = paged && p->layout.page_size < keys ? p->layout.page_size : keys;
     for (a.box_shift = 0; (1 << a.box_shift) < box_rows;) a.box_shift++;

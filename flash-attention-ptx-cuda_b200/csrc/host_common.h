@@ -135,6 +135,7 @@ struct GqaLaunch {
     int table_stride, page_size, n_pages;
     long long page_stride;                    // elements between pages
     const float* q_scale; const float* k_scale; const float* v_scale;   // e4m3: per (batch, KV head); fp16 with bf16 O: q_scale a factor per query row
+    bool remainders;                          // fp16: K and V of `batch` further sequences are the remainders of the first ones'
     float scale;
     cudaStream_t stream;
 };
@@ -144,11 +145,11 @@ int launch_decode_gqa(const GqaLaunch& g, DeviceState* st);
 // a 16-bit or e4m3 cache.
 struct CacheMap;
 int check_layout(const fa_cache_layout& l, int cache, int d_head, int seq_len_kv, int elem, CacheMap* map);
-// The kernel of fa_cache_read_u4 with any strides of the outputs (elements).  `live_only`: rows that a sequence does not have
-// are not written.
-int launch_read_u4(const fa_cache_read_args& p, long long o_batch, long long o_row, long long o_head, bool live_only, DeviceState* st);
-// fa_decode_gqa; with `row_factor` (fp16, more than 16 rows a query tile; device) each query row [B, T, Hq] has a factor on its
-// scores, and O is bf16.
-int decode_gqa(const fa_decode_gqa_args* a, const float* row_factor);
+// fa_cache_read_u4 into the copy that attention of many tokens works on: any strides of the outputs (elements), and rows that a sequence
+// does not have are not written.  `remainder` (fp16; 0: none): elements from a value to where its remainder goes.
+int launch_copy_u4(const fa_cache_read_args& p, long long o_batch, long long o_row, long long o_head, long long remainder);
+// fa_decode_gqa of more than 16 rows a query tile in fp16, two ways more.  `row_factor` (device): each query row [B, T, Hq] has a factor
+// on its scores, and O is bf16.  `remainders`: the cache's `batch_size` sequences are followed by as many of remainders.
+int decode_gqa(const fa_decode_gqa_args* a, const float* row_factor, bool remainders);
 
 }  // namespace fa

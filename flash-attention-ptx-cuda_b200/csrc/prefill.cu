@@ -140,6 +140,7 @@ struct GqaDev {
     int table_stride;
     int page_shift;         // log2(page size)
     int ahead;              // SMALL: key tiles loaded ahead, at most the stage counts
+    int n_batch;            // PARTS = 2: sequences, behind which their remainders lie
 };
 
 // Work list: item index -> (query tile, head), heaviest first when causal.  In grouped-query
@@ -233,7 +234,10 @@ __device__ __forceinline__ bool get_item(int k, int n_items, int n_bh, int n_qti
 // SMALL (grouped-query decode): at most 16 live rows in a query tile.
 // OBF: O is bf16.  fp16 operands with bf16 O: a bf16 caller whose queries come in fp16 times a factor for each row, which
 // q_scale holds ([B, T, Hq], grouped-query) and which goes into that row's softmax scale.
-template <int D, bool CAUSAL, bool BF16, bool FP8, bool GQA, bool GROUPED, bool SMALL, bool OBF = BF16>
+// PARTS = 2 (grouped-query, fp16): K and V come as fp16 values and their fp16 remainders, the remainders as further sequences behind
+// the values (gq.n_batch).  A tile passes its stage ring twice, both halves into the same accumulator, so that K and V count with 22
+// bits; a half frees its stage as soon as its products are done, or the next tile's load would wait for the whole tile.
+template <int D, bool CAUSAL, bool BF16, bool FP8, bool GQA, bool GROUPED, bool SMALL, bool OBF = BF16, int PARTS = 1>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
@@ -248,6 +252,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     static_assert(!SMALL || GQA, "few rows: decode only");
     constexpr bool ROW_FACTOR = OBF && !BF16;
     static_assert(!ROW_FACTOR || (GQA && !SMALL), "factors of rows: grouped-query attention of full query tiles");
+    static_assert(PARTS == 1 || (GQA && !SMALL && !BF16 && !FP8), "remainders: fp16, grouped-query, full query tiles");
     constexpr int ROWS = SMALL ? 16 : 128;                // rows with statistics
     constexpr int kRing = (D == 64 && SMALL) ? 8 : 4;     // entries of the Q K^T / P V completion rings
     constexpr int NBOX = L::kNBox, NK = L::NK, NV = L::NV;
@@ -271,6 +276,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bar_qf, bar_qe, bar_ofree[NO], bar_odone[NO];
     __shared__ __align__(8) uint64_t bar_kf[NK], bar_vf[NV];
+    __shared__ __align__(8) uint64_t bar_ke[PARTS > 1 ? NK : 1], bar_ve[PARTS > 1 ? NV : 1];     // a half's products are done
     // completion rings of the two MMA streams: Q K^T / P V of tile g arrive on entry g % kRing
     __shared__ __align__(8) uint64_t bar_qk[kRing], bar_pvd[kRing];
     __shared__ __align__(8) uint64_t bar_pf[kNU];            // P of the tile in score buffer u is in TMEM
@@ -305,6 +311,10 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         }
         for (int i = 0; i < NK; i++) mbar_init(smem_u32(&bar_kf[i]), 1);
         for (int i = 0; i < NV; i++) mbar_init(smem_u32(&bar_vf[i]), V8 ? 128 : 1);
+        if constexpr (PARTS > 1) {
+            for (int i = 0; i < NK; i++) mbar_init(smem_u32(&bar_ke[i]), 1);
+            for (int i = 0; i < NV; i++) mbar_init(smem_u32(&bar_ve[i]), 1);
+        }
         for (int i = 0; i < kRing; i++) { mbar_init(smem_u32(&bar_qk[i]), 1); mbar_init(smem_u32(&bar_pvd[i]), 1); }
         for (int i = 0; i < kNU; i++) mbar_init(smem_u32(&bar_pf[i]), 4);   // one arrival per warp of the owning group
         for (int i = 0; i < L::NV8; i++) {
@@ -353,14 +363,14 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         if (e < 0 || j >= it.n_kv) return -1;
         return gq.block_table[static_cast<size_t>(it.b) * gq.table_stride + e];
     };
-    auto load_cache_tile = [&](uint32_t dst, uint32_t bytes, const CUtensorMap* tm, uint32_t bar, const Item& it, int j, int pages, auto paged) {
+    auto load_cache_tile = [&](uint32_t dst, uint32_t bytes, const CUtensorMap* tm, uint32_t bar, const Item& it, int j, int pages, auto paged, int block) {
         constexpr int NB = FP8 ? 1 : NBOX;            // boxes per tile row: e4m3 rows are one 128-byte box
         constexpr int XS = FP8 ? 128 : 64;            // elements per box row
         const int r0 = (it.t0 + j) * kBN;
         if constexpr (!decltype(paged)::value) {
             if (elect_one()) {
                 mbar_arrive_expect_tx(bar, bytes);
-                for (int bx = 0; bx < NB; bx++) tma_load_4d(dst + bx * L::kBox, tm, bar, bx * XS, r0, it.hkv, it.b);
+                for (int bx = 0; bx < NB; bx++) tma_load_4d(dst + bx * L::kBox, tm, bar, bx * XS, r0, it.hkv, block);
             }
         } else {
             if (elect_one()) mbar_arrive_expect_tx(bar, bytes);
@@ -411,11 +421,20 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 const int sk = g % NK;
                 [[maybe_unused]] const int pages_j = pages;
                 if constexpr (decltype(paged)::value) pages = cache_pages(it, j + 1);
+                if constexpr (PARTS > 1) {
+                    for (int part = 0; part < PARTS; part++) {
+                        const int h = g * PARTS + part, s = h % NK;
+                        if (h >= NK && !mbar_wait(smem_u32(&bar_ke[s]), (h / NK - 1) & 1, ctl, kBarKEmpty)) { ok = false; break; }
+                        load_cache_tile(k_s + s * L::kKBytes, L::kKBytes, &tm_k, smem_u32(&bar_kf[s]), it, j, pages_j, paged, it.b + part * gq.n_batch);
+                    }
+                    if (!ok) break;
+                    continue;
+                }
                 // the slot was last read by Q K^T of tile g - NK
                 const int ak = SMALL && !V8 ? gq.ahead : NK;
                 if (g >= ak && !mbar_wait(smem_u32(&bar_qk[(g - ak) % kRing]), ((g - ak) / kRing) & 1, ctl, kBarKEmpty)) { ok = false; break; }
                 if constexpr (GQA) {
-                    load_cache_tile(k_s + sk * L::kKBytes, L::kKBytes, &tm_k, smem_u32(&bar_kf[sk]), it, j, pages_j, paged);
+                    load_cache_tile(k_s + sk * L::kKBytes, L::kKBytes, &tm_k, smem_u32(&bar_kf[sk]), it, j, pages_j, paged, it.b);
                 } else {
                     if (elect_one()) {
                         mbar_arrive_expect_tx(smem_u32(&bar_kf[sk]), L::kKBytes);
@@ -461,12 +480,17 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                     // e4m3 V lands in its own buffers; warps 12-15 turn it into the fp16 operand.
                     const int s8 = g % L::NV8;
                     if (g >= L::NV8 && !mbar_wait(smem_u32(&bar_v8e[s8]), (g / L::NV8 - 1) & 1, ctl, kBarV8Empty)) { ok = false; break; }
-                    load_cache_tile(v8_s + s8 * L::kV8Bytes, L::kV8Bytes, &tm_v, smem_u32(&bar_v8f[s8]), it, j, pages_j, paged);
+                    load_cache_tile(v8_s + s8 * L::kV8Bytes, L::kV8Bytes, &tm_v, smem_u32(&bar_v8f[s8]), it, j, pages_j, paged, it.b);
                 } else {
-                    const int sv = g % NV;
-                    // the slot was last read by P V of tile g - NV
+                    for (int part = 0; ok && part < PARTS; part++) {
+                    const int h = g * PARTS + part, sv = h % NV;
+                    // the slot was last read by P V of tile g - NV (of a half: by that half's)
                     const int av = SMALL ? gq.ahead : NV;
-                    if (g >= av && !mbar_wait(smem_u32(&bar_pvd[(g - av) % kRing]), ((g - av) / kRing) & 1, ctl, kBarVEmpty)) { ok = false; break; }
+                    if constexpr (PARTS > 1) {
+                        if (h >= NV && !mbar_wait(smem_u32(&bar_ve[sv]), (h / NV - 1) & 1, ctl, kBarVEmpty)) { ok = false; break; }
+                    } else {
+                        if (g >= av && !mbar_wait(smem_u32(&bar_pvd[(g - av) % kRing]), ((g - av) / kRing) & 1, ctl, kBarVEmpty)) { ok = false; break; }
+                    }
                     const uint32_t vdst = v_s + sv * L::kVBytes;
                     if constexpr (GQA) {
                         // Rows of the sequence's last tile past its end are stale cache contents when the
@@ -477,7 +501,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                         const int valid = it.kv_len - (it.t0 + j) * kBN;      // rows of this tile inside the sequence
                         const bool scrub = valid < kBN && (gq.seq_lens != nullptr || gq.block_table != nullptr);
                         const uint32_t full = scrub ? smem_u32(&bar_vraw) : smem_u32(&bar_vf[sv]);
-                        load_cache_tile(vdst, L::kVBytes, &tm_v, full, it, j, pages_j, paged);
+                        load_cache_tile(vdst, L::kVBytes, &tm_v, full, it, j, pages_j, paged, it.b + part * gq.n_batch);
                         if (scrub) {
                             if (!mbar_wait(full, n_scrub & 1, ctl, kBarVFull)) { ok = false; break; }
                             n_scrub++;
@@ -497,6 +521,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                         }
                         __syncwarp();
                     }
+                    }
+                    if (!ok) break;
                 }
             }
         }
@@ -524,6 +550,33 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             if (!get_item<CAUSAL, GQA, GROUPED>(r, n_items, n_bh, n_qtiles, seq_len, gq, it)) continue;
             if (!mbar_wait(smem_u32(&bar_qf), it_n & 1, ctl, kBarQFull)) break;
             for (int j = 0; j < it.n_kv; j++, g++) {
+                if constexpr (PARTS > 1) {
+                    const uint32_t sc = tmem + u * 128;
+                    for (int part = 0; part < PARTS; part++) {
+                        const int h = g * PARTS + part, s = h % NK;
+                        LaneWaits lw;
+                        mbar_wait(lw, smem_u32(&bar_kf[s]), (h / NK) & 1, ctl, kBarKFull);
+                        if (part == 0 && g >= kNU) mbar_wait(lw, smem_u32(&bar_pvd[(g - kNU) % kRing]), ((g - kNU) / kRing) & 1, ctl, kBarSFree);
+                        tc_fence_after();
+                        const uint64_t dk = make_sdesc(k_s + s * L::kKBytes, hi_k);
+                        if (elect_one() && lw.ok) {
+#pragma unroll
+                            for (int kk = 0; kk < D / 16; kk++) {
+                                const uint32_t off = ((kk >> 2) * L::kBox + (kk & 3) * 32) >> 4;
+                                mma_f16_ss(sc, dq + off, dk + off, idesc_qk, (part > 0 || kk > 0) ? 1u : 0u);
+                            }
+                            tc_commit(smem_u32(&bar_ke[s]));
+                            if (part == PARTS - 1) {
+                                tc_commit(smem_u32(&bar_qk[g % kRing]));
+                                if (j == it.n_kv - 1) tc_commit(smem_u32(&bar_qe));
+                            }
+                        }
+                        if (!warp_all(lw.ok)) { ok = false; break; }
+                    }
+                    if (!ok) break;
+                    u = (u == kNU - 1) ? 0 : u + 1;
+                    continue;
+                }
                 const int sk = g % NK;
                 LaneWaits lw;
                 mbar_wait(lw, smem_u32(&bar_kf[sk]), (g / NK) & 1, ctl, kBarKFull);
@@ -604,6 +657,34 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             Item it;
             if (!get_item<CAUSAL, GQA, GROUPED>(r, n_items, n_bh, n_qtiles, seq_len, gq, it)) continue;
             for (int j = 0; j < it.n_kv; j++, g++) {
+                if constexpr (PARTS > 1) {
+                    const uint32_t pc = tmem + u * 128;
+                    for (int part = 0; part < PARTS; part++) {
+                        const int h = g * PARTS + part, s = h % NV;
+                        LaneWaits lw;
+                        mbar_wait(lw, smem_u32(&bar_vf[s]), (h / NV) & 1, ctl, kBarVFull);
+                        if (part == 0) {
+                            mbar_wait(lw, smem_u32(&bar_pf[u]), u_phase, ctl, kBarPFull);
+                            if (j == 0 && it_n > 0) mbar_wait(lw, smem_u32(&bar_ofree[0]), (it_n - 1) & 1, ctl, kBarOFree);
+                        }
+                        tc_fence_after();
+                        const uint64_t dv = make_sdesc(v_s + s * L::kVBytes, hi_v);
+                        if (elect_one() && lw.ok) {
+#pragma unroll
+                            for (int kk = 0; kk < kBN / 16; kk++)
+                                mma_f16_ts(tmem + O_COL, pc + kk * 8, dv + kk * (2048 >> 4), idesc_pv, (j > 0 || part > 0 || kk > 0) ? 1u : 0u);
+                            tc_commit(smem_u32(&bar_ve[s]));
+                            if (part == PARTS - 1) {
+                                tc_commit(smem_u32(&bar_pvd[g % kRing]));
+                                if (j == it.n_kv - 1) tc_commit(smem_u32(&bar_odone[0]));
+                            }
+                        }
+                        if (!warp_all(lw.ok)) { ok = false; break; }
+                    }
+                    if (!ok) break;
+                    if (u == kNU - 1) { u = 0; u_phase ^= 1; } else { u++; }
+                    continue;
+                }
                 const int sv = g % NV;
                 LaneWaits lw;
                 mbar_wait(lw, smem_u32(&bar_vf[sv]), (g / NV) & 1, ctl, kBarVFull);
@@ -1290,11 +1371,11 @@ int launch_instance(const fa_prefill_args& a, DeviceState* st, const CUtensorMap
                             st->status, order);
 }
 
-template <int D, bool BF16, bool FP8, bool SMALL, bool OBF = BF16>
+template <int D, bool BF16, bool FP8, bool SMALL, bool OBF = BF16, int PARTS = 1>
 int launch_gqa_instance(const GqaLaunch& g, DeviceState* st, const CUtensorMap& tq, const CUtensorMap& tk,
                         const CUtensorMap& tv, const CUtensorMap& to) {
     using L = PrefillSmem<D, FP8, FP8, SMALL>;
-    auto kernel = prefill_kernel<D, false, BF16, FP8, true, false, SMALL, OBF>;
+    auto kernel = prefill_kernel<D, false, BF16, FP8, true, false, SMALL, OBF, PARTS>;
     static bool configured[64] = {};
     if (!configured[st->device]) {
         FA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
@@ -1312,7 +1393,7 @@ int launch_gqa_instance(const GqaLaunch& g, DeviceState* st, const CUtensorMap& 
     // they only come from L2 while the whole cache fits there.  B=8 Hkv=8 Skv=4096 D=128, 512 new tokens
     // (134 MB of cache, 16 query tiles): 301 us over all heads, 269 us 8 heads at a time.  A single query
     // tile reads everything once, in any order.
-    const int walk = n_qt > 1 ? heads_per_group(n_bh, g.kv_len, g.d_head, FP8 ? 1 : 2) : n_bh;
+    const int walk = n_qt > 1 ? heads_per_group(n_bh, g.kv_len, g.d_head, FP8 ? 1 : 2 * PARTS) : n_bh;
     // SMALL, 16-bit cache: how many of the stages to use.  All of them where CTAs are left alone with long
     // sequences while the rest have finished: one CTA then gets more of the bandwidth (d_head 128, lengths from
     // 1/16 of Skv up, cold inputs, two thirds / all of the stages: B=16 Hkv=8 Skv=4096 paged 48.1 / 43.9 us, B=32 Hkv=1
@@ -1327,7 +1408,7 @@ int launch_gqa_instance(const GqaLaunch& g, DeviceState* st, const CUtensorMap& 
                     g.tiles_per_split, g.group, g.n_kv_heads,
                     g.n_tok, tok_per_tile, n_qt, tok_per_tile * g.group, walk,
                     FastDiv(g.n_splits), FastDiv((uint32_t)walk * n_qt), FastDiv(walk), FastDiv(last_heads), FastDiv(g.n_kv_heads), g.seq_lens, g.block_table, g.table_stride,
-                    page_shift, ahead};
+                    page_shift, ahead, g.batch};
     return launch_dependent(kernel, grid, kThreads, L::kTotal, g.stream, 1, tq, tk, tv, to, nullptr, g.kv_len, n_bh, 1,
                             (int)n_items, g.scale * kLog2e, g.q_scale, g.k_scale, g.v_scale, st->status, gq);
 }
@@ -1385,7 +1466,7 @@ int launch_decode_gqa(const GqaLaunch& g, DeviceState* st) {
     // dense / strided cache: (d, key, KV head, batch); paged: (d, key in page, KV head, page)
     const bool paged = g.block_table != nullptr;
     const uint64_t rows = paged ? (uint64_t)g.page_size : (uint64_t)g.kv_len;
-    const uint64_t blocks = paged ? (uint64_t)g.n_pages : (uint64_t)g.batch;
+    const uint64_t blocks = paged ? (uint64_t)g.n_pages : (uint64_t)g.batch * (g.remainders ? 2 : 1);
     const uint64_t bstride = paged ? (uint64_t)g.page_stride : (uint64_t)g.batch_stride;
     const uint32_t box_rows = paged && g.page_size < kBN ? (uint32_t)g.page_size : (uint32_t)kBN;
     if ((rc = make_tensor_map_4d(&tk, g.k, g.dtype, g.d_head, rows, g.n_kv_heads, blocks, g.row_stride,
@@ -1394,6 +1475,11 @@ int launch_decode_gqa(const GqaLaunch& g, DeviceState* st) {
                                  g.head_stride, bstride, box_cols, box_rows)) != FA_OK) return rc;
     const int tok_per_tile = kBM / g.group < g.n_tok ? kBM / g.group : g.n_tok;
     const bool small = tok_per_tile * g.group <= 16;
+    if (g.remainders) {
+        if (small || paged || g.dtype != FA_DTYPE_F16 || g.o_dtype != FA_DTYPE_F16) return FA_ERR_UNSUPPORTED;
+        return g.d_head == 64 ? launch_gqa_instance<64, false, false, false, false, 2>(g, st, tq, tk, tv, to)
+                              : launch_gqa_instance<128, false, false, false, false, 2>(g, st, tq, tk, tv, to);
+    }
     if (g.o_dtype == FA_DTYPE_BF16 && g.dtype == FA_DTYPE_F16) {                // factors of rows: for full query tiles only
         if (small || g.q_scale == nullptr) return FA_ERR_UNSUPPORTED;
         return g.d_head == 64 ? launch_gqa_instance<64, false, false, false, true>(g, st, tq, tk, tv, to)

@@ -496,15 +496,13 @@ int fa_cache_read_u4(const fa_cache_read_args* args);
  * fa_decode_gqa_u4_workspace_bytes(...) of the same sizes on the same device; two calls that may
  * run at the same time need one each.
  *
- * Few query rows (T * Hq / Hkv < 96, or fewer than 512 keys): one pass over the codes, which are exact on the tensor core; P times
- * V's scale is rounded to fp16 (2^-12 of a term; up to 2^-26 of the largest scale among 64 neighbouring keys); about 12 MB of
- * workspace.  Many: fa_decode_gqa's kernel over a copy of K and V in fp16 (so they are
- * rounded once more, as a 16-bit cache of the same values would hold them), up to 256 MB of them or one
- * sequence's at a time, in the workspace; bf16 queries reach it as fp16 times a power of two for each
- * query row.  There a row whose q or keys hold a NaN yields O = 0, LSE = -inf, as in fa_decode_gqa; with few rows, NaN.
- *
- * A caller who wants the codes exact for many tokens too passes them in calls of fewer than 96 rows a KV head, the earlier
- * ones first (seq_lens says how far each call sees).
+ * Few query rows (T * Hq / Hkv < 96, f16 with d_head 128 < 128; or fewer than 512 keys): one pass over the codes, which are exact
+ * on the tensor core; P times V's scale is rounded to fp16 (2^-11 of a term; up to 2^-26 of the largest scale among 64 neighbouring
+ * keys); about 12 MB of workspace.  Many: fa_decode_gqa's kernel over a copy of K and V, up to 256 MB of them or one
+ * sequence's at a time, in the workspace.  f16: as fp16 values and remainders, of which 22 bits count.  bf16: as fp16 values (rounded
+ * once more, as a 16-bit cache of the same values would hold them), and queries as fp16 times a power of two for each
+ * query row.  P is rounded to fp16.  There a row whose q or keys hold a NaN yields O = 0, LSE = -inf, as in fa_decode_gqa; with few
+ * rows, NaN.
  *
  * Either way a row's scores (scale * q . K^) have to stay below 2^24 in magnitude: the maximum is taken off after a product of 32
  * bits.  What one row holds, NaN and infinities too, does not reach another.

@@ -15,10 +15,11 @@ def op(fa):
 
 
 def check_rows(q, cache, o, lse, scale, rows):
-    """The query rows that `rows` [B, T, Hq] names, each against 64 bits within a bound of its own.  Many rows go through a copy of
-    the cache in fp16, which rounds V^ and P (2^-12 each) and K^ (2^-12 of its elements); fewer rows round P times V's
-    scale (2^-12 of at most 2 |V^| + |V^|).  A score is off by at most d = scale * sum |q k| (2^-12 + 2^-20), the second for the
-    32-bit sums, so P by exp(+-2d); then O's own rounding."""
+    """The query rows that `rows` [B, T, Hq] names, each against 64 bits within a bound of its own.  A rounding to fp16
+    is off by half a step, finfo.eps / 2 = 2^-11.  Many rows go through a copy of the cache in fp16, which rounds V^ and P (2^-11
+    each) and K^ (2^-11 of its elements), fp16 queries P alone; fewer rows round P times V's scale (2^-11 of at most 2 |V^| + |V^|).
+    A score is off by at most d = scale * sum |q k| (2^-11 + 2^-20), the second for the 32-bit sums, so P by exp(+-2d); then O's
+    own rounding."""
     want, want_l, _, _ = reference(q, cache, scale)
     b, t, hq, d = q.shape
     hkv = cache.tensors[0].shape[2]
@@ -26,9 +27,9 @@ def check_rows(q, cache, o, lse, scale, rows):
         (kc, kp), (vc, vp) = cache.packed[0][i], cache.packed[1][i]
         k, v = u4_unpack(kc, kp), u4_unpack(vc, vp)
         x = q[i].double().abs().view(t, hkv, hq // hkv, d)
-        dev = scale * torch.einsum("thgd,hd->thg", x, k.abs().amax(0)).reshape(t, hq) * (2.0 ** -12 + 2.0 ** -20)
+        dev = scale * torch.einsum("thgd,hd->thg", x, k.abs().amax(0)).reshape(t, hq) * (2.0 ** -11 + 2.0 ** -20)
         top = v.abs().amax(0).repeat_interleave(hq // hkv, 0)[None]
-        tol = top * (3 * 2.0 ** -12 + 2.0 ** -18 + torch.expm1(2 * dev)[..., None]) + want[i].abs() * (torch.finfo(q.dtype).eps / 2 + 2.0 ** -12) + 2.0 ** -24
+        tol = top * (3 * 2.0 ** -11 + 2.0 ** -18 + torch.expm1(2 * dev)[..., None]) + want[i].abs() * (torch.finfo(q.dtype).eps / 2 + 2.0 ** -11) + 2.0 ** -24
         m = rows[i]
         assert bool(m.any())
         assert ((o[i].double() - want[i]).abs() <= tol)[m].all()
@@ -81,7 +82,7 @@ def test_padding_of_a_batch_holds_anything(op, dev, t):
 @pytest.mark.parametrize("d,t,skv", [(64, 5, 1024), (64, 40, 1024), (128, 40, 1024), (128, 64, 9000), (64, 48, 20000)])
 def test_results_far_below_fp16(op, dev, d, t, skv):
     """V of 1e-6 and bf16: O is rounded once, to bf16, also where few keys are split over many CTAs and merged.  All of V^ is
-    positive, so O = sum p V^ carries the relative errors of its terms: V^ is a multiple of 2^-24 and exact in fp16, P is off by 2^-12
+    positive, so O = sum p V^ carries the relative errors of its terms: V^ is a multiple of 2^-24 and exact in fp16, P is off by 2^-11
     (below 2^-14 by 2^-25, on a sum of P of 1 and more), and by the scores' error d as in check_rows; then half a step of bf16."""
     b, hq, hkv = 1, 8, 2
     g = torch.Generator(device=dev).manual_seed(d + t)
@@ -92,8 +93,8 @@ def test_results_far_below_fp16(op, dev, d, t, skv):
     o, lse = run(op, q, cache, 0.05)
     want, _, _, _ = reference(q, cache, 0.05)
     kk = u4_unpack(*cache.packed[0][0])
-    dev_s = 0.05 * float(torch.einsum("thgd,hd->thg", q[0].double().abs().view(t, hkv, hq // hkv, d), kk.abs().amax(0)).max()) * (2.0 ** -12 + 2.0 ** -20)
-    terms = 2.0 ** -12 + skv * 2.0 ** -25 + 2.0 ** -18 + float(torch.expm1(torch.tensor(2 * dev_s)))
+    dev_s = 0.05 * float(torch.einsum("thgd,hd->thg", q[0].double().abs().view(t, hkv, hq // hkv, d), kk.abs().amax(0)).max()) * (2.0 ** -11 + 2.0 ** -20)
+    terms = 2.0 ** -11 + skv * 2.0 ** -25 + 2.0 ** -18 + float(torch.expm1(torch.tensor(2 * dev_s)))
     rel = ((o.double() - want).abs() / want).max()
     assert rel <= (1 + terms) * (1 + 2.0 ** -8) - 1, float(rel)
 
@@ -117,8 +118,8 @@ def test_queries_of_zeros(op, dev, dtype, scale, t):
 def test_a_v_row_of_no_weight_and_a_huge_scale(op, dev, d, t, small):
     """One key of V^ up to 65504 whose weight is about 2^-60, between keys of values 2^small.  P times V's scale is rounded to fp16 in
     units of 2^E with 2^E at most a 16th of the largest scale, so below 2^-14 by 2^-25 of such a unit: times a code of up to 8,
-    at most 2^-26 of the largest scale for each key, on a sum of P of at least sum exp(s - max s).  That beside the file's
-    2^-12 of the terms, as in `check` there."""
+    at most 2^-26 of the largest scale for each key, on a sum of P of at least sum exp(s - max s).  That beside
+    half a step, 2^-11, of the terms."""
     b, hq, hkv, n = 2, 4, 1, 200
     g = torch.Generator(device=dev).manual_seed(t)
     base = torch.randn((d,), generator=g, device=dev).sign()
@@ -140,7 +141,7 @@ def test_a_v_row_of_no_weight_and_a_huge_scale(op, dev, d, t, small):
         s = s.masked_fill(~see[:, None], float("-inf"))
         assert (s[..., 70] - torch.logsumexp(s, -1) < -30).all()
         l = torch.exp(s - s.amax(-1, keepdim=True)).sum(-1)
-        tol = amount[i] * (2.0 ** -12 + 2 * off + steps) + want[i].abs() * 2.0 ** -11 + 2.0 ** -25 + (n * 2.0 ** -26 * float(vp[..., 0].max()) / l)[..., None]
+        tol = amount[i] * (2.0 ** -11 + 2 * off + steps) + want[i].abs() * 2.0 ** -11 + 2.0 ** -25 + (n * 2.0 ** -26 * float(vp[..., 0].max()) / l)[..., None]
         assert ((o[i].double() - want[i]).abs() <= tol).all()
 
 

@@ -41,7 +41,8 @@ def test_read(op, dev, dtype, d):
 @pytest.mark.parametrize("which", ["k", "v"])
 def test_attention_of_many_rows(op, dev, dtype, which):
     """The copy in fp16 holds +-65504 in the place of values past them, and nothing becomes infinite.  K: queries so small that
-    scores stay of order 1.  Bounds: scores are off by d = sum |q k| scale (2^-12 + 2^-20), P by exp(+-2d) and 2^-12, V^ by 2^-12."""
+    scores stay of order 1.  Bounds: scores are off by d = sum |q k| scale (2^-11 + 2^-20), P by exp(+-2d) and 2^-11, V^ by 2^-11 (half steps of
+    fp16)."""
     b, t, hq, hkv, n, d = 1, 40, 8, 2, 640, 64
     kc, kp = _cache(dev, b, n, hkv, d, 3)
     vc, vp = _cache(dev, b, n, hkv, d, 4)
@@ -58,7 +59,7 @@ def test_attention_of_many_rows(op, dev, dtype, which):
     s = s.masked_fill(~see[:, None, None, :], float("-inf"))
     p = torch.softmax(s, -1)
     want = torch.einsum("thgn,nhd->thgd", p, v)
-    off = 0.125 * torch.einsum("thgd,hd->thg", x.abs(), k.abs().amax(0)).max() * (2.0 ** -12 + 2.0 ** -20)
-    tol = torch.einsum("thgn,nhd->thgd", p, v.abs()) * (2.0 ** -11 + 2.0 ** -18 + torch.expm1(2 * off)) + want.abs() * torch.finfo(dtype).eps / 2 + n * 2.0 ** -25 * v.abs().max() + 2.0 ** -25
+    off = 0.125 * torch.einsum("thgd,hd->thg", x.abs(), k.abs().amax(0)).max() * (2.0 ** -11 + 2.0 ** -20)
+    tol = torch.einsum("thgn,nhd->thgd", p, v.abs()) * (2.0 ** -10 + 2.0 ** -18 + torch.expm1(2 * off)) + want.abs() * torch.finfo(dtype).eps / 2 + n * 2.0 ** -25 * v.abs().max() + 2.0 ** -25
     assert ((o[0].double().view_as(want) - want).abs() <= tol).all()
     assert ((lse[0].double().view(t, hkv, -1) - torch.logsumexp(s, -1)).abs() <= off + 2.0 ** -18).all()
