@@ -291,7 +291,7 @@ __device__ __forceinline__ uint32_t to_u4(const uint4& x, __half2* param) {
 
 // A thread keeps to one token and walks its heads, those of q, then k, then v, kAppendUnroll at a time; the next ones are
 // loaded before these are used, the first ones before the block computes its cos and sin.  What bounds it is the chain
-// of loads that a block waits for, one after the other (lengths, page, rows), and then the 150 instructions that 16 bytes of a
+// of loads that a block waits for, one after the other (lengths, page, rows), and then the 165 instructions that 16 bytes of a
 // row cost: small blocks of few tokens, 8 of them an SM (512 tokens to 8 sequences, Hq=32 Hkv=8 D=128, e4m3 / 4-bit with its read
 // back, us in a graph: 256 threads and 8 tokens 22.7 / 29.9, 128 and 2 20.0 / 26.6; one token to 16 sequences 3.3, 2.8; the scales
 // of e4m3 inverted once a block instead of once a row 20.3 -> 19.6).

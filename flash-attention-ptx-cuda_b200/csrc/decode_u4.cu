@@ -50,7 +50,7 @@ constexpr int tile_keys(int nt) { return nt == 1 ? 64 : 32; }
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kClusterTiles = 1;               // see make_plan
 constexpr int kManyRows = 96, kManyRowsF16 = 128, kManyKeys = 512;    // see many_rows
-constexpr size_t kCopyBytes = 256u << 20;      // of K and V in fp16 at a time
+constexpr size_t kCopyBytes = 256u << 20;      // of K and V in fp16 (and their remainders) at a time
 constexpr float kScaleRange = 0x1p-12f;        // V's scales may fall this far below what 2^E allows before E follows them
 constexpr float kGrow = 8.0f;                  // a running max may be exceeded by this much (in powers of two) before it is raised
 
