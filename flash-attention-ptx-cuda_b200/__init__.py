@@ -444,12 +444,12 @@ def _host_doubles(x, rotary_dim) -> int:
         return 0
     if x.__class__ is int:
         return x
-    if isinstance(x, ctypes.Array):
-        ok, n, at = x._type_ is ctypes.c_double, len(x), ctypes.addressof(x)
-    elif hasattr(x, "data_ptr"):
-        ok, n, at = x.device.type == "cpu" and x.is_floating_point() and x.element_size() == 8 and x.is_contiguous(), x.numel(), x.data_ptr()
-    else:
-        ok = False
+    try:
+        ok = x.is_cpu and x.element_size() == 8 and x.is_floating_point() and x.is_contiguous()
+        n, at = x.numel(), x.data_ptr()
+    except AttributeError:
+        ok = isinstance(x, ctypes.Array) and x._type_ is ctypes.c_double
+        n, at = (len(x), ctypes.addressof(x)) if ok else (0, 0)
     if not ok:
         raise TypeError("fa_b200: frequencies are contiguous doubles in host memory (a tensor, a ctypes array or an address)")
     if 2 * n < rotary_dim:
