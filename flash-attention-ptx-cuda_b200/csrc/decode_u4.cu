@@ -25,7 +25,7 @@
 // through the workspace and a second small kernel.  Short jobs are done in one launch instead: a cluster of up to 8 CTAs an
 // item, which merges through distributed shared memory (plan.cluster says when).
 //
-// Measured (f16, 4 query heads a KV head, D = 128, a call in a graph): B=32 Hkv=8 Skv=16384 126 us, 4.8 TB/s (loads alone 104; unpacking K and V
+// Measured (f16, 4 query heads a KV head, D = 128, a call in a graph): B=32 Hkv=8 Skv=16384 127 us, 4.8 TB/s (loads alone 104; unpacking K and V
 // takes the rest: instructions that wait for one another with two warps a scheduler, slots 50 % used); B=16 Skv=4096 21.5; B=1 Skv=2048
 // 7.4; 16 query rows B=32 Skv=16384 198.
 #include <atomic>
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
             // over 2^E, E such that the largest becomes 16 .. 32 when it is set: with P up to 2^8 and scales up to 2^7 times
             // 2^E a bracket stays below 2^15.  Below 2^-14 brackets lose digits, so E comes down again for a tile whose
             // scales are all far below what it allows (kScaleRange): a row of huge V^ costs its own tile alone.  (The second
-            // vote: B=32 Hkv=8 Skv=16384 126.2 -> 126.6 us with 4 heads a KV head, 125.7 -> 127.0 in bf16, 197 -> 198 with 16 rows.)
+            // vote: B=32 Hkv=8 Skv=16384 126.1 -> 127.1 us with 4 heads a KV head, 125.3 -> 126.9 in bf16, 196.7 -> 198.3 with 16 rows.)
             float s_max = 0.0f;
 #pragma unroll
             for (int i = 0; i < KPL; i++)
@@ -514,6 +514,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) u4_kernel(const __grid_constan
             if (__any_sync(0xffffffffu, s_max > s_limit) || (__all_sync(0xffffffffu, s_max < s_low) && __any_sync(0xffffffffu, s_max > 0.0f))) {
 #pragma unroll
                 for (int off = 16; off > 0; off >>= 1) s_max = fmaxf(s_max, __shfl_xor_sync(0xffffffffu, s_max, off));
+                s_max = fminf(s_max, kU4Max);                  // an infinite scale is lost by itself, not by what it does to E
                 const float down = __uint_as_float(((254u + 4u) << 23) - (__float_as_uint(s_max) & 0x7F800000u));
                 const float ratio = s_down == 0.0f ? 1.0f : down / s_down;
                 s_down = down;

@@ -181,3 +181,27 @@ def test_rows_that_are_not_numbers(op, dev, dtype, t):
         assert o[hit].isnan().all() and lse[hit].isnan().all()
     else:
         assert not o[hit].any() and (lse[hit] == float("-inf")).all()
+
+
+@pytest.mark.parametrize("t", [1, 6])
+def test_an_infinite_scale_stays_in_its_64_elements(op, dev, t):
+    """A pair of V (of another origin) whose scale is infinite: its 64 elements are lost, the row's other ones are not."""
+    b, hq, hkv, n, d = 32, 8, 4, 1500, 128
+    q, cache = make(dev, "f16", b, t, hq, hkv, n, d, seed=t)
+    clean, clean_l = run(op, q, cache, 0.0884, lens=False)
+    check(q, cache, clean, clean_l, 0.0884, n)
+    for i in range(b):
+        cache.tensors[3][i, 70 + 20 * i, :, i % 2, 0] = float("inf")
+    o, lse = run(op, q, cache, 0.0884, lens=False)
+    assert torch.equal(lse, clean_l)
+    _, _, amount, _ = reference(q, cache, 0.0884)
+    for i in range(b):
+        other = slice(64, 128) if i % 2 == 0 else slice(0, 64)
+        # both are P times V's scale rounded and O rounded (2^-11 each); and the tile of the infinity, 64 keys, counts in units for a scale of
+        # 65504, 2^-26 of that a key at most, on a sum of P of sum exp(s - max s)
+        k = u4_unpack(*cache.packed[0][i])
+        s = torch.einsum("thgd,nhd->thgn", q[i].double().view(t, hkv, hq // hkv, d), k) * 0.0884
+        l = torch.exp(clean_l[i].double().view(t, hkv, -1) - s.amax(-1)).view(t, hq, 1)
+        tol = 2 * (amount[i] * 2.0 ** -11 + clean[i].double().abs() * 2.0 ** -11) + 64 * 2.0 ** -26 * 65504 / l + 2.0 ** -24
+        assert ((o[i].double() - clean[i].double()).abs() <= tol)[..., other].all()
+        assert not torch.isfinite(o[i, :, :, 64 * (i % 2)]).all()
