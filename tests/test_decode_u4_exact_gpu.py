@@ -104,3 +104,24 @@ def test_small_values(op, dev):
     cache = Cache(dev, k.half(), v.half(), [n])
     o, lse = run(op, q, cache, 0.0884 * 2 ** 8)
     check_f16(q, cache, o, lse, 0.0884 * 2 ** 8)
+
+
+def test_captured_and_replayed(op, dev):
+    """The copy of both halves in a graph: new queries and lengths at replay, the same bits as a direct call."""
+    q, cache = make(dev, "f16", 2, 40, 8, 2, 1100, 128, [1100, 900], page=16, seed=13)
+    lens = torch.tensor(cache.lens, device=dev, dtype=torch.int32)
+    kc, kp, vc, vp = cache.tensors
+    side = torch.cuda.Stream(device=dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        op.decode_gqa_u4(q, kc, kp, vc, vp, 0.0884, lens, cache.table)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = op.decode_gqa_u4(q, kc, kp, vc, vp, 0.0884, lens, cache.table)
+    torch.cuda.synchronize()
+    q.copy_(q.flip(0))
+    lens.copy_(torch.tensor([500, 60], device=dev))
+    graph.replay()
+    torch.cuda.synchronize()
+    want = op.decode_gqa_u4(q, kc, kp, vc, vp, 0.0884, lens, cache.table)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
