@@ -1022,10 +1022,10 @@ int run_u4_rows(const U4Args& a, const Plan& p, DeviceState* st, cudaStream_t st
 // From which number of rows, us in a graph, row blocks / copy, Hkv=8: bf16 D=128 B=8 Skv=4096 80 rows 76 / 65, 96 88 / 66, B=1 Skv=4096
 // 80 17.5 / 18.9, 96 26 / 19.5; D=64 B=8 Skv=4096 80 53 / 41, B=1 Skv=4096 80 12.7 / 15.1, 96 19 / 15; f16 D=128 B=8 Skv=4096 96 85 / 106, 128
 // 110 / 108, B=1 Skv=16384 96 49 / 55, 128 60 / 57; D=64 B=8 Skv=4096 80 53 / 55, 96 61 / 55.  (Blocks of 32 rows need more registers than there
-// are: 97 and 163 us where those of 16 take 61 and 109.)  Caches of fewer than 512 rows keep the exact codes in bf16 and one
-// launch in either type, although the copy is faster there with a batch (511 rows, bf16 values: B=1 256 query rows 10.5 / 11.8, 2000 54.9 /
-// 15.6; B=8 96 27.8 / 17.0, 2000 239 / 45): what that costs is bounded.  The rule asks for the cache's capacity, which the host knows;
-// the lengths are on the device.
+// are: 97 and 163 us where those of 16 take 61 and 109.)  In caches of fewer than 512 rows the copy is
+// faster with a batch too (511 rows, a copy of the values alone: B=1 256 query rows 10.5 / 11.8, 2000 54.9 / 15.6; B=8 96 27.8 / 17.0, 2000
+// 239 / 45), but what the exact codes in one launch cost is bounded there, so they stay.  The rule asks for the cache's capacity,
+// which the host knows; the lengths are on the device.
 struct ManyPlan {
     int batch;                                // sequences of a copy
     int splits;                               // KV splits of the 16-bit kernel

@@ -323,8 +323,8 @@ def rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, positions: to
          interleaved: bool = False, amplitude: float = 1.0, inverse: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """Rotary positions (``fa_rope``) of q ``[B, Hq, S, D]`` and k ``[B, Hkv, S, D]`` (any strides; Hkv may be 0).
 
-    ``inv_freq`` float64 ``[rotary_dim / 2]`` in CPU memory; ``positions`` integer ``[S]`` or ``[B, S]`` on the device,
-    default 0 .. S-1; ``inverse`` turns back.  Returns the rotated (q, k), contiguous.
+    ``inv_freq`` float64 ``[rotary_dim / 2]`` in CPU memory; ``positions`` integer ``[S]`` or ``[B, S]`` on the device
+    (taken as int32), default 0 .. S-1; ``inverse`` turns back.  Returns the rotated (q, k), contiguous.
 
     ``torch.ops.fa_b200.rope`` is the same; plain tensors in eager mode go to the kernel without the dispatcher, whose
     20 us a call (50 with a gradient) a short prompt would feel; and forward-mode tangents are known here alone."""

@@ -61,6 +61,8 @@ def check_f16(q, cache, o, lse, scale):
     (8, 64, 16, 2, 4000, 0, None),                     # several tiles a CTA, several items
     (1, 32, 4, 1, 30000, 16, [29999]),                 # split over the keys, and merged
     (4, 127, 2, 2, 2000, 0, [2000, 1999, 127, 1]),     # a row below the border of d_head 128
+    (2, 1, 128, 1, 700, 0, [700, 3]),                  # one token of a group that fills a query tile
+    (2, 2, 300, 3, 5000, 16, [4999, 2500]),            # a group of 100, split over the keys
 ])
 def test_many_rows(op, dev, d, b, t, hq, hkv, skv, page, lens):
     q, cache = make(dev, "f16", b, t, hq, hkv, skv, d, lens, page, seed=t)

@@ -43,6 +43,8 @@ def check_rows(q, cache, o, lse, scale, rows):
     (1, 24, 8, 2, 1024, 0),             # the smallest number that goes by the copy
     (2, 40, 6, 2, 1030, 16),
     (2, 130, 5, 1, 700, 0),             # several query tiles
+    (2, 1, 128, 1, 700, 0),             # one token of a group that fills a query tile
+    (2, 2, 300, 3, 5000, 16),           # a group of 100, split over the keys
 ])
 def test_rows_of_any_size_side_by_side(op, dev, dtype, d, b, t, hq, hkv, skv, page):
     """Rows of order 1, 1e-3 and 1e12 (fp16: 6e4), and rows that hold a NaN or an infinity, within each KV head, by head and
